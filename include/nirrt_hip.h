@@ -47,8 +47,8 @@ extern "C" {
 #define NIRRT_E_NODEVICE (-4) /* no gfx950 device visible                              */
 #define NIRRT_E_STREAM (-5)   /* random-word stream exhausted inside nirrt_run         */
 #define NIRRT_E_CLOUD (-6)    /* nirrt_run + NIRRT_F_PNG: guidance cloud refresh due (not an error) */
-#define NIRRT_E_LIBM (-7)     /* the restated libm routines left their supported domain (a NaN steer result): the iteration was
-                                 dropped and the run stopped instead of inserting a NaN vertex */
+#define NIRRT_E_LIBM (-7)     /* a NaN steer result (non-finite coordinates, or a question to the host's libm that was not answered within
+                                 20 s): the iteration was dropped and the run stopped instead of inserting a NaN vertex */
 #define NIRRT_E_PARK (-8)     /* nirrt_run with park_limit: the launch ended early because enough trees were waiting for a
                                  guidance-cloud refresh (not an error: resume with the remaining budget) */
 
@@ -204,11 +204,11 @@ int nirrt_set_cloud(nirrt_tree *t, int64_t n, const double *pts, double sample_r
 /* ---- one whole iteration --------------------------------------------------------------------- */
 /* Loop body of RRTStar2D.planning (rrt_star_2d.py:37-55) / IRRTStar2D.planning
  * (irrt_star_2d.py:54-73) given node_rand: nearest -> steer -> edge collision -> insert -> Near ->
- * choose_parent -> rewire [-> InGoalRegion].  Steer runs on the device: 2D with glibc 2.35's atan2 / cos / sin restated
- * (csrc/glibc235_libm.inc: bit-identical to the reference on an x86-64 FMA host with that libm - nirrt_libm_probe lets a caller
- * check its own host), 3D with IEEE operations only; a NaN result ends the call with NIRRT_E_LIBM. */
+ * choose_parent -> rewire [-> InGoalRegion].  Steer runs on the device: 2D with the roundings of the host's atan2 / cos / sin (decided on
+ * the device or asked from the calling thread while it waits: bit-identical to the reference on this host - nirrt_libm_probe lets a
+ * caller check its libm), 3D with IEEE operations only; a NaN result ends the call with NIRRT_E_LIBM. */
 int nirrt_step(nirrt_tree *t, const double *node_rand, uint32_t flags, nirrt_step_result *res);
-/* Same body with the steer done by the caller (for hosts whose libm is not the restated one): nearest_idx from
+/* Same body with the steer done by the caller (for hosts whose libm is further off than the device allows for): nearest_idx from
  * nirrt_nearest, node_new = new_state(node_nearest, node_rand) computed on the host. */
 int nirrt_extend(nirrt_tree *t, int64_t nearest_idx, const double *node_new, uint32_t flags, nirrt_step_result *res);
 

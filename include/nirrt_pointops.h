@@ -97,7 +97,7 @@ int nirrt_fps_f64_batch(const double *pts, int n_clouds, const int *cnt, const i
  * original order.  jobs: HOST array whose pointers are DEVICE addresses; clouds: DEVICE (n_jobs, n_points, 3) f64 out; n_cand /
  * n_out: HOST out (candidates after the filters / points of the cloud).  The caller advances the problem's generator by
  * 2 * (2 or 3) * n_raw words.  The 3D ellipsoid candidates (ellipsoid_point_cloud_sampling_3d, point_cloud_mask_utils_3d.py:
- * 132-200) go through the device's sin / cos: equal to the host's within a few ulp (<= 1e-9 on the coordinates), not bit for bit. */
+ * 132-200) go through sin / cos with the host libm's roundings: bit-equal to the host's. */
 typedef struct nirrt_cloud_job {
     const uint32_t *words;     /* DEVICE */
     const uint8_t *free_tab;   /* DEVICE, 2D: (h + 1) x (w + 1), 1 = the 2 x 2 pixel block around the integer position is free */
@@ -138,12 +138,12 @@ int nirrt_connect_round(const nirrt_connect_job *jobs, int n_jobs, double radius
                         int device_id);
 int nirrt_connect_masks(const nirrt_connect_job *jobs, int n_jobs, double radius, const int32_t *seed_idx, int device_id);
 
-/* The library's restatement of glibc 2.35's atan2 / sin / cos (csrc/glibc235_libm.inc: what math.atan2 / math.cos / math.sin of
- * the reference's new_state, rrt_star_2d.py:67-78, and np.sin / np.cos of irrt_star_3d.py:146-158 resolve to on an x86-64 FMA host
- * with that libm) evaluated ON THE DEVICE for the caller's arguments: fn 0 = atan2(a[i], b[i]), 1 = sin(a[i]), 2 = cos(a[i]);
- * a, b, out HOST f64 (n,).  A caller compares `out` with its own libm bit for bit before trusting the device-side steer / samplers
- * on this host (nirrt_star_amd/_hip.libm_check does, once per process); arguments whose restated path the translator could not
- * express (|x| > 1e8, Inf) return NaN. */
+/* atan2 / sin / cos (what math.atan2 / math.cos / math.sin of the reference's new_state, rrt_star_2d.py:67-78, and np.sin / np.cos of
+ * irrt_star_3d.py:146-158 call) as the steer and the samplers get them: evaluated ON THE DEVICE to ~70 bits, the values whose rounding is
+ * not certain by a call of this host's libm.  fn 0 = atan2(a[i], b[i]), 1 = sin(a[i]), 2 = cos(a[i]); a, b, out HOST f64 (n,).  A caller
+ * compares `out` with its own libm bit for bit before trusting the device-side steer / samplers on this host
+ * (nirrt_star_amd/_hip.libm_check does, once per process): a difference means a libm that is more than 1/2 + 1/32 ulp off.  sin and
+ * cos of |x| > 65536 or Inf return NaN. */
 int nirrt_libm_probe(int32_t fn, int64_t n, const double *a, const double *b, double *out, int device_id);
 
 #ifdef __cplusplus

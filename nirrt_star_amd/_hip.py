@@ -159,12 +159,13 @@ def _run_args():
     return a
 
 
-# ---- does this host's libm compute what the device's restatement computes? ----------------------------------------------------
+# ---- does the device get this host's libm right? --------------------------------------------------------------------------------
 # The reference steers with math.atan2 / math.cos / math.sin (rrt_star_2d.py:67-78) and samples the 3D unit ball with np.sin /
-# np.cos (irrt_star_3d.py:146-158): whatever libm its host has.  The device evaluates glibc 2.35's x86-64 FMA variants, restated
-# (csrc/glibc235_libm.inc).  On a host with another libm / CPU the REFERENCE computes other last bits, and the device-resident
-# loop would no longer be bit-identical to it: the planner classes then default to mode="exact" (steer / sampling with the host's
-# libm between two launches).  Checked once per process, the first time a planner asks (needs a GPU).
+# np.cos (irrt_star_3d.py:146-158): whatever libm its host has.  The device decides these values itself where a libm within
+# 1/2 + 1/32 ulp can only return one double and asks the host's libm otherwise (csrc/glibc235_libm.inc, csrc/nirrt_ask.hpp).  On a host
+# whose libm is further off the device-resident loop would no longer be bit-identical to the reference: the planner classes then
+# default to mode="exact" (steer / sampling with the host's libm between two launches).  Checked once per process, the first time a
+# planner asks (needs a GPU).
 _libm_ok = None
 
 
@@ -201,10 +202,10 @@ def libm_check(device_id=0, n=4096, force=False):
             bad.append("%s: %d of %d" % (name, diff, n))
     _libm_ok = not bad
     if bad:
-        warnings.warn("nirrt_star_amd: this host's libm differs from the one the device code restates (glibc 2.35, x86-64, FMA) - "
+        warnings.warn("nirrt_star_amd: this host's libm differs from what the device expects of one (results within 1/2 + 1/32 ulp) - "
                       + "; ".join(bad) + " arguments give other bits.  The reference itself computes this host's values, so the "
-                      "planner classes now default to mode='exact' (steer and sampling on the host, bit-identical, slower); "
-                      "scripts/libm_port/make_inc.sh regenerates the restatement from another libm.", RuntimeWarning, stacklevel=2)
+                      "planner classes now default to mode='exact' (steer and sampling on the host, bit-identical, slower).",
+                      RuntimeWarning, stacklevel=2)
     return _libm_ok
 
 

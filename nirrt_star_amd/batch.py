@@ -275,8 +275,8 @@ class Guidance:
         self.device_id = device_id
         self.device_clouds = os.environ.get("NIRRT_HOST_CLOUDS", "0") != "1"   # clouds generated on the device (0: the host path of round 2)
         self.device_input = os.environ.get("NIRRT_HOST_INPUT", "0") != "1"     # network input blocks assembled on the device
-        # parity runs: the 3D ellipsoid candidates (mode 3 of nirrt_guidance_clouds) go through the device's sin / cos and equal the
-        # host's only to a few ulp - a candidate ON an obstacle / range boundary can flip.  NIRRT_HOST_ELLIPSOID3D=1 (or
+        # the 3D ellipsoid candidates (mode 3 of nirrt_guidance_clouds) go through sin / cos with the host libm's roundings; on a host
+        # whose libm is beyond the bound the device assumes (_hip.libm_check) NIRRT_HOST_ELLIPSOID3D=1 (or
         # `host_ellipsoid_3d=True`) draws exactly those clouds with numpy / glibc on the host (bit-reproducible, slower).
         self.host_ellipsoid_3d = host_ellipsoid_3d if host_ellipsoid_3d is not None else os.environ.get("NIRRT_HOST_ELLIPSOID3D", "0") == "1"
         self.calls = 0                      # PointNet++ forwards (batched ones count once)

@@ -2228,10 +2228,11 @@ __device__ __forceinline__ double wg_chain_of_new(Lds<NT> &s, const TreeHot &t, 
     return c;
 }
 
-// glibc 2.35's sin / cos / atan2 (the x86-64 FMA variants: what math.sin / math.cos / math.atan2 of the reference's interpreter
-// call on an FMA + AVX2 host), restated instruction by instruction - see csrc/glibc235_libm.inc.  With them the 2D steer is
-// bit-identical to the reference's (rounds 1-4 used the device's own libm: vertices within 1e-9, and on degenerate trees - free
-// straight start-goal segment, hundreds of near-ties per rewiring pass - an ulp was enough to flip a parent now and then).
+// atan2 / sin / cos with the roundings of the host's libm (what math.atan2 / math.cos / math.sin of the reference's interpreter
+// call): evaluated on the device where the rounding is certain, asked from the host where it is not - see csrc/glibc235_libm.inc and
+// csrc/nirrt_ask.hpp.  With them the 2D steer is bit-identical to the reference's (the device library's own sin / cos: vertices within
+// 1e-9, and on degenerate trees - free straight start-goal segment, hundreds of near-ties per rewiring pass - an ulp was enough to flip
+// a parent now and then).
 #define GLIBC_NS glibc235
 #define GLIBC_UNIFORM 1
 #include "glibc235_device.inc"
@@ -2248,9 +2249,9 @@ __device__ __forceinline__ void steer(const TreeHot &t, const double *from, cons
     double dist = hypot_py<D>(d);
     double m = dist < t.step_len ? dist : t.step_len;
     if (D == 2) {
-        const glibc235::v2d cs = glibc235::cos_sin_atan2(d[1], d[0]);
-        out[0] = from[0] + m * cs.x;
-        out[1] = from[1] + m * cs.y;
+        const nirrt_ask::v2d o = glibc235::steer_point(from[0], from[1], d[1], d[0], m);
+        out[0] = o.x;
+        out[1] = o.y;
     } else {
         double dir[3] = {0., 0., 0.};
         if (dist != 0) {
@@ -2491,8 +2492,8 @@ NIRRT_FN __device__ void it_extend()
         res->node_new[0] = node_new[0]; res->node_new[1] = node_new[1]; res->node_new[2] = D == 3 ? node_new[D - 1] : 0.;
     }
     bool collided = wg_collision<D, NT>(s, nearest, node_new, clr);
-    // the restated libm routines return NaN on the paths their translation does not cover (|theta| > 1e8, Inf: unreachable for
-    // atan2's results, but nothing else would notice): no NaN vertex enters the tree - the iteration is dropped and the run ends
+    // a question to the host's libm that nobody answered comes back as NaN (nirrt_ask.hpp), and so does a steer of non-finite
+    // coordinates: no NaN vertex enters the tree - the iteration is dropped and the run ends
     if (D == 2 && !host_steer && (node_new[0] != node_new[0] || node_new[1] != node_new[1])) {   // (a NaN end point collides with nothing)
         collided = true;
         if (tid == 0) t.status = NIRRT_E_LIBM;

@@ -1,6 +1,9 @@
 // nirrt_hip.hip — kernels + C ABI (include/nirrt_hip.h) of libnirrt_hip.so, gfx950 only.
 //
 // Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -fPIC -shared
+#define NIRRT_ASK_DEVICE
+#include "nirrt_ask.hpp"
+#include "nirrt_libm_host.hpp"
 #include "nirrt_device.hpp"
 
 #include <algorithm>
@@ -9,7 +12,10 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <atomic>
 #include <limits>
+#include <mutex>
+#include <new>
 #include <string>
 #include <tuple>
 #include <vector>
@@ -339,6 +345,101 @@ static int sync_check(nirrt_tree *t)
     return NIRRT_OK;
 }
 
+// ---- answering the kernels' questions to the host's libm (nirrt_ask.hpp) ---------------------------------------------------------
+// One box of slots per device, made before the first launch that may ask and kept until the process ends (kernels of other threads
+// may be using it).  Whoever waits for such a launch answers: every thread that waits looks at the same queue, one at a time.
+namespace {
+struct AskBox {
+    nirrt_ask::Slot *req = nullptr, *rep = nullptr;   // pinned, coherent
+    std::atomic<unsigned long long> next{0};          // tickets answered so far
+    std::atomic_flag busy = ATOMIC_FLAG_INIT;
+};
+std::mutex g_ask_mu;
+AskBox *g_ask_boxes[64];
+}
+
+// (the calling thread's current device is `device`)
+static AskBox *ask_box(int device)
+{
+    if (device < 0 || device >= 64) return nullptr;
+    std::lock_guard<std::mutex> hold(g_ask_mu);
+    if (g_ask_boxes[device]) return g_ask_boxes[device];
+    AskBox *b = new (std::nothrow) AskBox;
+    nirrt_ask::Box dev{};
+    const size_t bytes = sizeof(nirrt_ask::Slot) * nirrt_ask::RING;
+    void *d_req = nullptr, *d_rep = nullptr;
+    bool ok = b && hipHostMalloc((void **)&b->req, bytes, hipHostMallocMapped | hipHostMallocCoherent) == hipSuccess &&
+              hipHostMalloc((void **)&b->rep, bytes, hipHostMallocMapped | hipHostMallocCoherent) == hipSuccess &&
+              hipHostGetDevicePointer(&d_req, b->req, 0) == hipSuccess && hipHostGetDevicePointer(&d_rep, b->rep, 0) == hipSuccess &&
+              hipMalloc((void **)&dev.ticket, 256) == hipSuccess;
+    if (ok) {
+        memset((void *)b->req, 0, bytes);
+        memset((void *)b->rep, 0, bytes);
+        dev.req = (nirrt_ask::Slot *)d_req;
+        dev.rep = (nirrt_ask::Slot *)d_rep;
+        const unsigned long long zero = 0;
+        ok = hipMemcpy(dev.ticket, &zero, sizeof(zero), hipMemcpyHostToDevice) == hipSuccess &&
+             hipMemcpyToSymbol(HIP_SYMBOL(nirrt_ask::g_box), &dev, sizeof(dev)) == hipSuccess;
+    }
+    if (!ok) {
+        (void)hipGetLastError();
+        if (b) {
+            if (b->req) (void)hipHostFree(b->req);
+            if (b->rep) (void)hipHostFree(b->rep);
+        }
+        if (dev.ticket) (void)hipFree(dev.ticket);
+        delete b;
+        return nullptr;
+    }
+    return g_ask_boxes[device] = b;
+}
+
+// answers what is waiting (at most a few hundred questions): their number
+static int ask_serve(AskBox *b)
+{
+    if (b->busy.test_and_set(std::memory_order_acquire)) return 0;
+    int n = 0;
+    unsigned long long t = b->next.load(std::memory_order_relaxed);
+    for (; n < 256; n++, t++) {
+        const volatile uint64_t *q = b->req[t % nirrt_ask::RING].w;
+        const uint64_t seq = q[0], fn = q[1], ua = q[2], ub = q[3], chk = q[4];
+        if (seq != t + 1 || chk != nirrt_ask::checksum(seq, fn, ua, ub)) break;
+        double x, y, r0 = 0., r1 = 0.;
+        memcpy(&x, &ua, 8);
+        memcpy(&y, &ub, 8);
+        switch ((int)fn) {
+        case nirrt_ask::FN_STEER: r0 = nirrt_libm_host::p_atan2(x, y); r1 = nirrt_libm_host::p_sin(r0); r0 = nirrt_libm_host::p_cos(r0); break;
+        default: r0 = nirrt_libm_host::p_sin(x); r1 = nirrt_libm_host::p_cos(x); break;
+        }
+        uint64_t u0, u1;
+        memcpy(&u0, &r0, 8);
+        memcpy(&u1, &r1, 8);
+        volatile uint64_t *p = b->rep[t % nirrt_ask::RING].w;
+        p[1] = u0;
+        p[2] = u1;
+        p[4] = nirrt_ask::checksum(seq, u0, u1, 0);
+        p[0] = seq;
+    }
+    b->next.store(t, std::memory_order_relaxed);
+    b->busy.clear(std::memory_order_release);
+    return n;
+}
+
+// hipStreamSynchronize for a stream whose kernels may ask
+static hipError_t ask_wait(AskBox *b, hipStream_t st)
+{
+    if (!b) return hipStreamSynchronize(st);
+    for (unsigned idle = 0;;) {
+        idle = ask_serve(b) ? 0 : idle + 1;
+        if (idle == 1 || idle % 32 == 31) {    // (a launch with open questions has not ended)
+            const hipError_t e = hipStreamQuery(st);
+            if (e != hipErrorNotReady) return e;
+            (void)hipGetLastError();           // ("not ready" is no error of the next call)
+        }
+        __builtin_ia32_pause();
+    }
+}
+
 static int push_desc(nirrt_tree *t)
 {
     HIPCHK(hipMemcpyAsync(t->dev, &t->host, sizeof(TreeDev), hipMemcpyHostToDevice, t->stream));
@@ -353,7 +454,6 @@ static int push_desc(nirrt_tree *t)
 // device go back to the driver at once (nirrt_pool_trim returns that one too): a long-lived process that plans batches of
 // varying iter_max neither grows without bound nor starves other users of the device (torch) of memory.
 #include <map>
-#include <mutex>
 namespace {
 struct ArenaPool {
     std::mutex mu;
@@ -1297,14 +1397,15 @@ static int do_step(nirrt_tree *t, const double *p, int host_steer, int64_t neare
 {
     if (!t || !p || !res) return NIRRT_E_ARG;
     HIPCHK(hipSetDevice(t->device));
+    AskBox *ask = t->dim == 2 && !host_steer ? ask_box(t->device) : nullptr;   // (3D steers need IEEE operations only)
     DISPATCH_BY_SIZE(t, k_step, t->dev, p[0], p[1], t->dim == 3 ? p[2] : 0., host_steer, (int)nearest_idx, (unsigned)flags,
                      &t->scratch_dev->step);
-    int rc = sync_check(t);
-    if (rc) return rc;
+    HIPCHK(hipGetLastError());
+    HIPCHK(ask_wait(ask, t->stream));
     *res = t->scratch->step;
     t->last_n = res->n;
     if (res->status) {
-        g_err = res->status == NIRRT_E_LIBM ? "the restated libm routines returned NaN for this steer (argument outside their supported domain)"
+        g_err = res->status == NIRRT_E_LIBM ? "a steer came out as NaN (non-finite coordinates, or the question to the host's libm was not answered)"
                                             : "capacity exceeded inside step";
         return res->status;
     }
@@ -1772,6 +1873,7 @@ static int run_sampling(nirrt_tree *const *trees, int32_t n_trees, const nirrt_r
     HIPCHK_R(dalloc(sizeof(long long) * 2 * nt * COLLECT_W, (void **)&d_col));
     hipLaunchKernelGGL(k_collect, dim3((n_trees + 255) / 256), dim3(256), 0, st, (TreeDev *const *)d_ptrs, n_trees, d_col);
     HIPCHK_R(hipStreamSynchronize(st));   // inputs in place before any group's stream starts
+    AskBox *ask = D == 2 || (a->flags & NIRRT_F_IRRT) ? ask_box(t0->device) : nullptr;   // (3D RRT* needs IEEE operations only)
     for (Group &g : groups) {
         RunSampleDev rd;
         const int o = g.b0;
@@ -1812,7 +1914,7 @@ static int run_sampling(nirrt_tree *const *trees, int32_t n_trees, const nirrt_r
     }
     float ms_max = 0.f;
     for (Group &g : groups) {
-        HIPCHK_R(hipStreamSynchronize(g.st));
+        HIPCHK_R(ask_wait(ask, g.st));
     }
     for (Group &g : groups) {
         // first group's start -> this group's end: groups that each fill the GPU run one after the other, whatever their streams
@@ -1915,13 +2017,14 @@ extern "C" int nirrt_run(nirrt_tree *const *trees, int32_t n_trees, const nirrt_
     hipEvent_t e0, e1;
     HIPCHK(hipEventCreate(&e0));
     HIPCHK(hipEventCreate(&e1));
+    AskBox *ask = D == 2 ? ask_box(t0->device) : nullptr;
     HIPCHK(hipEventRecord(e0, st));
     long long n_hi = 0;
     for (int i = 0; i < n_trees; i++) n_hi = std::max(n_hi, trees[i]->last_n);
     LAUNCH_V(run_variant(n_trees, a->flags, n_hi, a->iters), D, k_run_replay, n_trees, st, (TreeDev *const *)d_ptrs, rd);
     HIPCHK(hipEventRecord(e1, st));
     HIPCHK(hipGetLastError());
-    HIPCHK(hipStreamSynchronize(st));
+    HIPCHK(ask_wait(ask, st));
     float ms = 0.f;
     HIPCHK(hipEventElapsedTime(&ms, e0, e1));
     if (a->kernel_ms) *a->kernel_ms = ms;

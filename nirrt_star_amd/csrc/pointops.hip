@@ -8,8 +8,14 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdlib.h>
+#include <string.h>
 
-// glibc 2.35's sin / cos (restated; every lane its own argument): the 3D ellipsoid candidates of the guidance clouds
+// sin / cos with the host libm's roundings, every lane its own argument (the 3D ellipsoid candidates of the guidance clouds): an undecided
+// value is marked and filled in by the host after the launch
+#include <math.h>
+#include <thread>
+#include "nirrt_ask.hpp"
+#include "nirrt_libm_host.hpp"
 #define GLIBC_NS glibc235v
 #define GLIBC_UNIFORM 0
 #include "glibc235_device.inc"
@@ -550,9 +556,10 @@ extern "C" int nirrt_fps_f64_batch(const double *pts, int n_clouds, const int *c
 }
 
 // ------------------------------------------------------------------------------------------------
-// nirrt_libm_probe: the restated glibc routines (csrc/glibc235_libm.inc) evaluated on the device for arguments the CALLER chooses -
-// the Python binding compares them with the host's own math.atan2 / math.sin / math.cos before it trusts the device-side steer
-// (a host whose libm is not glibc 2.35 / x86-64 / FMA computes other last bits in the REFERENCE: nirrt_star_amd/_hip.libm_check)
+// nirrt_libm_probe: atan2 / sin / cos as the device-side steer and samplers get them (csrc/glibc235_libm.inc: evaluated on the device,
+// the undecided ones by a call of this host's libm) for arguments the CALLER chooses - the Python binding compares them with its own
+// math.atan2 / math.sin / math.cos before it trusts the device-resident loop (a libm whose error is beyond the bound the routines
+// assume would differ: nirrt_star_amd/_hip.libm_check)
 // ------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void k_libm_probe(int fn, long long n, const double *a, const double *b, double *out)
 {
@@ -565,6 +572,13 @@ __global__ __launch_bounds__(256) void k_libm_probe(int fn, long long n, const d
     out[i] = r;
 }
 
+static bool is_mark(double v)
+{
+    uint64_t u;
+    memcpy(&u, &v, 8);
+    return u == nirrt_ask::MARK;
+}
+
 extern "C" int nirrt_libm_probe(int32_t fn, int64_t n, const double *a, const double *b, double *out, int device_id)
 {
     if (fn < 0 || fn > 2 || n < 0 || (n > 0 && (!a || !out || (fn == 0 && !b)))) return -1;
@@ -573,19 +587,6 @@ extern "C" int nirrt_libm_probe(int32_t fn, int64_t n, const double *a, const do
     double *d = nullptr;
     if (hipMalloc(&d, sizeof(double) * 3 * (size_t)n) != hipSuccess) { (void)hipGetLastError(); return -2; }
     int rc = 0;
-    // test hook (tests/test_libm_check_gpu.py): NIRRT_LIBM_PROBE_FLIP=1 flips the lowest bit of one word of the sin / cos table for
-    // the duration of the probe - what a table that does not belong to the host's libm looks like to the caller
-    const char *flip = getenv("NIRRT_LIBM_PROBE_FLIP");
-    const bool do_flip = flip && *flip && *flip != '0';
-    uint64_t saved[440];
-    if (do_flip) {
-        if (hipMemcpyFromSymbol(saved, HIP_SYMBOL(glibc235v::T_sincos), sizeof(saved)) != hipSuccess) rc = -2;
-        if (!rc) {
-            uint64_t bad[440];
-            for (int i = 0; i < 440; i++) bad[i] = saved[i] ^ ((i % 4 == 0) ? 1ull : 0ull);   // the leading word of every entry
-            if (hipMemcpyToSymbol(HIP_SYMBOL(glibc235v::T_sincos), bad, sizeof(bad)) != hipSuccess) rc = -2;
-        }
-    }
     if (!rc && hipMemcpy(d, a, sizeof(double) * (size_t)n, hipMemcpyHostToDevice) != hipSuccess) rc = -2;
     if (!rc && fn == 0 && hipMemcpy(d + n, b, sizeof(double) * (size_t)n, hipMemcpyHostToDevice) != hipSuccess) rc = -2;
     if (!rc) {
@@ -593,9 +594,23 @@ extern "C" int nirrt_libm_probe(int32_t fn, int64_t n, const double *a, const do
                            (const double *)(d + n), d + 2 * n);
         if (hipGetLastError() != hipSuccess || hipMemcpy(out, d + 2 * n, sizeof(double) * (size_t)n, hipMemcpyDeviceToHost) != hipSuccess) rc = -2;
     }
-    if (do_flip && hipMemcpyToSymbol(HIP_SYMBOL(glibc235v::T_sincos), saved, sizeof(saved)) != hipSuccess) rc = -2;
     (void)hipFree(d);
     if (rc == -2) (void)hipGetLastError();
+    if (!rc) {
+        for (int64_t i = 0; i < n; i++)
+            if (is_mark(out[i]))
+                out[i] = fn == 0 ? nirrt_libm_host::p_atan2(a[i], b[i]) : fn == 1 ? nirrt_libm_host::p_sin(a[i]) : nirrt_libm_host::p_cos(a[i]);
+        // test hook (tests/test_libm_check_gpu.py): NIRRT_LIBM_PROBE_FLIP=1 flips the lowest bit of every eighth sine and cosine -
+        // what a host whose libm is beyond the assumed bound looks like to the caller
+        const char *flip = getenv("NIRRT_LIBM_PROBE_FLIP");
+        if (flip && *flip && *flip != '0' && fn != 0)
+            for (int64_t i = 0; i < n; i += 8) {
+                uint64_t u;
+                memcpy(&u, &out[i], 8);
+                u ^= 1ull;
+                memcpy(&out[i], &u, 8);
+            }
+    }
     return rc;
 }
 
@@ -613,8 +628,7 @@ extern "C" int nirrt_fps_f64(const double *pts, int N, int num_samples, unsigned
 // (a = w0 >> 5, b = w1 >> 6, (a * 2^26 + b) / 2^53), uniform(lo, hi) = lo + (hi - lo) * u, the ellipse transform as numpy's
 // dgemm evaluates it for K = 3 (fma chain in k order: fma(a1, s1, a0 * s0), the z term adds an exact zero), np.linalg.norm
 // (axis) = sqrt(x*x + y*y), astype(int) = truncation.  The 3D ellipsoid candidates (point_cloud_mask_utils_3d.py:132-200) go
-// through sin / cos: the device's own (OCML), so they agree with the host's to a few ulp, not bit for bit - like the informed
-// samples of the 3D loop.
+// through sin / cos with the host libm's roundings (k_cloud_angles): bit-equal too.
 // ------------------------------------------------------------------------------------------------
 struct nirrt_cloud_job {
     const unsigned *words;          // DEVICE: generator outputs from the problem's current position (>= 2 * n_doubles of them)
@@ -635,9 +649,39 @@ __device__ __forceinline__ double mt_double(const unsigned *w, long long j)
 }
 
 #define CAND_NT 256
+// The spherical angles of the ellipsoid candidates (mode 3) of all clouds: ang[4 c ..] = sin theta, cos theta, sin phi, cos phi of
+// candidate c = cloud * n_raw + i.  A value whose rounding in the host's libm is not certain (one in sixteen) goes into a list -
+// AskItem, in whatever order the lanes arrive: each writes its own place - which the host fills in by calling its libm and
+// k_cloud_answers puts back.  (3D refresh of 256 clouds: 6.3 M values, 0.39 M of them asked.)
+struct AskItem { double v; unsigned at; int is_cos; };
+__global__ __launch_bounds__(CAND_NT) void k_cloud_angles(const nirrt_cloud_job *jobs, int n_raw, double *ang, AskItem *items, unsigned cap, unsigned *n_items)
+{
+    const nirrt_cloud_job *jb = jobs + blockIdx.y;
+    const int i = blockIdx.x * CAND_NT + threadIdx.x;
+    if (jb->mode != 3 || i >= n_raw) return;
+    const double PI = 3.141592653589793;
+    const double th = 0.0 + (PI - 0.0) * mt_double(jb->words, (long long)n_raw + i);
+    const double ph = 0.0 + (2 * PI - 0.0) * mt_double(jb->words, 2ll * n_raw + i);
+    const long long c = 4 * ((long long)blockIdx.y * n_raw + i);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const double x = j < 2 ? th : ph;
+        const double v = (j & 1) ? glibc235v::cos_fn(x) : glibc235v::sin_fn(x);
+        ang[c + j] = v;
+        if ((unsigned long long)__double_as_longlong(v) == nirrt_ask::MARK) {
+            const unsigned at = atomicAdd(n_items, 1u);
+            if (at < cap) { items[at].v = x; items[at].at = (unsigned)(c + j); items[at].is_cos = j & 1; }
+        }
+    }
+}
+__global__ __launch_bounds__(CAND_NT) void k_cloud_answers(const AskItem *items, unsigned n, double *ang)
+{
+    const unsigned i = blockIdx.x * CAND_NT + threadIdx.x;
+    if (i < n) ang[items[i].at] = items[i].v;
+}
 // one workgroup per cloud: candidate i of cloud b -> (x, y, z) + keep flag; survivors compacted in order into the SoA
 // buffer region [b * n_raw, (b + 1) * n_raw) (x of all clouds, then y, then z), cnt[b] = their number
-__global__ __launch_bounds__(CAND_NT) void k_cloud_candidates(const nirrt_cloud_job *jobs, int n_raw, double *buf, long long total, int *cnt)
+__global__ __launch_bounds__(CAND_NT) void k_cloud_candidates(const nirrt_cloud_job *jobs, int n_raw, const double *ang, double *buf, long long total, int *cnt)
 {
     __shared__ int wave_tot[CAND_NT / 64];
     __shared__ int base_s;
@@ -660,13 +704,9 @@ __global__ __launch_bounds__(CAND_NT) void k_cloud_candidates(const nirrt_cloud_
                 } else {
                     // rng.uniform(0, 1, n), rng.uniform(0, pi, n), rng.uniform(0, 2 pi, n): three arrays drawn one after the other;
                     // spherical coordinates -> unit ball -> (C.L) . s + x_center, then the range test
-                    const double PI = 3.141592653589793;
                     const double rr = 0.0 + (1.0 - 0.0) * mt_double(jb.words, (long long)i);
-                    const double th = 0.0 + (PI - 0.0) * mt_double(jb.words, (long long)n_raw + i);
-                    const double ph = 0.0 + (2 * PI - 0.0) * mt_double(jb.words, 2ll * n_raw + i);
-                    // (np.sin / np.cos of numpy 2.2 are libm's for float64: the restated glibc functions, one argument per lane)
-                    const double st = glibc235v::sin_fn(th), ct = glibc235v::cos_fn(th);
-                    const double sp = glibc235v::sin_fn(ph), cp = glibc235v::cos_fn(ph);
+                    const double *an = ang + 4 * ((long long)blockIdx.x * n_raw + i);
+                    const double st = an[0], ct = an[1], sp = an[2], cp = an[3];   // (np.sin / np.cos of numpy 2.2 are libm's for float64)
                     const double s0 = rr * st * cp, s1 = rr * st * sp, s2 = rr * ct;
                     x = __builtin_fma(jb.a[2], s2, __builtin_fma(jb.a[1], s1, jb.a[0] * s0)) + jb.a[9];
                     y = __builtin_fma(jb.a[5], s2, __builtin_fma(jb.a[4], s1, jb.a[3] * s0)) + jb.a[10];
@@ -756,6 +796,36 @@ __global__ __launch_bounds__(CAND_NT) void k_cloud_compact(const double *buf, lo
 
 static FpsScratch g_cloud_scratch[16];
 
+// k_cloud_angles, the asked values by this host's libm (several threads for many of them), k_cloud_answers
+static int cloud_angles(const nirrt_cloud_job *d_jobs, int n_jobs, int n_raw, double *d_ang, unsigned *d_nask, AskItem *d_ask, unsigned cap)
+{
+    unsigned n = 0;
+    if (hipMemcpy(d_nask, &n, sizeof(n), hipMemcpyHostToDevice) != hipSuccess) return -2;
+    hipLaunchKernelGGL(k_cloud_angles, dim3((unsigned)((n_raw + CAND_NT - 1) / CAND_NT), (unsigned)n_jobs), dim3(CAND_NT), 0, 0, d_jobs, n_raw, d_ang,
+                       d_ask, cap, d_nask);
+    if (hipGetLastError() != hipSuccess || hipMemcpy(&n, d_nask, sizeof(n), hipMemcpyDeviceToHost) != hipSuccess) return -2;
+    if (n > cap) return -2;
+    if (n == 0) return 0;
+    std::vector<AskItem> items(n);
+    if (hipMemcpy(items.data(), d_ask, sizeof(AskItem) * (size_t)n, hipMemcpyDeviceToHost) != hipSuccess) return -2;
+    auto answer = [&items](size_t lo, size_t hi) {
+        for (size_t i = lo; i < hi; i++) items[i].v = items[i].is_cos ? nirrt_libm_host::p_cos(items[i].v) : nirrt_libm_host::p_sin(items[i].v);
+    };
+    const size_t parts = n >= 32768 ? 8 : 1;   // (a thread costs ~50 us, 4096 calls ~100 us)
+    std::vector<std::thread> workers;
+    size_t lo = 0;
+    for (size_t p = 1; p < parts; p++) {
+        const size_t hi = n * p / parts;
+        try { workers.emplace_back(answer, lo, hi); } catch (...) { break; }   // (no thread to be had: the rest is done here)
+        lo = hi;
+    }
+    answer(lo, n);
+    for (std::thread &t : workers) t.join();
+    if (hipMemcpy(d_ask, items.data(), sizeof(AskItem) * (size_t)n, hipMemcpyHostToDevice) != hipSuccess) return -2;
+    hipLaunchKernelGGL(k_cloud_answers, dim3((n + CAND_NT - 1) / CAND_NT), dim3(CAND_NT), 0, 0, (const AskItem *)d_ask, n, d_ang);
+    return hipGetLastError() == hipSuccess ? 0 : -2;
+}
+
 // Candidates -> down-sampling -> compaction for n_jobs clouds, all on `device_id`.  jobs: HOST array (its pointers are DEVICE
 // addresses); clouds: DEVICE (n_jobs, n_points, 3) f64 out; n_cand / n_out: HOST out (candidates that survived the filters / points
 // of the final cloud, <= n_points).  n_raw <= 16384.
@@ -771,7 +841,14 @@ extern "C" int nirrt_guidance_clouds(const nirrt_cloud_job *jobs, int n_jobs, in
     const size_t b_pts = (sizeof(double) * 3 * (size_t)total + a256) & ~a256, b_sel = ((size_t)total + a256) & ~a256;
     const size_t b_off = (sizeof(long long) * (size_t)n_jobs + a256) & ~a256, b_int = (sizeof(int) * (size_t)n_jobs + a256) & ~a256;
     const size_t b_job = (sizeof(nirrt_cloud_job) * (size_t)n_jobs + a256) & ~a256;
-    const size_t need = b_pts + b_sel + b_off + 3 * b_int + b_job;
+    bool ellipsoids = false;
+    for (int b = 0; b < n_jobs; b++) ellipsoids = ellipsoids || jobs[b].mode == 3;
+    if (ellipsoids && total > (1ll << 29)) return -1;   // (32-bit places in the list of asked values)
+    // list of asked values: one in sixteen of 4 total; room for a quarter, never less than all of a small batch
+    const unsigned ask_cap = ellipsoids ? (unsigned)(4 * total < total + 1024 ? 4 * total : total + 1024) : 0u;
+    const size_t b_ang = ellipsoids ? (sizeof(double) * 4 * (size_t)total + a256) & ~a256 : 0;
+    const size_t b_ask = ellipsoids ? 256 + ((sizeof(AskItem) * (size_t)ask_cap + a256) & ~a256) : 0;
+    const size_t need = b_pts + b_sel + b_off + 3 * b_int + b_job + b_ang + b_ask;
     std::lock_guard<std::mutex> hold(g_fps_mu);
     FpsScratch &sc = g_cloud_scratch[device_id & 15];
     if (sc.cap < need) {
@@ -787,6 +864,9 @@ extern "C" int nirrt_guidance_clouds(const nirrt_cloud_job *jobs, int n_jobs, in
     long long *d_off = (long long *)(base + b_pts + b_sel);
     int *d_cnt = (int *)(base + b_pts + b_sel + b_off), *d_ns = d_cnt + b_int / sizeof(int), *d_nout = d_ns + b_int / sizeof(int);
     nirrt_cloud_job *d_jobs = (nirrt_cloud_job *)(base + b_pts + b_sel + b_off + 3 * b_int);
+    double *d_ang = (double *)(base + b_pts + b_sel + b_off + 3 * b_int + b_job);
+    unsigned *d_nask = (unsigned *)((char *)d_ang + b_ang);
+    AskItem *d_ask = (AskItem *)((char *)d_nask + 256);
     std::vector<long long> h_off((size_t)n_jobs);
     std::vector<int> h_ns((size_t)n_jobs, n_points);
     for (int b = 0; b < n_jobs; b++) h_off[b] = (long long)b * n_raw;
@@ -795,12 +875,14 @@ extern "C" int nirrt_guidance_clouds(const nirrt_cloud_job *jobs, int n_jobs, in
         hipMemcpy(d_off, h_off.data(), sizeof(long long) * (size_t)n_jobs, hipMemcpyHostToDevice) != hipSuccess ||
         hipMemcpy(d_ns, h_ns.data(), sizeof(int) * (size_t)n_jobs, hipMemcpyHostToDevice) != hipSuccess)
         rc = -2;
+    if (!rc && ellipsoids) rc = cloud_angles(d_jobs, n_jobs, n_raw, d_ang, d_nask, d_ask, ask_cap);
     if (!rc) {
         // The three kernels run on the NULL stream on purpose: the generator outputs they read are complete (nirrt_generator_words
         // waits for its launch), and the clouds they write are read next by torch's default stream - the legacy stream orders
         // that without events.  (With NIRRT_BATCH_GROUPS >= 2 - off by default, see batch.run_batch - the launch waits
         // for the other group's persistent kernel when the tree streams are blocking ones.)
-        hipLaunchKernelGGL(k_cloud_candidates, dim3(n_jobs), dim3(CAND_NT), 0, 0, (const nirrt_cloud_job *)d_jobs, n_raw, d, total, d_cnt);
+        hipLaunchKernelGGL(k_cloud_candidates, dim3(n_jobs), dim3(CAND_NT), 0, 0, (const nirrt_cloud_job *)d_jobs, n_raw,
+                           (const double *)d_ang, d, total, d_cnt);
         // k_fps_f64 leaves clouds with cnt <= num_samples alone (k_cloud_compact keeps all of their points)
         if (n_raw <= 20 * FPS64_NT && fps64_in_registers()) {
             if (jobs[0].mode >= 2)

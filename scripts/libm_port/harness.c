@@ -1,4 +1,6 @@
-// CPU validation of the transliterated glibc functions against the libm they were taken from:  gcc -O2 -ffp-contract=off harness.c -lm
+// CPU check of csrc/glibc235_libm.inc against this machine's libm (the C library's atan2 / sin / cos, called):
+//   gcc -O2 -fno-builtin -ffp-contract=off harness.c -lm -o harness && ./harness 20000000
+// A result that the routines decide themselves has to be the libm's, bit for bit; the last line says how many they decided.
 #include <math.h>
 #include <stdint.h>
 #include <stdio.h>
@@ -17,13 +19,21 @@ static inline uint64_t B(double d) { uint64_t u; memcpy(&u, &d, 8); return u; }
 #define S32(off) ((uint32_t)(stk[(off) / 8] >> (((off) & 4) * 8)))
 #define W32(off, v) (stk[(off) / 8] = (stk[(off) / 8] & ~(0xffffffffull << (((off) & 4) * 8))) | ((uint64_t)(uint32_t)(v) << (((off) & 4) * 8)))
 static inline uint64_t LD64(int64_t a);
+// (a question to the libm counts)
+static long g_asked = 0;
+static double ask2(double y, double x) { g_asked++; return atan2(y, x); }
+static double ask_s(double x) { g_asked++; return sin(x); }
+static double ask_c(double x) { g_asked++; return cos(x); }
+#define LIBM_ASK_ATAN2(y, x) ask2(y, x)
+#define LIBM_ASK_SIN(x) ask_s(x)
+#define LIBM_ASK_COS(x) ask_c(x)
 #define LD32(a) ((uint32_t)LD64(a))
 #include "../../nirrt_star_amd/csrc/glibc235_libm.inc"
 
 static inline uint64_t LD64(int64_t a)
 {
     if (a >= LIBM_T_SINCOS_BASE && a < LIBM_T_SINCOS_BASE + 8 * 440) return T_sincos[(a - LIBM_T_SINCOS_BASE) / 8];
-    if (a >= LIBM_T_ATAN_BASE && a < LIBM_T_ATAN_BASE + 8 * 241 * 7) return T_atan[(a - LIBM_T_ATAN_BASE) / 8];
+    if (a >= LIBM_T_ATAN_BASE && a < LIBM_T_ATAN_BASE + 8) return T_atan[(a - LIBM_T_ATAN_BASE) / 8];
     g_unsupported++;
     return 0;
 }
@@ -32,7 +42,7 @@ static double rnd(void) { rs ^= rs << 13; rs ^= rs >> 7; rs ^= rs << 17; return 
 
 int main(int argc, char **argv)
 {
-    long n = argc > 1 ? atol(argv[1]) : 10000000, bad_a = 0, bad_s = 0, bad_c = 0;
+    long n = argc > 1 ? atol(argv[1]) : 10000000, bad_a = 0, bad_s = 0, bad_c = 0, bad_v = 0, undecided = 0;
     for (long i = 0; i < n; i++) {
         double sc = (i % 7 == 0) ? 1e-3 : (i % 11 == 0 ? 1e-9 : 224.0);
         double dy = (2 * rnd() - 1) * sc, dx = (2 * rnd() - 1) * sc;
@@ -43,6 +53,9 @@ int main(int argc, char **argv)
         double s1 = sin(th), s2 = glibc_sin(th, 0), c1 = cos(th), c2 = glibc_cos(th, 0);
         if (B(s1) != B(s2)) { if (bad_s++ < 5) printf("sin(%a) = %a, port %a\n", th, s1, s2); }
         if (B(c1) != B(c2)) { if (bad_c++ < 5) printf("cos(%a) = %a, port %a\n", th, c1, c2); }
+        double fx = 224 * rnd(), fy = 224 * rnd(), len = sqrt(dx * dx + dy * dy), m = len < 10 ? len : 10, ox, oy;
+        if (!libm_steer(fx, fy, dy, dx, m, &ox, &oy)) undecided++;
+        else if (B(ox) != B(fx + m * c1) || B(oy) != B(fy + m * s1)) { if (bad_v++ < 5) printf("steer(%a, %a, %a, %a)\n", fx, fy, dy, dx); }
     }
     // angles over a wider range than atan2 produces (sin / cos on their own)
     long bad_w = 0;
@@ -51,5 +64,7 @@ int main(int argc, char **argv)
         if (B(sin(th)) != B(glibc_sin(th, 0)) || B(cos(th)) != B(glibc_cos(th, 0))) { if (bad_w++ < 5) printf("wide: %a\n", th); }
     }
     printf("%ld samples: atan2 mismatches %ld, sin %ld, cos %ld, wide-range sin/cos %ld, unsupported paths hit %d\n", n, bad_a, bad_s, bad_c, bad_w, g_unsupported);
-    return (bad_a || bad_s || bad_c || bad_w || g_unsupported) ? 1 : 0;
+    printf("steer mismatches %ld; asked the libm: %.4f of the function values, %.4f of the steers\n", bad_v, (double)g_asked / (3. * n + 2. * (n / 4)),
+           (double)undecided / n);
+    return (bad_v || bad_a || bad_s || bad_c || bad_w || g_unsupported) ? 1 : 0;
 }
