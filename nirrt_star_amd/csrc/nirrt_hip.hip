@@ -1684,8 +1684,8 @@ static void report_stats(const nirrt_run_args *a, int i, const long long *after,
 // Lane groups of one nirrt_run call must run AT THE SAME TIME (the few wide workgroups of the heavy trees next to the many
 // one-wave trees).  Tree streams do not guarantee that: thousands of them share the handful of hardware queues, and two
 // launches that land on the same queue run one after the other (measured: the 64-lane group started the moment the 256-lane
-// group ended).  Three streams per device, created back to back (consecutive streams get consecutive hardware queues), the
-// first with the highest priority - it carries the widest, longest-running trees.
+// group ended).  Three streams per device, created back to back (consecutive streams get consecutive hardware queues), all of the
+// default priority (work on streams of different priorities has hung); the widest, longest-running trees are launched first.
 // One set per calling THREAD and device: concurrent nirrt_run calls from worker threads (run_batch with NIRRT_BATCH_GROUPS /
 // NIRRT_BATCH_INFLIGHT > 1) must not share streams - their launches would serialize and each call's event timing would contain
 // the other call's kernels.  (The few streams of a worker thread that ends are not destroyed: HIP may already be shutting down.)
@@ -1696,10 +1696,8 @@ static hipStream_t *group_streams(int device)
     auto it = sets.find(device);
     if (it == sets.end()) {
         Set s;
-        int lo = 0, hi = 0;   // (numerically lower = higher priority)
-        if (hipDeviceGetStreamPriorityRange(&lo, &hi) != hipSuccess) { lo = hi = 0; (void)hipGetLastError(); }
         for (int i = 0; i < 3; i++)
-            if (hipStreamCreateWithPriority(&s.st[i], hipStreamNonBlocking, i == 0 ? hi : lo) != hipSuccess) {
+            if (hipStreamCreateWithFlags(&s.st[i], hipStreamNonBlocking) != hipSuccess) {
                 (void)hipGetLastError();
                 for (int j = 0; j < i; j++) (void)hipStreamDestroy(s.st[j]);
                 return nullptr;
@@ -1788,7 +1786,7 @@ static int run_sampling(nirrt_tree *const *trees, int32_t n_trees, const nirrt_r
     // trees' own streams come from a pool of 32 per device: two nirrt_run calls from two threads could land on the same one -
     // their launches would serialize and each call's kernel_ms would contain the other's kernels.
     if (hipStream_t *gs = group_streams(t0->device))
-        for (size_t gi = 0; gi < groups.size(); gi++) groups[gi].st = gs[groups.size() > 1 ? gi : 2];   // (one group: a normal-priority stream)
+        for (size_t gi = 0; gi < groups.size(); gi++) groups[gi].st = gs[groups.size() > 1 ? gi : 2];
     bool identity = true;
     for (int j = 0; j < n_trees; j++) identity = identity && perm[(size_t)j] == j;
     std::vector<TreeDev *> ptrs((size_t)n_trees);
