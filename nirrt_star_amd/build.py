@@ -12,20 +12,23 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 SO = os.path.join(HERE, "libnirrt_hip.so")
-SOURCES = [os.path.join(CSRC, "nirrt_hip.hip"), os.path.join(CSRC, "pointops.hip")]
+SOURCES = [os.path.join(CSRC, "nirrt_hip.hip"), os.path.join(CSRC, "pointops.hip"), os.path.join(CSRC, "nnops.hip")]
 DEPS = SOURCES + [os.path.join(CSRC, "nirrt_device.hpp"), os.path.join(CSRC, "nirrt_kernels.inc"), os.path.join(CSRC, "glibc235_libm.inc"), os.path.join(CSRC, "glibc235_device.inc"),
                   os.path.join(CSRC, "nirrt_ask.hpp"), os.path.join(CSRC, "nirrt_libm_host.hpp"),
-                  os.path.join(os.path.dirname(HERE), "include", "nirrt_hip.h")]
+                  os.path.join(os.path.dirname(HERE), "include", "nirrt_hip.h"), os.path.join(os.path.dirname(HERE), "include", "nirrt_nnops.h")]
 # one module-wide LDS object at the same address in every kernel: the non-inlined loop-body functions then address it
 # with constant offsets instead of a per-kernel offset-table lookup (see LdsData in csrc/nirrt_device.hpp)
 # -fno-optimize-sibling-calls: keeps LLVM from marking the calls of the loop-body functions `tail`; only then does its
 # inter-procedural register allocation drop the callee-saved saves of those local functions (48 VGPRs = 12.8 KB of
 # scratch written and read back per wave and iteration otherwise - a quarter of the kernel's measured HBM writes).
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 (some of their forms have given wrong results; the host pass warns that it does not
+# know the feature, which is harmless)
 # -sink-insts-to-avoid-spills: the persistent loops call the loop's phases with nothing alive in registers (csrc/nirrt_kernels.inc,
 # run_tree_body) - except what machine LICM hoists out of the loop: LDS base addresses, zero constants.  Those were saved to
 # scratch and reloaded around every call (9 dwords per lane and iteration); with this flag they are re-materialised where they
 # are used and the loops of k_run_sample / k_run_pool have no scratch access at all.
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC", "-shared",
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          "-fno-optimize-sibling-calls", "-mllvm", "-amdgpu-lower-module-lds-strategy=module"]
 # (an -mllvm option the compiler does not know is a hard error: probed once per build, dropped with a note if this ROCm lacks it -
 #  the library is then correct but its persistent loops reload a few hoisted constants from scratch every iteration)
@@ -70,11 +73,24 @@ def optional_flags(hipcc):
 
 
 def _compile(so, extra, verbose):
+    """the sources side by side, then one link"""
+    import tempfile
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    cmd = [hipcc] + FLAGS + optional_flags(hipcc) + extra + ["-o", so] + SOURCES
-    if verbose:
-        print(" ".join(cmd))
-    subprocess.check_call(cmd)
+    flags = FLAGS + optional_flags(hipcc) + extra
+    with tempfile.TemporaryDirectory() as d:
+        objs, jobs = [], []
+        for src in SOURCES:
+            objs.append(os.path.join(d, os.path.basename(src) + ".o"))
+            cmd = [hipcc] + flags + ["-c", "-o", objs[-1], src]
+            if verbose:
+                print(" ".join(cmd))
+            jobs.append((cmd, subprocess.Popen(cmd)))
+        for cmd, job in jobs:
+            if job.wait() != 0:
+                for _, other in jobs:
+                    other.wait()
+                raise subprocess.CalledProcessError(job.returncode, cmd)
+        subprocess.check_call([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", so] + objs)
 
 
 def build(force=False, verbose=False, small=True):

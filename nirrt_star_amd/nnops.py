@@ -1,0 +1,338 @@
+"""Dense operators of the guidance network's layers and of its training step: hand-written HIP kernels of libnirrt_hip.so
+(csrc/nnops.hip, C ABI include/nirrt_nnops.h), launched on the current torch stream, differentiable where a gradient makes sense.
+
+    linear_act            act(x W^T + b) + r in one kernel, with its backward pass
+    linear_cross_entropy  a classification head with softmax cross entropy; the scores are never kept, forward or backward
+    grad_norm             2-norm over many tensors
+    clip_grad_norm_       the same, and the clipping by it (in place, or into other tensors)
+
+float32, bfloat16 and float16; sums are held in 32 bits and rounded once.  Tensors must live on the GPU (a CPU tensor is an error,
+there is no other implementation); rows may have any stride, other layouts are copied.  Results are the same bits for the same input
+(no atomics).  Backward passes are differentiable once.
+"""
+import ctypes as C
+
+import numpy as np
+import torch
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+_DIM_MAX = 0x7fffffff - 256
+
+
+def _lib():
+    from . import _hip
+    L = _hip.load()
+    if not hasattr(L, "_nn_ready"):
+        vp, i, l, f = C.c_void_p, C.c_int, C.c_int64, C.c_float
+        L.nirrt_nn_linear_workspace.argtypes = [i, l, l, l]
+        L.nirrt_nn_linear.argtypes = [i, i, vp, l, vp, l, vp, vp, l, vp, l, vp, l, l, l, vp, vp]
+        L.nirrt_nn_linear_backward_workspace.argtypes = [i, i, l, l, l]
+        L.nirrt_nn_linear_backward.argtypes = [i, i, vp, l, vp, l, vp, vp, l, vp, vp, vp, l, l, l, vp, vp]
+        L.nirrt_nn_cross_entropy_workspace.argtypes = [i, l, l, l]
+        L.nirrt_nn_cross_entropy.argtypes = [i, vp, l, vp, l, vp, vp, vp, l, vp, vp, vp, l, l, l, vp, vp]
+        L.nirrt_nn_cross_entropy_backward_workspace.argtypes = [i, l, l, l]
+        L.nirrt_nn_cross_entropy_backward.argtypes = [i, vp, l, vp, l, vp, vp, vp, l, vp, vp, i, vp, vp, vp, vp, l, l, l, vp, vp]
+        L.nirrt_nn_norm_workspace.argtypes = [vp, C.c_int32]
+        L.nirrt_nn_norm.argtypes = [vp, C.c_int32, vp, vp, vp]
+        L.nirrt_nn_scale_by_norm.argtypes = [vp, C.c_int32, vp, f, vp]
+        for name in ("linear", "linear_backward", "cross_entropy", "cross_entropy_backward", "norm"):
+            getattr(L, "nirrt_nn_%s_workspace" % name).restype = l
+            getattr(L, "nirrt_nn_%s" % name).restype = i
+        L.nirrt_nn_scale_by_norm.restype = i
+        L._nn_ready = True
+    return L
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _check(rc, what):
+    if rc != 0:
+        raise RuntimeError("libnirrt_hip %s failed (%d)" % (what, rc))
+
+
+def _on(device):
+    """the C functions launch on the calling thread's current device"""
+    return torch.cuda.device(device)
+
+
+def _need(name, first, **others):
+    """one device (a GPU) and one element type for all of them"""
+    if not first.is_cuda:
+        raise RuntimeError("nirrt_star_amd.nnops.%s got a CPU tensor: the package only has the HIP kernels (move it to 'cuda')" % name)
+    if first.dtype not in _TYPES:
+        raise ValueError("%s: float32, bfloat16 or float16, not %s" % (name, first.dtype))
+    for key, t in others.items():
+        if t is None:
+            continue
+        if t.device != first.device:
+            raise ValueError("%s: %s is on %s, the input on %s" % (name, key, t.device, first.device))
+        if t.dtype != first.dtype:
+            raise ValueError("%s: %s is %s, the input %s" % (name, key, t.dtype, first.dtype))
+
+
+def _rows(t):
+    """(..., k) -> (rows, k) with unit column stride and rows that do not overlap (a copy if need be), and its row stride"""
+    k = t.shape[-1]
+    if t.dim() != 2:
+        t = t.reshape(t.numel() // k if k else _prod(t.shape[:-1]), k)
+    m = t.shape[0]
+    if m <= 1 or k == 0:
+        return (t if k <= 1 or t.stride(1) == 1 else t.contiguous()), max(k, 1)
+    if (k > 1 and t.stride(1) != 1) or t.stride(0) < k:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+def _prod(shape):
+    n = 1
+    for s in shape:
+        n *= int(s)
+    return n
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _workspace(nbytes, device):
+    if nbytes < 0:
+        raise RuntimeError("libnirrt_hip: bad sizes for a workspace")
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _sizes_ok(name, *dims):
+    if any(d > _DIM_MAX for d in dims):
+        raise ValueError("%s: a dimension of %d is beyond %d" % (name, max(dims), _DIM_MAX))
+
+
+# ---- linear layer ---------------------------------------------------------------------------------------------------------------------
+def _linear_forward(x, w, b, r, act, keep):
+    """-> y, z (what the backward pass needs of the pre-activation: None, y itself, or a tensor of its own)"""
+    m, n, k = _prod(x.shape[:-1]), w.shape[0], w.shape[1]
+    x2, ldx = _rows(x)
+    w2, ldw = _rows(w)
+    y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
+    r2, ldr = _rows(r) if r is not None else (None, n)
+    z = None
+    if keep and act:
+        z = y if act == 1 and r is None else torch.empty(m, n, dtype=x.dtype, device=x.device)
+    if m and n:
+        L, dt = _lib(), _TYPES[x.dtype]
+        ws = _workspace(L.nirrt_nn_linear_workspace(dt, m, n, k), x.device)
+        _check(L.nirrt_nn_linear(dt, act, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b), _ptr(r2), ldr, y.data_ptr(), n,
+                                 None if z is None or z is y else z.data_ptr(), m, n, k, _ptr(ws), _stream(x.device)), "linear")
+    return y, z
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, b, r, act):
+        keep = ctx.needs_input_grad[0] or ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        with _on(x.device):
+            y, z = _linear_forward(x, w, b, r, act, keep)
+        ctx.act = act
+        if keep:
+            ctx.save_for_backward(x, w, z)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        need = ctx.needs_input_grad
+        dx = dw = db = None
+        if need[0] or need[1] or need[2]:
+            x, w, z = ctx.saved_tensors
+            m, n, k = _prod(x.shape[:-1]), w.shape[0], w.shape[1]
+            with _on(x.device):
+                dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
+                dw = torch.empty(n, k, dtype=x.dtype, device=x.device) if need[1] else None
+                db = torch.empty(n, dtype=x.dtype, device=x.device) if need[2] else None
+                if n == 0 and dx is not None:
+                    dx.zero_()
+                dy2, lddy = _rows(dy)
+                x2, ldx = _rows(x)
+                w2, ldw = _rows(w)
+                L, dt = _lib(), _TYPES[x.dtype]
+                ws = _workspace(L.nirrt_nn_linear_backward_workspace(dt, ctx.act, m, n, k), x.device)
+                if n:
+                    _check(L.nirrt_nn_linear_backward(dt, ctx.act, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(z), dy2.data_ptr(), lddy, _ptr(dx),
+                                                      _ptr(dw), _ptr(db), m, n, k, _ptr(ws), _stream(x.device)), "linear_backward")
+        return dx, dw, db, (dy if need[3] else None), None
+
+
+def linear_act(x, weight, bias=None, residual=None, activation="none"):
+    """act(x weight^T + bias) + residual: x (..., k), weight (n, k), bias (n,), residual (..., n) -> (..., n), all of one type.
+    activation: "none", "relu", "gelu" (with erf) or "silu".  Gradients for x, weight, bias and residual."""
+    if activation not in ACTIVATIONS:
+        raise ValueError("linear_act: activation %r is not one of %s" % (activation, ", ".join(ACTIVATIONS)))
+    _need("linear_act", x, weight=weight, bias=bias, residual=residual)
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError("linear_act: x %s and weight %s do not fit" % (tuple(x.shape), tuple(weight.shape)))
+    n = weight.shape[0]
+    if bias is not None and tuple(bias.shape) != (n,):
+        raise ValueError("linear_act: bias %s, expected (%d,)" % (tuple(bias.shape), n))
+    if residual is not None and residual.shape != x.shape[:-1] + (n,):
+        raise ValueError("linear_act: residual %s, expected %s" % (tuple(residual.shape), tuple(x.shape[:-1] + (n,))))
+    _sizes_ok("linear_act", _prod(x.shape[:-1]), n, weight.shape[1])
+    if bias is not None:
+        bias = bias.contiguous()
+    act = ACTIVATIONS[activation]
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
+        return _Linear.apply(x, weight, bias, residual, act)
+    with _on(x.device):
+        return _linear_forward(x, weight, bias, residual, act, False)[0]
+
+
+# ---- head with softmax cross entropy ---------------------------------------------------------------------------------------------------
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, b, target, cw, ignore, mode):
+        rows, v, k = target.numel(), w.shape[0], w.shape[1]
+        with _on(x.device):
+            x2, ldx = _rows(x)
+            w2, ldw = _rows(w)
+            lse = torch.empty(rows, dtype=torch.float32, device=x.device)
+            nll = torch.empty(target.shape, dtype=torch.float32, device=x.device)
+            total = torch.empty(3, dtype=torch.float32, device=x.device)
+            L, dt = _lib(), _TYPES[x.dtype]
+            ws = _workspace(L.nirrt_nn_cross_entropy_workspace(dt, rows, v, k), x.device)
+            _check(L.nirrt_nn_cross_entropy(dt, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b), target.data_ptr(), _ptr(cw), ignore, lse.data_ptr(),
+                                            nll.data_ptr(), total.data_ptr(), rows, v, k, _ptr(ws), _stream(x.device)), "cross_entropy")
+        ctx.ignore, ctx.mode = ignore, mode
+        ctx.save_for_backward(x, w, b, target, cw, lse, total)
+        return nll if mode == "none" else total[2 if mode == "mean" else 0]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        x, w, b, target, cw, lse, total = ctx.saved_tensors
+        rows, v, k = target.numel(), w.shape[0], w.shape[1]
+        need = ctx.needs_input_grad
+        with _on(x.device):
+            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
+            dw = torch.empty(v, k, dtype=x.dtype, device=x.device) if need[1] else None
+            db = torch.empty(v, dtype=x.dtype, device=x.device) if need[2] else None
+            x2, ldx = _rows(x)
+            w2, ldw = _rows(w)
+            dloss = dloss.float().contiguous()
+            L, dt = _lib(), _TYPES[x.dtype]
+            ws = _workspace(L.nirrt_nn_cross_entropy_backward_workspace(dt, rows, v, k), x.device)
+            _check(L.nirrt_nn_cross_entropy_backward(dt, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b), target.data_ptr(), _ptr(cw), ctx.ignore,
+                                                     lse.data_ptr(), dloss.data_ptr(), 1 if ctx.mode == "none" else 0,
+                                                     total.data_ptr() if ctx.mode == "mean" else None, _ptr(dx), _ptr(dw), _ptr(db), rows, v, k,
+                                                     _ptr(ws), _stream(x.device)), "cross_entropy_backward")
+        return dx, dw, db, None, None, None, None
+
+
+def linear_cross_entropy(x, weight, target, bias=None, class_weight=None, ignore_index=-100, reduction="mean"):
+    """softmax cross entropy of the scores x weight^T + bias against target, without keeping the scores: x (..., k), weight (classes, k),
+    target int64 (...), bias (classes,), class_weight float32 (classes,).  Rows whose target is ignore_index count for nothing (their
+    gradients are zero, whatever they hold); any other target outside [0, classes) gives NaN.  reduction: "mean" = sum of weight x loss
+    over the sum of weights (NaN if no row counts), "sum", or "none" (the shape of target); the loss is float32.  Gradients for x, weight
+    and bias."""
+    name = "linear_cross_entropy"
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError("%s: reduction %r is not mean, sum or none" % (name, reduction))
+    _need(name, x, weight=weight, bias=bias)
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.shape[0] < 1:
+        raise ValueError("%s: x %s and weight %s do not fit" % (name, tuple(x.shape), tuple(weight.shape)))
+    if target.dtype != torch.int64 or target.device != x.device or target.shape != x.shape[:-1]:
+        raise ValueError("%s: target must be int64 %s on %s" % (name, tuple(x.shape[:-1]), x.device))
+    v = weight.shape[0]
+    if bias is not None and tuple(bias.shape) != (v,):
+        raise ValueError("%s: bias %s, expected (%d,)" % (name, tuple(bias.shape), v))
+    if class_weight is not None and (class_weight.dtype != torch.float32 or class_weight.device != x.device or tuple(class_weight.shape) != (v,)
+                                     or class_weight.requires_grad):
+        raise ValueError("%s: class_weight must be float32 (%d,) on %s, without a gradient" % (name, v, x.device))
+    _sizes_ok(name, target.numel(), v, weight.shape[1])
+    return _LinearCrossEntropy.apply(x, weight, bias.contiguous() if bias is not None else None, target.contiguous(),
+                                     class_weight.contiguous() if class_weight is not None else None, int(ignore_index), reduction)
+
+
+# ---- norm and clipping of many tensors -------------------------------------------------------------------------------------------------
+_TENSOR = np.dtype([("data", "<u8"), ("out", "<u8"), ("n", "<i8"), ("dtype", "<i4"), ("out_dtype", "<i4")])   # nirrt_nn_tensor
+
+
+def _tensor_list(name, tensors):
+    ts = [t for t in tensors if t is not None]
+    if not ts:
+        raise ValueError("%s: no tensors" % name)
+    dev = ts[0].device
+    if dev.type != "cuda":
+        raise RuntimeError("nirrt_star_amd.nnops.%s got a CPU tensor: the package only has the HIP kernels (move it to 'cuda')" % name)
+    for t in ts:
+        if t.device != dev or t.dtype not in _TYPES or t.layout != torch.strided:
+            raise ValueError("%s: dense float32, bfloat16 or float16 tensors of one device, not %s %s on %s" % (name, t.layout, t.dtype, t.device))
+    return ts, dev
+
+
+def _table(ts, outs=None):
+    tab = np.zeros(len(ts), dtype=_TENSOR)
+    tab["data"] = [t.data_ptr() for t in ts]
+    tab["n"] = [t.numel() for t in ts]
+    tab["dtype"] = [_TYPES[t.dtype] for t in ts]
+    if outs is not None:
+        tab["out"] = [t.data_ptr() for t in outs]
+        tab["out_dtype"] = [_TYPES[t.dtype] for t in outs]
+    return tab
+
+
+def _norm(tab, dev):
+    L = _lib()
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    ws = _workspace(L.nirrt_nn_norm_workspace(tab.ctypes.data, len(tab)), dev)
+    _check(L.nirrt_nn_norm(tab.ctypes.data, len(tab), norm.data_ptr(), _ptr(ws), _stream(dev)), "norm")
+    return norm
+
+
+@torch.no_grad()
+def grad_norm(tensors):
+    """2-norm of all elements of the tensors (None entries are skipped), summed in 64 bits in a fixed order -> float32 scalar on their device"""
+    ts, dev = _tensor_list("grad_norm", tensors)
+    with _on(dev):
+        return _norm(_table([t.contiguous() for t in ts]), dev)
+
+
+@torch.no_grad()
+def clip_grad_norm_(grads, max_norm, out=None):
+    """scales the tensors by min(1, max_norm / (norm + 1e-6)), norm as grad_norm gives it, and returns the norm (float32 scalar on their
+    device; nothing waits for it).  In place, or into `out`: as many contiguous tensors of the same shapes, of any of the three types
+    (half-precision gradients into float32 ones, say).  None entries are skipped (in `out` too).  A tensor may be named once only, and an
+    `out` tensor may share memory with its own gradient (of the same type) but not with another one."""
+    name = "clip_grad_norm_"
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError("%s: max_norm %r" % (name, max_norm))
+    grads = list(grads)
+    if out is not None:
+        out = list(out)
+        if len(out) != len(grads) or any((g is None) != (o is None) for g, o in zip(grads, out)):
+            raise ValueError("%s: %d gradients, %d outputs (None where the gradient is)" % (name, len(grads), len(out)))
+    ts, dev = _tensor_list(name, grads)
+    src = [t if t.is_contiguous() else t.contiguous() for t in ts]
+    if out is None:
+        dst = src
+    else:
+        dst, dev_o = _tensor_list(name, out)
+        if dev_o != dev or any(o.shape != t.shape or not o.is_contiguous() for o, t in zip(dst, ts)):
+            raise ValueError("%s: outputs must be contiguous, of the gradients' shapes and on their device" % name)
+    tab = _table(src, dst)
+    full = tab[tab["n"] > 0]
+    if len(np.unique(full["out"])) != len(full):
+        raise ValueError("%s: a tensor is named twice" % name)
+    if out is not None:
+        own = full["out"] == full["data"]
+        if np.isin(full["out"][~own], full["data"]).any() or (full["dtype"][own] != full["out_dtype"][own]).any():
+            raise ValueError("%s: an output shares memory with another gradient, or with its own of another type" % name)
+    with _on(dev):
+        norm = _norm(tab, dev)
+        _check(_lib().nirrt_nn_scale_by_norm(tab.ctypes.data, len(tab), norm.data_ptr(), max_norm, _stream(dev)), "scale_by_norm")
+        if out is None:
+            for t, s in zip(ts, src):
+                if s is not t:
+                    t.copy_(s)
+    return norm

@@ -1,4 +1,4 @@
-"""PointNet++ MSG segmentation net for point-cloud guidance, forward only, PyTorch-ROCm.
+"""PointNet++ MSG segmentation net for point-cloud guidance, PyTorch-ROCm: inference, and the step it is trained with.
 
 Architecture + state-dict layout of the reference (pointnet_pointnet2/models/pointnet2.py:7-42,
 pointnet2_utils.py:207-317) so its checkpoints load unchanged (240 tensors: sa{1-4}.conv_blocks.i.j,
@@ -14,6 +14,10 @@ on MI355X:
     O(N log N) sort.  The model therefore runs on 'cuda' only (pointops raises on CPU tensors; the test
     suite replaces the pointops functions from tests/conftest.py for its CPU runs).
 
+Training (`get_model.loss`, `train_step`): the reference's weighted negative log likelihood (get_loss, pointnet2.py:45-51) as ONE operator
+with the head's product (nnops.linear_cross_entropy: the class scores are never written), and the gradients' norm and clipping over all
+parameters at once (nnops.clip_grad_norm_).
+
 Semantics kept from the reference: FPS starts at torch.randint(0, N) drawn from the CPU generator
 (pointnet2_utils.py:77); ball query = first K indices in ascending order with squared distance
 <= r^2, padded with the first hit (:89-109); grouped features are [point feats, xyz - centre] (:247-250);
@@ -23,7 +27,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import pointops
+from . import nnops, pointops
 
 SA_SPECS = [  # npoint, radii, nsamples, in_channel, mlps   (pointnet2.py:11-14)
     (1024, [0.05, 0.1], [16, 32], 6, [[16, 16, 32], [32, 32, 64]]),
@@ -222,6 +226,19 @@ class get_model(nn.Module):
         levels behind it work on 1024 / 256 / 64 / 16 sampled points, the feature propagation and the head per point: cloud b's
         first n_valid[b] output rows are what a forward over that cloud alone gives (up to the library GEMMs' summation order,
         as for any batch), the rows behind them mean nothing."""
+        f0, f4 = self._point_features(points, fps_starts, n_valid)
+        if self._head is not None and not self.training:
+            B, N, _ = f0.shape
+            w, b = self._head
+            x = _affine_relu(b, f0.reshape(B * N, -1), w)
+            x = torch.addmm(self.conv2.bias, x, self.conv2.weight.reshape(self.conv2.weight.shape[0], -1).t()).view(B, N, -1)
+        else:
+            x = self.drop1(F.relu(self.bn1(self.conv1(f0.permute(0, 2, 1)))))
+            x = self.conv2(x).permute(0, 2, 1)
+        return F.log_softmax(x, dim=-1), f4.permute(0, 2, 1)
+
+    def _point_features(self, points, fps_starts, n_valid):
+        """-> per-point features (B, N, 128), features of the 16 points of the last level (B, 16, 1024)"""
         feats0 = points.permute(0, 2, 1).contiguous()       # (B, N, 6)
         xyz0 = feats0[:, :, :3].contiguous()
         st = fps_starts or [None] * 4
@@ -234,15 +251,27 @@ class get_model(nn.Module):
         f2 = self.fp3(xyz2, xyz3, f2, f3)
         f1 = self.fp2(xyz1, xyz2, f1, f2)
         f0 = self.fp1(xyz0, xyz1, None, f1)                 # (B, N, 128)
-        if self._head is not None and not self.training:
-            B, N, _ = f0.shape
-            w, b = self._head
-            x = _affine_relu(b, f0.reshape(B * N, -1), w)
-            x = torch.addmm(self.conv2.bias, x, self.conv2.weight.reshape(self.conv2.weight.shape[0], -1).t()).view(B, N, -1)
-        else:
-            x = self.drop1(F.relu(self.bn1(self.conv1(f0.permute(0, 2, 1)))))
-            x = self.conv2(x).permute(0, 2, 1)
-        return F.log_softmax(x, dim=-1), f4.permute(0, 2, 1)
+        return f0, f4
+
+    def loss(self, points, labels, class_weight=None, fps_starts=None):
+        """mean cross entropy of the points' labels (B, N) int64 (-100: the point counts for nothing), weighted by class (the training
+        set's labelweights), as the reference trains with: F.nll_loss(log_softmax, target, weight).  With gradients for all parameters;
+        head and loss are one operator."""
+        f0, _ = self._point_features(points, fps_starts, None)
+        x = self.drop1(F.relu(self.bn1(self.conv1(f0.permute(0, 2, 1)))))
+        return nnops.linear_cross_entropy(x.permute(0, 2, 1), self.conv2.weight.squeeze(2), labels, bias=self.conv2.bias, class_weight=class_weight)
+
+
+def train_step(model, optimizer, points, labels, class_weight=None, max_norm=None, fps_starts=None):
+    """one optimiser step on a batch of clouds: points (B, 6, N), labels (B, N) -> (loss, norm of the gradients before clipping), scalars on
+    the device.  max_norm: the gradients are scaled down to this norm (None: they are left as they are)."""
+    optimizer.zero_grad(set_to_none=True)
+    loss = model.loss(points, labels, class_weight, fps_starts)
+    loss.backward()
+    grads = [p.grad for group in optimizer.param_groups for p in group["params"]]
+    norm = nnops.grad_norm(grads) if max_norm is None else nnops.clip_grad_norm_(grads, max_norm)
+    optimizer.step()
+    return loss.detach(), norm
 
 
 def pc_normalize(pc):
