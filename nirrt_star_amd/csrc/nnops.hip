@@ -30,7 +30,8 @@ constexpr int CHUNKS = ROW_BYTES / 16;
 
 template <class T> struct Elem { static constexpr int PER_CHUNK = 16 / sizeof(T), STEP = ROW_BYTES / sizeof(T); };
 
-__device__ __forceinline__ int sw(int row) { return (row ^ (row >> 3)) & 7; }   // 8 lanes on 8 neighbouring (or every 4th) rows: 8 places
+// 8 lanes on 8 neighbouring (or every 4th) rows: 8 places; rows 32 apart: the same (their addresses differ by a constant)
+__device__ __forceinline__ int sw(int row) { return (row ^ ((row >> 3) & 3)) & 7; }
 
 __device__ __forceinline__ f32x16 mma(bf16_t, u32x4 a, u32x4 b, f32x16 c)
 {
@@ -47,15 +48,38 @@ __device__ __forceinline__ f32x16 mma(float, u32x4 a, u32x4 b, f32x16 c)
     return c;
 }
 
-// one operand: element (r, k) at p[r * ld + k] (KC) or p[k * ld + r] (RC); vec: whole 16-byte chunks (KC) / 4 elements (RC) are aligned.
-// skip (RC, or null): row k of the operand counts as zeros where skip[k] == 0, whatever it holds
+// one operand: element (r, k) at p[r * ld + k] (KC) or p[k * ld + r] (RC)
 template <class T> struct Operand {
     const T *p;
     int64_t ld;
     int rows;
-    int vec;
-    const float *skip;
 };
+
+// N elements from any address of their type (the hardware takes vector loads off their alignment)
+template <class T, int N> struct Pack { T e[N]; };
+template <class T, int N> __device__ __forceinline__ Pack<T, N> load_pack(const T *p)
+{
+    Pack<T, N> v;
+    __builtin_memcpy(&v, p, sizeof(v));
+    return v;
+}
+template <class T, int N> __device__ __forceinline__ void store_pack(T *p, const Pack<T, N> &v) { __builtin_memcpy(p, &v, sizeof(v)); }
+// the first n of them only (zeros behind)
+template <class T, int N> __device__ __forceinline__ Pack<T, N> load_some(const T *p, int n)
+{
+    if (n >= N) return load_pack<T, N>(p);
+    Pack<T, N> v;
+#pragma unroll
+    for (int e = 0; e < N; e++) v.e[e] = e < n ? p[e] : (T)0.f;
+    return v;
+}
+template <class T, int N> __device__ __forceinline__ void store_some(T *p, const Pack<T, N> &v, int n)
+{
+    if (n >= N) { store_pack(p, v); return; }
+#pragma unroll
+    for (int e = 0; e < N; e++)
+        if (e < n) p[e] = v.e[e];
+}
 
 // a thread's share of one K-step of R rows: global memory -> registers -> LDS
 template <class T, int R, int NT, bool RC> struct Stage {
@@ -72,7 +96,7 @@ template <class T, int R, int NT, bool RC> struct Stage {
                 const T *q = o.p + (int64_t)row * o.ld + k;
                 u32x4 x = {0, 0, 0, 0};
                 if (row < o.rows && k < k1) {
-                    if (o.vec && k + CE <= k1) x = *(const u32x4 *)q;
+                    if (k + CE <= k1) __builtin_memcpy(&x, q, 16);
                     else {
                         T e[CE];
 #pragma unroll
@@ -93,8 +117,8 @@ template <class T, int R, int NT, bool RC> struct Stage {
                     T f[VR];
 #pragma unroll
                     for (int s = 0; s < VR; s++) f[s] = (T)0.f;
-                    if (k + j < k1 && row < o.rows && !(o.skip && o.skip[k + j] == 0.f)) {
-                        if (o.vec && row + VR <= o.rows) __builtin_memcpy(f, __builtin_assume_aligned(q, VR * sizeof(T)), VR * sizeof(T));
+                    if (k + j < k1 && row < o.rows) {
+                        if (row + VR <= o.rows) __builtin_memcpy(f, q, VR * sizeof(T));
                         else {
 #pragma unroll
                             for (int s = 0; s < VR; s++)
@@ -130,7 +154,7 @@ template <class T, int R, int NT, bool RC> struct Stage {
 
 // the tile of C that a wave holds: MI x NI blocks of 32 x 32; block register e of a lane is row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32
 template <class T, int BM, int BN, int WM, int WN, bool RCA, bool RCB> struct Tile {
-    static constexpr int NT = 64 * WM * WN, MI = BM / WM / 32, NI = BN / WN / 32;
+    static constexpr int NT = 64 * WM * WN, WAVES_M = WM, WAVES_N = WN, MI = BM / WM / 32, NI = BN / WN / 32;
     static constexpr int LDS_CHUNKS = (BM + BN) * CHUNKS;
     f32x16 acc[MI][NI];
 
@@ -179,6 +203,183 @@ template <class T, int BM, int BN, int WM, int WN, bool RCA, bool RCB> struct Ti
     }
 };
 
+// ---- the same tile with operands that go from global memory to the LDS directly ---------------------------------------------------
+// For operands whose 16-byte chunks are aligned and whole (see direct()): buffer loads write the LDS without passing through registers,
+// out-of-range offsets give zeros.  The LDS place of a lane's chunk is fixed (base + 16 lane), so the swizzle is applied to the global
+// address.  A KC operand lies as in Tile; an RC operand lies as it is, STEP rows of k with R elements each, and is transposed on its way
+// out: 16-bit by the transposing LDS read (4 k x 16 rows per 16 lanes), 32-bit because an MFMA operand is one element per lane anyway.
+// Two stages: one is multiplied while the other is on its way; one barrier per step.
+constexpr unsigned NOWHERE = 0x7ffffff0u;   // an offset beyond every buffer (direct() keeps them below)
+
+template <class T, int R, int NT, bool RC> struct DirectOperand {
+    static constexpr int CE = Elem<T>::PER_CHUNK, STEP = Elem<T>::STEP, N = R * CHUNKS / NT, PER_K = R / CE;
+    const char *base;          // of the step to load next
+    int64_t bytes, advance;    // valid bytes from base on, per step
+    unsigned at[N];            // a lane's offset in a step
+    int first;                 // KC: the first k of its chunk (the same in all N: rows NT / 8 apart have the same swizzle)
+
+    // 16-byte blocks of an RC row are moved by whole bank groups: 64 bytes by k mod 4 (16-bit: a transposing read takes 4 k x 64 bytes at
+    // a time), 128 bytes by k / 4 (32-bit: the halves of a wave read k 4 apart)
+    static __device__ __forceinline__ int turn(int k) { return sizeof(T) == 2 ? (R >= 128 ? (k & 3) << 2 : (k & 1) << 2) : ((k >> 2) & 1) << 3; }
+
+    __device__ __forceinline__ void start(const Operand<T> &o, int r0, int k0, int k1, int tid)
+    {
+        const int64_t row_bytes = o.ld * (int64_t)sizeof(T);
+        if constexpr (!RC) {
+            const int rows = o.rows - r0 < R ? o.rows - r0 : R;
+            base = (const char *)(o.p + (int64_t)r0 * o.ld + k0);
+            bytes = (rows - 1) * row_bytes + (int64_t)(k1 - k0) * sizeof(T);
+            advance = ROW_BYTES;
+        } else {
+            base = (const char *)(o.p + (int64_t)k0 * o.ld + r0);
+            // (whole 4-byte words count as in or out of range: the last one belongs to the row even if only half of it does)
+            bytes = ((int64_t)(k1 - k0 - 1) * row_bytes + (int64_t)(o.rows - r0) * sizeof(T) + 3) & ~3ll;
+            advance = STEP * row_bytes;
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int p = i * NT + tid;
+            if constexpr (!RC) {
+                const int r = p >> 3, c = (p & 7) ^ sw(r);
+                at[i] = (unsigned)(r * row_bytes + c * 16);
+                first = c * CE;
+            } else {
+                const int k = p / PER_K, c = (p % PER_K) ^ turn(k);
+                at[i] = (unsigned)(k * row_bytes + c * 16);
+                first = 0;
+            }
+        }
+    }
+    // left: k still to come, this step's included
+    __device__ __forceinline__ void load(u32x4 *lds, int left, int wave)
+    {
+#ifdef __HIP_DEVICE_COMPILE__   // (the host pass does not know the buffer and LDS types)
+        const int64_t lim = bytes < (int64_t)NOWHERE ? bytes : (int64_t)NOWHERE;
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)(lim > 0 ? lim : 0), 0x00020000);
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)(lds + i * NT + wave * 64), 16,
+                                                     RC || first < left ? at[i] : NOWHERE, 0, 0, 0);
+#endif
+        base += advance;
+        bytes -= advance;
+    }
+};
+
+// reads the operands of an MFMA group (32 bytes of k, s = 0 .. 3) for M blocks of 32 rows: the lane's byte offsets in the operand's part of
+// a stage, so that everything else is a constant in the instruction
+template <class T, int R, bool RC, int M> struct Reader {
+    int at[RC ? M : CHUNKS / 2];
+
+    __device__ __forceinline__ void start(int row0, int lane, int where)
+    {
+        if constexpr (!RC) {
+            const int r = row0 + (lane & 31), c = (lane >> 5) ^ sw(r);
+#pragma unroll
+            for (int s = 0; s < CHUNKS / 2; s++) at[s] = where + r * ROW_BYTES + (c ^ (2 * s)) * 16;
+        } else {
+            typedef DirectOperand<T, R, 64, true> Op;
+            const int i = lane & 15, k = sizeof(T) == 2 ? 8 * (lane >> 5) + (i >> 2) : 4 * (lane >> 5);
+            const int row = sizeof(T) == 2 ? row0 + (lane & 16) + 4 * (i & 3) : row0 + (lane & 31);
+#pragma unroll
+            for (int m = 0; m < M; m++) at[m] = where + k * (R * (int)sizeof(T)) + (((row + 32 * m) * (int)sizeof(T)) ^ (Op::turn(k) * 16));
+        }
+    }
+    __device__ __forceinline__ void flip(int stage)
+    {
+#pragma unroll
+        for (int i = 0; i < (RC ? M : CHUNKS / 2); i++) at[i] ^= stage;
+    }
+    __device__ __forceinline__ u32x4 read(const u32x4 *lds, int m, int s) const
+    {
+#ifdef __HIP_DEVICE_COMPILE__
+        const __attribute__((address_space(3))) char *p = (const __attribute__((address_space(3))) char *)lds;
+        if constexpr (!RC) {
+            return *(const __attribute__((address_space(3))) u32x4 *)(p + at[s] + m * 32 * ROW_BYTES);
+        } else if constexpr (sizeof(T) == 2) {
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            s16x4 q[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                q[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p + at[m] + (16 * s + 4 * h) * (R * 2)));
+            u32x4 v;
+            __builtin_memcpy(&v, q, 16);
+            return v;
+        } else {
+            u32x4 v;
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = *(const __attribute__((address_space(3))) unsigned *)(p + at[m] + (8 * s + j) * (R * 4));
+            return v;
+        }
+#else
+        return u32x4{};
+#endif
+    }
+};
+
+template <class T, int BM, int BN, int WM, int WN, bool RCA, bool RCB> struct DirectTile {
+    static constexpr int NT = 64 * WM * WN, WAVES_M = WM, WAVES_N = WN, MI = BM / WM / 32, NI = BN / WN / 32, STAGE = (BM + BN) * CHUNKS;
+    static constexpr int LDS_CHUNKS = 2 * STAGE;
+    f32x16 acc[MI][NI];
+
+    static __device__ __forceinline__ int row(int wave, int lane, int mi, int e) { return (wave / WN) * (BM / WM) + mi * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3); }
+    static __device__ __forceinline__ int col(int wave, int lane, int ni) { return (wave % WN) * (BN / WN) + ni * 32 + (lane & 31); }
+
+    __device__ __forceinline__ void mainloop(const Operand<T> &a, const Operand<T> &b, int i0, int j0, int k0, int k1, u32x4 *lds)
+    {
+        const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+#pragma unroll
+        for (int mi = 0; mi < MI; mi++)
+#pragma unroll
+            for (int ni = 0; ni < NI; ni++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[mi][ni][e] = 0.f;
+        if (k0 >= k1) return;
+        DirectOperand<T, BM, NT, RCA> oa;
+        DirectOperand<T, BN, NT, RCB> ob;
+        oa.start(a, i0, k0, k1, tid);
+        ob.start(b, j0, k0, k1, tid);
+        __syncthreads();                     // (a tile before this one has been read)
+        oa.load(lds, k1 - k0, wave);
+        ob.load(lds + BM * CHUNKS, k1 - k0, wave);
+        Reader<T, BM, RCA, MI> xa;
+        Reader<T, BN, RCB, NI> xb;
+        xa.start((wave / WN) * (BM / WM), lane, 0);
+        xb.start((wave % WN) * (BN / WN), lane, BM * ROW_BYTES);
+        int other = STAGE;
+        for (int k = k0; k < k1; k += Elem<T>::STEP) {
+            __syncthreads();                 // this step has arrived, and the stage of the one before has been read
+            const int left = k1 - k - Elem<T>::STEP;
+            if (left > 0) {
+                oa.load(lds + other, left, wave);
+                ob.load(lds + other + BM * CHUNKS, left, wave);
+            }
+            // operands of the next group are read while this one is multiplied
+            u32x4 fa[2][MI], fb[2][NI];
+#pragma unroll
+            for (int mi = 0; mi < MI; mi++) fa[0][mi] = xa.read(lds, mi, 0);
+#pragma unroll
+            for (int ni = 0; ni < NI; ni++) fb[0][ni] = xb.read(lds, ni, 0);
+#pragma unroll
+            for (int s = 0; s < CHUNKS / 2; s++) {
+                if (s + 1 < CHUNKS / 2) {
+#pragma unroll
+                    for (int mi = 0; mi < MI; mi++) fa[(s + 1) & 1][mi] = xa.read(lds, mi, s + 1);
+#pragma unroll
+                    for (int ni = 0; ni < NI; ni++) fb[(s + 1) & 1][ni] = xb.read(lds, ni, s + 1);
+                }
+#pragma unroll
+                for (int mi = 0; mi < MI; mi++)
+#pragma unroll
+                    for (int ni = 0; ni < NI; ni++) acc[mi][ni] = mma((T)0.f, fa[s & 1][mi], fb[s & 1][ni], acc[mi][ni]);
+            }
+            xa.flip(STAGE * 16);
+            xb.flip(STAGE * 16);
+            other ^= STAGE;
+        }
+    }
+};
+
 // workgroup -> tile.  Consecutive workgroups go to the 8 XCDs in turn, each with an L2 of its own: XCD x gets a contiguous share of
 // the tiles, walked in groups of 8 tile rows, so that what its workgroups read at one time overlaps.
 __device__ __forceinline__ void tile_of(int id, int count, int tiles_i, int tiles_j, int &ti, int &tj)
@@ -191,40 +392,80 @@ __device__ __forceinline__ void tile_of(int id, int count, int tiles_i, int tile
 }
 
 // ---- activations ---------------------------------------------------------------------------------------------------------------
+// Phi(z) and e = exp(-z^2 / 2) (its density is 0.3989 e): Phi(-|z|) = 1/2 erfcx(|z| / sqrt 2) e, erfcx as a polynomial of degree 9 in
+// t = 1 / (1 + 0.3 x) (weighted least squares on x in [0, 14]: relative error 4e-8; behind it e is 0).  A sixth of erfcf's instructions.
+__device__ __forceinline__ float normal_cdf(float z, float &e)
+{
+    const float a = __builtin_fabsf(z);
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.21213203435596426f, a, 1.f));
+    float q = -0.12661783397197723f;
+    q = __builtin_fmaf(q, t, 0.471831738948822f);
+    q = __builtin_fmaf(q, t, -0.4847019910812378f);
+    q = __builtin_fmaf(q, t, 0.5170591473579407f);
+    q = __builtin_fmaf(q, t, -0.07405535876750946f);
+    q = __builtin_fmaf(q, t, 0.206387460231781f);
+    q = __builtin_fmaf(q, t, 0.1504683643579483f);
+    q = __builtin_fmaf(q, t, 0.17042377591133118f);
+    q = __builtin_fmaf(q, t, 0.16920475661754608f);
+    e = __expf(-0.5f * z * z);
+    const float tail = 0.5f * q * t * e;
+    return z > 0.f ? 1.f - tail : tail;
+}
+__device__ __forceinline__ float logistic(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
 __device__ __forceinline__ float act_value(int act, float z)
 {
+    float e;
     switch (act) {
     case NIRRT_NN_ACT_RELU: return z > 0.f ? z : (z == z ? 0.f : z);          // (NaN stays)
-    case NIRRT_NN_ACT_GELU: return 0.5f * z * erfcf(z * -0.70710678118654752f);
-    case NIRRT_NN_ACT_SILU: return z / (1.f + __expf(-z));
+    case NIRRT_NN_ACT_GELU: return z * normal_cdf(z, e);
+    case NIRRT_NN_ACT_SILU: return z * logistic(z);
     default: return z;
     }
 }
 __device__ __forceinline__ float act_slope(int act, float z)
 {
+    float e;
     switch (act) {
     case NIRRT_NN_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-    case NIRRT_NN_ACT_GELU: return 0.5f * erfcf(z * -0.70710678118654752f) + z * 0.39894228040143268f * __expf(-0.5f * z * z);
-    case NIRRT_NN_ACT_SILU: { const float s = 1.f / (1.f + __expf(-z)); return s * (1.f + z * (1.f - s)); }
+    case NIRRT_NN_ACT_GELU: { const float c = normal_cdf(z, e); return __builtin_fmaf(z * 0.39894228040143268f, e, c); }
+    case NIRRT_NN_ACT_SILU: { const float s = logistic(z); return s * (1.f + z * (1.f - s)); }
     default: return 1.f;
     }
 }
 
-// ---- what a product does with an element of C ------------------------------------------------------------------------------------
+// ---- what a product does with four neighbouring elements C[i, j ..] (n of them, 1 .. 4, exist) ---------------------------------------
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+template <class T> __device__ __forceinline__ f32x4 load4(const T *p, int n)
+{
+    const Pack<T, 4> q = load_some<T, 4>(p, n);
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = (float)q.e[e];
+    return v;
+}
+template <class T> __device__ __forceinline__ void store4(T *p, f32x4 v, int n)
+{
+    Pack<T, 4> q;
+#pragma unroll
+    for (int e = 0; e < 4; e++) q.e[e] = (T)v[e];
+    store_some(p, q, n);
+}
 // y = act(C + b[j]) + r, and z
 template <class T> struct EpiLinear {
     const T *b, *r;
     T *y, *z;
     int64_t ldr, ldy;
     int act, n;
-    __device__ __forceinline__ float column(int j) const { return b ? (float)b[j] : 0.f; }
-    __device__ __forceinline__ void put(float c, float col, int i, int j) const
+    __device__ __forceinline__ void put(f32x4 c, int i, int j, int cnt) const
     {
-        const float v = c + col;
-        if (z) z[(int64_t)i * n + j] = (T)v;
-        float o = act_value(act, v);
-        if (r) o += (float)r[(int64_t)i * ldr + j];
-        y[(int64_t)i * ldy + j] = (T)o;
+        if (b) c += load4(b + j, cnt);
+        if (z) store4(z + (int64_t)i * n + j, c, cnt);
+        if (act != NIRRT_NN_ACT_NONE) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) c[e] = act_value(act, c[e]);
+        }
+        if (r) c += load4(r + (int64_t)i * ldr + j, cnt);
+        store4(y + (int64_t)i * ldy + j, c, cnt);
     }
 };
 // out = scale C (contiguous rows of n); scale on the device or 1
@@ -233,88 +474,128 @@ template <class T> struct EpiPlain {
     const float *scale;
     float factor;
     int n;
-    __device__ __forceinline__ float column(int) const { return scale ? *scale * factor : factor; }
-    __device__ __forceinline__ void put(float c, float col, int i, int j) const { out[(int64_t)i * n + j] = (T)(c * col); }
+    __device__ __forceinline__ void put(f32x4 c, int i, int j, int cnt) const { store4(out + (int64_t)i * n + j, c * (scale ? *scale * factor : factor), cnt); }
 };
 // acc (+)= C in fp32: the sum over pieces of the reduction that are multiplied one after the other
-struct EpiAccumulate {
+template <class T> struct EpiAccumulate {
     float *out;
     int n, first;
-    __device__ __forceinline__ float column(int) const { return 0.f; }
-    __device__ __forceinline__ void put(float c, float, int i, int j) const
+    __device__ __forceinline__ void put(f32x4 c, int i, int j, int cnt) const
     {
         float *q = out + (int64_t)i * n + j;
-        *q = first ? c : *q + c;
+        store4(q, first ? c : c + load4(q, cnt), cnt);
     }
 };
 
-// BM x BN tiles, the reduction cut into gridDim.y parts of `part`; with more than one, the parts go to `partial` (part, i, j) for k_join
-template <class T, int BM, int BN, int WM, int WN, bool RCA, bool RCB, class Epi>
-__global__ __launch_bounds__(64 * WM * WN) void k_gemm(Operand<T> a, Operand<T> b, int m, int n, int k, int part, float *partial, Epi epi)
+// BM x BN tiles, the reduction cut into gridDim.y parts of `part`; with more than one, the parts go to `partial` (part, i, j) for k_join.
+// A wave hands its accumulators to the epilogue through the LDS, 32 rows at a time: an MFMA block has a row's elements in 32 lanes, the
+// epilogue wants four of a row in one (16-byte accesses, and code once instead of once per accumulator register).
+template <class T, int BM, int BN, class Tl, class Epi>
+__global__ __launch_bounds__(Tl::NT) void k_gemm(Operand<T> a, Operand<T> b, int m, int n, int k, int part, float *partial, Epi epi)
 {
-    typedef Tile<T, BM, BN, WM, WN, RCA, RCB> Tl;
-    __shared__ u32x4 lds[Tl::LDS_CHUNKS];
+    constexpr int COLS = Tl::NI * 32, LD = COLS + 4, SLAB = 32 * LD / 4;      // (4 more: rows 4 apart start in other banks)
+    __shared__ u32x4 lds[Tl::LDS_CHUNKS > SLAB * (Tl::NT / 64) ? Tl::LDS_CHUNKS : SLAB * (Tl::NT / 64)];
     Tl t;
     int ti, tj;
     tile_of(blockIdx.x, gridDim.x, (m + BM - 1) / BM, (n + BN - 1) / BN, ti, tj);
     const int k0 = blockIdx.y * part, k1 = k - k0 < part ? k : k0 + part;
     t.mainloop(a, b, ti * BM, tj * BN, k0, k1, lds);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    float *pp = partial + (gridDim.y > 1 ? (int64_t)blockIdx.y * m * n : 0);
+    float *pp = gridDim.y > 1 ? partial + (int64_t)blockIdx.y * m * n : nullptr;
+    const int i0 = ti * BM + Tl::row(wave, 0, 0, 0), j0 = tj * BN + Tl::col(wave, 0, 0);
+    float *slab = (float *)(lds + wave * SLAB);
+    __syncthreads();                        // (the last step has been read)
 #pragma unroll
-    for (int ni = 0; ni < Tl::NI; ni++) {
-        const int j = tj * BN + Tl::col(wave, lane, ni);
-        if (j >= n) continue;
-        const float col = epi.column(j);
+    for (int mi = 0; mi < Tl::MI; mi++) {
 #pragma unroll
-        for (int mi = 0; mi < Tl::MI; mi++)
+        for (int ni = 0; ni < Tl::NI; ni++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int i = ti * BM + Tl::row(wave, lane, mi, e);
-                if (i >= m) continue;
-                if (gridDim.y > 1) pp[(int64_t)i * n + j] = t.acc[mi][ni][e];
-                else epi.put(t.acc[mi][ni][e], col, i, j);
+            for (int e = 0; e < 16; e++) slab[(8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * LD + ni * 32 + (lane & 31)] = t.acc[mi][ni][e];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 2
+        for (int q = 0; q < COLS / 8; q++) {
+            const int at = q * 64 + lane, r = at / (COLS / 4), c = at % (COLS / 4) * 4, i = i0 + 32 * mi + r, j = j0 + c;
+            const f32x4 v = *(const f32x4 *)(slab + r * LD + c);
+            if (i < m && j < n) {
+                const int cnt = n - j < 4 ? n - j : 4;
+                if (pp) store4(pp + (int64_t)i * n + j, v, cnt);
+                else epi.put(v, i, j, cnt);
             }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
 }
 // the parts of a cut reduction, added in their order
 template <class Epi> __global__ __launch_bounds__(256) void k_join(const float *partial, int parts, int m, int n, Epi epi)
 {
-    const int64_t size = (int64_t)m * n;
-    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < size; at += (int64_t)gridDim.x * 256) {
-        float s = 0.f;
-        for (int p = 0; p < parts; p++) s += partial[p * size + at];
-        const int i = (int)(at / n), j = (int)(at - (int64_t)i * n);
-        epi.put(s, epi.column(j), i, j);
+    const int64_t size = (int64_t)m * n, quads = (n + 3) / 4, all = m * quads;
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < all; at += (int64_t)gridDim.x * 256) {
+        const int i = (int)(at / quads), j = (int)(at - i * quads) * 4, cnt = n - j < 4 ? n - j : 4;
+        const float *p = partial + (int64_t)i * n + j;
+        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int q = 0; q < parts; q++) s += load4(p + q * size, cnt);
+        epi.put(s, i, j, cnt);
     }
 }
 
 // ---- dz = dy act'(z) and its column sums -------------------------------------------------------------------------------------------
-// grid (column blocks of 256, row chunks): a thread walks its column of the chunk
+// grid (column blocks, row chunks).  A row's 16-byte packs lie on `lanes` (a power of two) neighbouring lanes, 256 / lanes rows at a time;
+// a lane keeps the sums of its columns over the chunk, the rows' lanes meet in the LDS: sums (chunk, column), joined by k_column_join.
 template <class T>
-__global__ __launch_bounds__(256) void k_dz(const T *z, const T *dy, int64_t lddy, T *dz, float *sums, int m, int n, int chunk, int act)
+__global__ __launch_bounds__(256) void k_dz(const T *z, const T *dy, int64_t lddy, T *dz, float *sums, int m, int n, int chunk, int lanes, int act)
 {
-    const int j = blockIdx.x * 256 + threadIdx.x;
-    if (j >= n) return;
-    const int i0 = blockIdx.y * chunk, i1 = m - i0 < chunk ? m : i0 + chunk;
-    float s = 0.f;
-    for (int i = i0; i < i1; i++) {
-        float d = (float)dy[(int64_t)i * lddy + j];
-        if (act != NIRRT_NN_ACT_NONE) {
-            d *= act_slope(act, (float)z[(int64_t)i * n + j]);
-            if (dz) dz[(int64_t)i * n + j] = (T)d;
+    constexpr int V = 16 / sizeof(T);
+    __shared__ float meet[256 * V];
+    const int l = threadIdx.x & (lanes - 1), rr = threadIdx.x / lanes, step = 256 / lanes, j = (blockIdx.x * lanes + l) * V;
+    const int i0 = blockIdx.y * chunk, i1 = m - i0 < chunk ? m : i0 + chunk, cnt = n - j < V ? n - j : V;
+    float s[V];
+#pragma unroll
+    for (int e = 0; e < V; e++) s[e] = 0.f;
+    if (cnt > 0)
+#pragma unroll 2
+        for (int i = i0 + rr; i < i1; i += step) {
+            Pack<T, V> d = load_some<T, V>(dy + (int64_t)i * lddy + j, cnt);
+            if (act != NIRRT_NN_ACT_NONE) {
+                const Pack<T, V> q = load_some<T, V>(z + (int64_t)i * n + j, cnt);
+#pragma unroll
+                for (int e = 0; e < V; e++) {
+                    const float v = (float)d.e[e] * act_slope(act, (float)q.e[e]);
+                    s[e] += v;
+                    d.e[e] = (T)v;
+                }
+                if (dz) store_some(dz + (int64_t)i * n + j, d, cnt);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; e++) s[e] += (float)d.e[e];
+            }
         }
-        s += d;
+    if (!sums) return;
+#pragma unroll
+    for (int e = 0; e < V; e++) meet[threadIdx.x * V + e] = s[e];
+    __syncthreads();
+    for (int c = threadIdx.x; c < lanes * V; c += 256) {
+        float a = 0.f;
+        for (int r = 0; r < step; r++) a += meet[r * lanes * V + c];
+        const int col = blockIdx.x * lanes * V + c;
+        if (col < n) sums[(int64_t)blockIdx.y * n + col] = a;
     }
-    if (sums) sums[(int64_t)blockIdx.y * n + j] = s;
 }
-template <class T> __global__ __launch_bounds__(256) void k_column_join(const float *sums, int parts, T *out, int n)
+// out[j] = factor scale sum over parts of sums[p, j], in a fixed order: 64 columns x 4 shares of the parts per workgroup
+template <class T> __global__ __launch_bounds__(256) void k_column_join(const float *sums, int parts, const float *scale, float factor, T *out, int64_t n)
 {
-    const int j = blockIdx.x * 256 + threadIdx.x;
-    if (j >= n) return;
+    __shared__ float meet[4][64];
+    const int64_t j = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
     float s = 0.f;
-    for (int p = 0; p < parts; p++) s += sums[(int64_t)p * n + j];
-    out[j] = (T)s;
+    if (j < n)
+#pragma unroll 8
+        for (int p = threadIdx.x >> 6; p < parts; p += 4) s += sums[p * n + j];
+    meet[threadIdx.x >> 6][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (threadIdx.x < 64 && j < n)
+        out[j] = (T)(((meet[0][threadIdx.x] + meet[1][threadIdx.x]) + (meet[2][threadIdx.x] + meet[3][threadIdx.x])) * (scale ? *scale * factor : factor));
 }
 
 // ---- cross entropy -----------------------------------------------------------------------------------------------------------------
@@ -325,57 +606,77 @@ __device__ __forceinline__ float row_weight(const float *cw, int64_t t, int64_t 
     return cw ? cw[t] : 1.f;
 }
 
+constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
+
 // C[v, r] = w_v . x_r: a lane holds scores of NI rows r (its columns), so the running maximum and sum over the classes stay in the
 // lane; the two halves of a wave and the waves above one another meet once, at the end.  grid (row tiles, parts of the classes).
-template <class T, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void k_ce_stats(Operand<T> w, Operand<T> x, const T *b, const int64_t *target, int rows, int classes,
+template <class T, int BM, int BN, class Tl>
+__global__ __launch_bounds__(Tl::NT) void k_ce_stats(Operand<T> w, Operand<T> x, const T *b, const int64_t *target, int rows, int classes,
                                                            int k, int part, float2 *stats, float *target_score)
 {
-    typedef Tile<T, BM, BN, WM, WN, false, false> Tl;
+    constexpr int WM = Tl::WAVES_M, WN = Tl::WAVES_N;
     __shared__ u32x4 lds[Tl::LDS_CHUNKS];
     __shared__ float2 meet[2 * WM][BN];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r0 = blockIdx.x * BN;
-    float m[Tl::NI], s[Tl::NI];
-    int64_t tg[Tl::NI];
+    __shared__ __attribute__((aligned(16))) float add[BM];   // log2(e) b of the tile's classes, -inf behind the last
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r0 = blockIdx.x * BN, top_row = Tl::row(wave, lane, 0, 0);
+    float m[Tl::NI], s[Tl::NI], mine[Tl::NI];                 // everything in units of log2: one fma and one exp2 per score
+    int tg[Tl::NI];
 #pragma unroll
     for (int ni = 0; ni < Tl::NI; ni++) {
         m[ni] = -__builtin_inff();
-        s[ni] = 0.f;
+        s[ni] = mine[ni] = 0.f;
         const int r = r0 + Tl::col(wave, lane, ni);
-        tg[ni] = r < rows ? target[r] : -1;
+        const int64_t t = r < rows ? target[r] : -1;
+        tg[ni] = t >= 0 && t < classes ? (int)t : -1;
     }
     const int v_end = classes - (int)blockIdx.y * part < part ? classes : ((int)blockIdx.y + 1) * part;
     for (int v0 = blockIdx.y * part; v0 < v_end; v0 += BM) {
         Tl t;
+        __syncthreads();                                     // (the tile before has been added)
+        for (int c = threadIdx.x; c < BM; c += Tl::NT) add[c] = v0 + c < v_end ? (b ? LOG2E * (float)b[v0 + c] : 0.f) : -__builtin_inff();
         t.mainloop(w, x, v0, r0, 0, k, lds);
+        if (k == 0) __syncthreads();                         // (otherwise the products' barriers stand between)
 #pragma unroll
         for (int mi = 0; mi < Tl::MI; mi++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int v = v0 + Tl::row(wave, lane, mi, e);
-                const float add = v < v_end ? (b ? (float)b[v] : 0.f) : -__builtin_inff();
+            for (int q = 0; q < 4; q++) {
+                const f32x4 bb = *(const f32x4 *)(add + top_row + mi * 32 + 8 * q);
 #pragma unroll
-                for (int ni = 0; ni < Tl::NI; ni++) t.acc[mi][ni][e] = v < v_end ? t.acc[mi][ni][e] + add : add;
+                for (int ni = 0; ni < Tl::NI; ni++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) t.acc[mi][ni][4 * q + e] = __builtin_fmaf(t.acc[mi][ni][4 * q + e], LOG2E, bb[e]);
             }
 #pragma unroll
         for (int ni = 0; ni < Tl::NI; ni++) {
             float top = m[ni];
-            const int64_t want = tg[ni] - v0;
 #pragma unroll
             for (int mi = 0; mi < Tl::MI; mi++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) top = fmaxf(top, t.acc[mi][ni][e]);
-            float sum = 0.f;
             const float ref = top == -__builtin_inff() ? 0.f : top;   // (nothing but -inf so far: exp(-inf) adds zeros)
+            const int want = tg[ni] - v0 - top_row;
+            if (__ballot(tg[ni] >= v0 && tg[ni] < v0 + BM)) {         // a row of this wave has its target in the tile
+#pragma unroll
+                for (int mi = 0; mi < Tl::MI; mi++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) mine[ni] = want == mi * 32 + 8 * (e >> 2) + (e & 3) ? t.acc[mi][ni][e] : mine[ni];
+            }
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int mi = 0; mi < Tl::MI; mi++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    sum += __expf(t.acc[mi][ni][e] - ref);
-                    if (want == Tl::row(wave, lane, mi, e) && want < v_end - v0) target_score[r0 + Tl::col(wave, lane, ni)] = t.acc[mi][ni][e];
-                }
-            s[ni] = s[ni] * __expf(m[ni] - ref) + sum;
+                for (int e = 0; e < 16; e++) sum[e & 3] += __builtin_amdgcn_exp2f(t.acc[mi][ni][e] - ref);
+            s[ni] = s[ni] * __builtin_amdgcn_exp2f(m[ni] - ref) + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
             m[ni] = top;
+        }
+    }
+    // the lane that met a row's target leaves its score: its share of the classes holds 4-row groups 8 apart from its own row on
+#pragma unroll
+    for (int ni = 0; ni < Tl::NI; ni++) {
+        const int in = tg[ni] - (int)blockIdx.y * part;
+        if (tg[ni] >= 0 && in >= 0 && tg[ni] < v_end) {
+            const int at = in % BM - top_row;
+            if (at >= 0 && at < Tl::MI * 32 && (at & 7) < 4) target_score[r0 + Tl::col(wave, lane, ni)] = mine[ni] * LN2;
         }
     }
 #pragma unroll
@@ -387,7 +688,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_ce_stats(Operand<T> w, Operand
         for (int p = 0; p < 2 * WM; p++) top = fmaxf(top, meet[p][c].x);
         const float ref = top == -__builtin_inff() ? 0.f : top;
 #pragma unroll
-        for (int p = 0; p < 2 * WM; p++) sum += meet[p][c].y * __expf(meet[p][c].x - ref);
+        for (int p = 0; p < 2 * WM; p++) sum += meet[p][c].y * __builtin_amdgcn_exp2f(meet[p][c].x - ref);
         if (r0 + c < rows) stats[(int64_t)blockIdx.y * rows + r0 + c] = make_float2(top, sum);
     }
 }
@@ -402,8 +703,8 @@ __global__ __launch_bounds__(256) void k_ce_rows(const float2 *stats, int parts,
         float top = -__builtin_inff(), sum = 0.f;
         for (int p = 0; p < parts; p++) top = fmaxf(top, stats[(int64_t)p * rows + r].x);
         const float ref = top == -__builtin_inff() ? 0.f : top;
-        for (int p = 0; p < parts; p++) { const float2 q = stats[(int64_t)p * rows + r]; sum += q.y * __expf(q.x - ref); }
-        const float l = top + logf(sum);
+        for (int p = 0; p < parts; p++) { const float2 q = stats[(int64_t)p * rows + r]; sum += q.y * __builtin_amdgcn_exp2f(q.x - ref); }
+        const float l = (top + __builtin_amdgcn_logf(sum)) * LN2;
         const int64_t t = target[r];
         const float wt = row_weight(cw, t, ignore, classes);
         const float loss = t == ignore ? 0.f : (wt == wt ? wt * (l - target_score[r]) : wt);
@@ -436,54 +737,85 @@ __global__ __launch_bounds__(256) void k_ce_total(const double *sums, int blocks
         total[2] = (float)(a / b);          // (no row counts: 0 / 0)
     }
 }
-// c_r = dloss_r weight_r (/ total weight): rel[r] = c_r / max |c|, scale[0] = max |c|; one workgroup
-__global__ __launch_bounds__(1024) void k_ce_coefficients(const float *dloss, int stride, const float *total, const int64_t *target, const float *cw,
-                                                          int64_t ignore, int rows, int classes, float *rel, float *scale)
+// c_r = dloss_r weight_r (/ total weight), 0 where ignored
+__device__ __forceinline__ float row_coefficient(const float *dloss, int stride, const float *total, const int64_t *target, const float *cw,
+                                                 int64_t ignore, int classes, int64_t r)
 {
-    __shared__ float part[16];
-    const float div = total ? 1.f / total[1] : 1.f;
-    float top = 0.f;
-    bool bad = false;
-    for (int r = threadIdx.x; r < rows; r += 1024) {
-        const int64_t t = target[r];
-        const float c = t == ignore ? 0.f : dloss[stride ? r : 0] * row_weight(cw, t, ignore, classes) * div;
-        rel[r] = c;
-        bad = bad || c != c;
-        top = fmaxf(top, fabsf(c));
-    }
-    if (bad) top = __builtin_inff();            // (a NaN row: the scale says so below)
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
-    __syncthreads();
-    top = part[0];
-#pragma unroll
-    for (int p = 1; p < 16; p++) top = fmaxf(top, part[p]);
-    // no row counts, or something is not finite: rel keeps the coefficients themselves
-    const bool usable = top > 0.f && top < __builtin_inff();
-    if (usable)
-        for (int r = threadIdx.x; r < rows; r += 1024) rel[r] = rel[r] / top;
-    if (threadIdx.x == 0) scale[0] = usable ? top : 1.f;
+    const int64_t t = target[r];
+    if (t == ignore) return 0.f;
+    const float c = dloss[stride ? r : 0] * row_weight(cw, t, ignore, classes);
+    return total ? c / total[1] : c;
 }
-// g' = rel_r (exp(l - lse_r) - [v = target]) FACTOR in the element type, stored (v, r): the product C[v, r] again.  16-bit products need
-// 16-bit operands; rel <= 1 keeps the range, and FACTOR 4096 in f16 lifts probabilities of large vocabularies (1e-5) out of its
-// subnormals.  Relative error of a rounding: 2^-9 (bf16), 2^-12 (f16) of the element, like the rounding of dz in the linear layer.
+__device__ __forceinline__ float block_max(float v, float *part)   // 256 threads
+{
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+}
+__global__ __launch_bounds__(256) void k_ce_coefficients(const float *dloss, int stride, const float *total, const int64_t *target, const float *cw,
+                                                         int64_t ignore, int rows, int classes, float *coef, float *tops)
+{
+    __shared__ float part[4];
+    const int r = blockIdx.x * 256 + threadIdx.x;
+    const float c = r < rows ? row_coefficient(dloss, stride, total, target, cw, ignore, classes, r) : 0.f;
+    if (r < rows) coef[r] = c;
+    const float top = block_max(fabsf(c), part);      // (a NaN does not count here: it is in coef)
+    if (threadIdx.x == 0) tops[blockIdx.x] = top;
+}
+// scale = the largest |c| (1 if no row counts or it is infinite): {scale, 1 / scale}
+__global__ __launch_bounds__(256) void k_ce_scale(const float *tops, int blocks, float *scale)
+{
+    __shared__ float part[4];
+    float top = 0.f;
+    for (int i = threadIdx.x; i < blocks; i += 256) top = fmaxf(top, tops[i]);
+    top = block_max(top, part);
+    if (threadIdx.x == 0) {
+        const bool usable = top > 1e-30f && top < __builtin_inff();
+        scale[0] = usable ? top : 1.f;
+        scale[1] = usable ? 1.f / top : 1.f;
+    }
+}
+// x with the rows that do not count set to zero (whatever they hold: 0 x NaN must not reach dw) and its rows padded with zeros to ld, so
+// that whole aligned chunks can be read; one pass over x, a small part of the products behind it
+template <class T>
+__global__ __launch_bounds__(256) void k_ce_rows_copy(const T *x, int64_t ldx, const float *coef, T *out, int64_t ld, int rows, int k)
+{
+    constexpr int V = 16 / sizeof(T);
+    const int64_t per = ld / V, all = rows * per;
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < all; at += (int64_t)gridDim.x * 256) {
+        const int64_t r = at / per;
+        const int c = (int)(at - r * per) * V;
+        Pack<T, V> v = {};
+        if (!coef || coef[r] != 0.f) v = load_some<T, V>(x + r * ldx + c, k - c);
+        store_pack(out + r * ld + c, v);
+    }
+}
+// g' = c_r / scale (exp(l - lse_r) - [v = target]) FACTOR in the element type, stored (v, r): the product C[v, r] again.  16-bit products
+// need 16-bit operands; c / scale <= 1 keeps the range, and FACTOR 4096 in f16 lifts probabilities of large vocabularies (1e-5) out of
+// its subnormals.  Relative error of a rounding: 2^-9 (bf16), 2^-12 (f16) of the element, like the rounding of dz in the linear layer.
 template <class T> struct Factor { static constexpr float VALUE = 1.f; };
 template <> struct Factor<f16_t> { static constexpr float VALUE = 4096.f; };
 template <class T> struct EpiSoftmaxGrad {
     T *g;
     int64_t ldg;
     const T *b;
-    const float *lse, *rel;
+    const float *lse, *coef, *scale;
     const int64_t *target;
     int64_t v0;
-    __device__ __forceinline__ float column(int) const { return 0.f; }
-    __device__ __forceinline__ void put(float c, float, int i, int j) const
+    __device__ __forceinline__ void put(f32x4 c, int i, int j, int cnt) const
     {
-        const float coef = rel[j];
-        float p = __expf(c + (b ? (float)b[v0 + i] : 0.f) - lse[j]);
-        if (target[j] == v0 + i) p -= 1.f;
-        g[(int64_t)i * ldg + j] = coef == 0.f ? (T)0.f : (T)(p * coef * Factor<T>::VALUE);
+        const float add = b ? (float)b[v0 + i] : 0.f, lift = scale[1] * Factor<T>::VALUE;
+        const f32x4 l = load4(lse + j, cnt), w = load4(coef + j, cnt);
+        f32x4 o;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            float p = __expf(c[e] + add - l[e]);
+            if (e < cnt && target[j + e] == v0 + i) p -= 1.f;
+            o[e] = w[e] == 0.f ? 0.f : p * (w[e] * lift);
+        }
+        store4(g + (int64_t)i * ldg + j, o, cnt);
     }
 };
 // db[v] = scale / FACTOR sum_r g'[v, r]: a wave per class
@@ -497,6 +829,179 @@ template <class T> __global__ __launch_bounds__(256) void k_ce_bias(const T *g, 
     for (int d = 32; d > 0; d >>= 1) s += __shfl_down(s, d);
     if ((threadIdx.x & 63) == 0) db[v] = (T)(s * *scale * (1.f / Factor<T>::VALUE));
 }
+// ---- cross entropy of few classes (V <= 8): one pass over x forward, one backward ------------------------------------------------------
+// Two classes and 128 inputs are what the guidance network's head has: a tile of 64 classes would be empty but for two, and what bounds the
+// operator is reading x (forward) and reading x and writing dx (backward).  A row's 16-byte packs lie on G neighbouring lanes (64 / G rows
+// per wave, NC packs per lane), the scores are summed over the G lanes with shuffles, everything in fp32; backward, a lane keeps dw of its
+// columns over all rows of the workgroup, and the workgroups' shares are joined in a fixed order.
+template <class T, int V, int NC> struct FewRow {
+    static constexpr int P = 16 / sizeof(T);
+    float x[NC * P];
+    __device__ __forceinline__ void load(const T *row, int k, int g, int G, bool on)
+    {
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            const int at = (c * G + g) * P;
+            Pack<T, P> v = {};
+            if (on && at < k) v = load_some<T, P>(row + at, k - at);
+#pragma unroll
+            for (int e = 0; e < P; e++) x[c * P + e] = (float)v.e[e];
+        }
+    }
+    // scores of the classes below `classes` (the others -inf), in all G lanes; w (class, padded k) in the LDS
+    __device__ __forceinline__ void scores(const float *w, const float *bias, int kp, int classes, int g, int G, float *l) const
+    {
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            float s = 0.f;
+            if (v < classes)
+#pragma unroll
+                for (int c = 0; c < NC; c++)
+#pragma unroll
+                    for (int e = 0; e < P; e += 4) {
+                        const f32x4 q = *(const f32x4 *)(w + v * kp + (c * G + g) * P + e);
+#pragma unroll
+                        for (int d = 0; d < 4; d++) s = __builtin_fmaf(x[c * P + e + d], q[d], s);
+                    }
+            l[v] = s;
+        }
+        for (int d = 1; d < G; d <<= 1)
+#pragma unroll
+            for (int v = 0; v < V; v++) l[v] += __shfl_xor(l[v], d);
+#pragma unroll
+        for (int v = 0; v < V; v++) l[v] = v < classes ? l[v] + bias[v] : -__builtin_inff();
+    }
+};
+template <class T> __device__ __forceinline__ void few_weights(const T *w, int64_t ldw, const T *b, int classes, int k, int kp, float *lw, float *lb)
+{
+    for (int at = threadIdx.x; at < classes * kp; at += 256) {
+        const int v = at / kp, c = at - v * kp;
+        lw[at] = c < k ? (float)w[v * ldw + c] : 0.f;
+    }
+    if (threadIdx.x < (unsigned)classes) lb[threadIdx.x] = b ? (float)b[threadIdx.x] : 0.f;
+    __syncthreads();
+}
+template <class T, int V, int NC>
+__global__ __launch_bounds__(256) void k_ce_few(const T *x, int64_t ldx, const T *w, int64_t ldw, const T *b, const int64_t *target, const float *cw,
+                                                int64_t ignore, int rows, int classes, int k, int G, float *lse, float *nll, double *sums)
+{
+    extern __shared__ float few[];           // classes x kp weights, V biases
+    __shared__ double part[2][4];
+    const int kp = NC * G * FewRow<T, V, NC>::P, lane = threadIdx.x & 63, g = lane & (G - 1), per = 256 / G;
+    float *lb = few + classes * kp;
+    few_weights(w, ldw, b, classes, k, kp, few, lb);
+    double a = 0., n = 0.;
+    for (int r0 = blockIdx.x * per; r0 < rows; r0 += gridDim.x * per) {
+        const int r = r0 + threadIdx.x / G;
+        FewRow<T, V, NC> q;
+        float l[V];
+        q.load(x + (int64_t)r * ldx, k, g, G, r < rows);
+        q.scores(few, lb, kp, classes, g, G, l);
+        if (r < rows && g == 0) {
+            float top = -__builtin_inff(), sum = 0.f, mine = 0.f;
+            const int64_t t = target[r];
+#pragma unroll
+            for (int v = 0; v < V; v++) top = fmaxf(top, l[v]);
+            const float ref = top == -__builtin_inff() ? 0.f : top;
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                sum += v < classes ? __expf(l[v] - ref) : 0.f;
+                if (t == v) mine = l[v];
+            }
+            const float z = top + logf(sum), wt = row_weight(cw, t, ignore, classes);
+            const float loss = t == ignore ? 0.f : (wt == wt ? wt * (z - mine) : wt);
+            lse[r] = z;
+            nll[r] = loss;
+            a += loss;
+            n += wt;
+        }
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) { a += __shfl_down(a, d); n += __shfl_down(n, d); }
+    if (lane == 0) { part[0][threadIdx.x >> 6] = a; part[1][threadIdx.x >> 6] = n; }
+    __syncthreads();
+    if (threadIdx.x < 2) sums[2 * blockIdx.x + threadIdx.x] = (part[threadIdx.x][0] + part[threadIdx.x][1]) + (part[threadIdx.x][2] + part[threadIdx.x][3]);
+}
+// shares (workgroup, class, k) of dw and behind them (workgroup, class) of db, both fp32; dx written whole
+template <class T, int V, int NC>
+__global__ __launch_bounds__(256) void k_ce_few_backward(const T *x, int64_t ldx, const T *w, int64_t ldw, const T *b, const int64_t *target,
+                                                         const float *cw, int64_t ignore, const float *lse, const float *dloss, int stride,
+                                                         const float *total, T *dx, float *dw, float *db, int rows, int classes, int k, int G)
+{
+    constexpr int P = FewRow<T, V, NC>::P;
+    extern __shared__ float few[];           // classes x kp weights, V biases; later 256 / G x kp shares of one class
+    const int kp = NC * G * P, lane = threadIdx.x & 63, g = lane & (G - 1), per = 256 / G;
+    float *lb = few + classes * kp;
+    few_weights(w, ldw, b, classes, k, kp, few, lb);
+    float aw[V][NC * P], ab[V];
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        ab[v] = 0.f;
+#pragma unroll
+        for (int e = 0; e < NC * P; e++) aw[v][e] = 0.f;
+    }
+    for (int r0 = blockIdx.x * per; r0 < rows; r0 += gridDim.x * per) {
+        const int r = r0 + threadIdx.x / G;
+        const float c = r < rows ? row_coefficient(dloss, stride, total, target, cw, ignore, classes, r) : 0.f;
+        FewRow<T, V, NC> q;
+        float l[V], out[NC * P];
+        q.load(x + (int64_t)r * ldx, k, g, G, r < rows && c != 0.f);          // (a row that does not count is zeros, whatever it holds)
+        q.scores(few, lb, kp, classes, g, G, l);
+        const float z = r < rows ? lse[r] : 0.f;
+        const int64_t t = r < rows ? target[r] : -1;
+#pragma unroll
+        for (int e = 0; e < NC * P; e++) out[e] = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; v++)
+            if (v < classes) {
+                const float p = __expf(l[v] - z) - (t == v ? 1.f : 0.f), gr = c == 0.f ? 0.f : p * c;
+                ab[v] += gr;
+#pragma unroll
+                for (int m = 0; m < NC; m++)
+#pragma unroll
+                    for (int e = 0; e < P; e++) {
+                        aw[v][m * P + e] = __builtin_fmaf(gr, q.x[m * P + e], aw[v][m * P + e]);
+                        out[m * P + e] = __builtin_fmaf(gr, few[v * kp + (m * G + g) * P + e], out[m * P + e]);
+                    }
+            }
+        if (dx && r < rows) {
+#pragma unroll
+            for (int m = 0; m < NC; m++) {
+                const int at = (m * G + g) * P;
+                T *o = dx + (int64_t)r * k + at;
+                Pack<T, P> v;
+#pragma unroll
+                for (int e = 0; e < P; e++) v.e[e] = (T)out[m * P + e];
+                store_some(o, v, k - at);
+            }
+        }
+    }
+    // the workgroup's rows meet class by class
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        if (v >= classes) break;
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < NC; m++)
+#pragma unroll
+            for (int e = 0; e < P; e++) few[(threadIdx.x / G) * kp + (m * G + g) * P + e] = aw[v][m * P + e];
+        __syncthreads();
+        for (int c = threadIdx.x; c < k; c += 256) {
+            float s = 0.f;
+            for (int q = 0; q < per; q++) s += few[q * kp + c];
+            dw[((int64_t)blockIdx.x * classes + v) * k + c] = s;
+        }
+        __syncthreads();
+        if (g == 0) few[threadIdx.x / G] = ab[v];
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            float s = 0.f;
+            for (int q = 0; q < per; q++) s += few[q];
+            db[(int64_t)blockIdx.x * classes + v] = s;
+        }
+    }
+}
+
 template <class T> __global__ __launch_bounds__(256) void k_cast(const float *in, const float *scale, float factor, T *out, int64_t n)
 {
     const float f = *scale * factor;
@@ -504,65 +1009,104 @@ template <class T> __global__ __launch_bounds__(256) void k_cast(const float *in
 }
 
 // ---- norm and clipping of many tensors -------------------------------------------------------------------------------------------------
-constexpr int TABLE = 128;                // tensors per launch: the table travels in the kernel's arguments (2.9 KB), no copy to wait for
+constexpr int TABLE = 160;                // tensors per launch: the table travels in the kernel's arguments (3.7 KB), no copy to wait for
 constexpr int BLOCK_ELEMS = 16384;        // elements per workgroup
 struct TensorTable {
     const void *in[TABLE];
     void *out[TABLE];
-    int64_t n[TABLE];
-    int first[TABLE];                     // first workgroup of the tensor
-    uint8_t dtype[TABLE], out_dtype[TABLE];
+    int first[TABLE + 1];                 // first workgroup of the tensor; the last one's end
+    uint16_t last[TABLE];                 // elements of the tensor's last workgroup - 1
+    uint8_t types[TABLE];                 // dtype | out_dtype << 4
     int count;
 };
-__device__ __forceinline__ int tensor_of(const TensorTable &t, int block)
+// the tensor of a workgroup, its element range in it
+__device__ __forceinline__ int tensor_of(const TensorTable &t, int block, int64_t &i0, int &n)
 {
     int lo = 0, hi = t.count - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (t.first[mid] <= block) lo = mid; else hi = mid - 1;
     }
+    i0 = (int64_t)(block - t.first[lo]) * BLOCK_ELEMS;
+    n = block + 1 == t.first[lo + 1] ? t.last[lo] + 1 : BLOCK_ELEMS;
     return lo;
 }
-__device__ __forceinline__ float elem(const void *p, int dtype, int64_t i)
+// f(eight elements as fp32, how many of them exist, index) over the range, packs of eight neighbouring elements per thread
+template <class T, class F> __device__ __forceinline__ void for_packs(const T *p, int n, F f)
 {
-    return dtype == NIRRT_NN_F32 ? ((const float *)p)[i] : dtype == NIRRT_NN_BF16 ? (float)((const bf16_t *)p)[i] : (float)((const f16_t *)p)[i];
+#pragma unroll 4
+    for (int i = threadIdx.x * 8; i < n; i += 256 * 8) {
+        float v[8];
+        const int cnt = n - i < 8 ? n - i : 8;
+        const Pack<T, 8> q = load_some<T, 8>(p + i, cnt);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = (float)q.e[e];
+        f(v, cnt, i);
+    }
 }
+template <class F> __device__ __forceinline__ void for_packs_of(const void *p, int dtype, int64_t i0, int n, F f)
+{
+    if (dtype == NIRRT_NN_F32) for_packs((const float *)p + i0, n, f);
+    else if (dtype == NIRRT_NN_BF16) for_packs((const bf16_t *)p + i0, n, f);
+    else for_packs((const f16_t *)p + i0, n, f);
+}
+// squares are summed in double: no overflow below the largest element squared, and the order does not matter to the last bits of the norm
 __global__ __launch_bounds__(256) void k_norm_parts(TensorTable t, double *parts)
 {
     __shared__ double part[4];
-    const int e = tensor_of(t, blockIdx.x);
-    const int64_t i0 = (int64_t)(blockIdx.x - t.first[e]) * BLOCK_ELEMS, i1 = t.n[e] - i0 < BLOCK_ELEMS ? t.n[e] : i0 + BLOCK_ELEMS;
+    int64_t i0;
+    int n;
+    const int e = tensor_of(t, blockIdx.x, i0, n);
     double s = 0.;
-    for (int64_t i = i0 + threadIdx.x; i < i1; i += 256) { const double v = elem(t.in[e], t.dtype[e], i); s += v * v; }
+    for_packs_of(t.in[e], t.types[e] & 15, i0, n, [&](const float *v, int, int) {
+        double a = 0.;
+#pragma unroll
+        for (int q = 0; q < 8; q++) a = __builtin_fma((double)v[q], (double)v[q], a);
+        s += a;
+    });
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) s += __shfl_down(s, d);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0) parts[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
-__global__ __launch_bounds__(256) void k_norm_total(const double *parts, int64_t n, float *norm)
+__global__ __launch_bounds__(1024) void k_norm_total(const double *parts, int64_t n, float *norm)
 {
-    __shared__ double part[4];
+    __shared__ double part[16];
     double s = 0.;
-    for (int64_t i = threadIdx.x; i < n; i += 256) s += parts[i];
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < n; i += 1024) s += parts[i];
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) s += __shfl_down(s, d);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) *norm = (float)sqrt((part[0] + part[1]) + (part[2] + part[3]));
+    if (threadIdx.x == 0) {
+        s = 0.;
+#pragma unroll
+        for (int q = 0; q < 16; q++) s += part[q];
+        *norm = (float)sqrt(s);
+    }
+}
+template <class T> __device__ __forceinline__ void put_pack(T *o, const float *v, float f, int cnt)
+{
+    Pack<T, 8> q;
+#pragma unroll
+    for (int e = 0; e < 8; e++) q.e[e] = (T)(v[e] * f);
+    store_some(o, q, cnt);
 }
 __global__ __launch_bounds__(256) void k_scale(TensorTable t, const float *norm, float max_norm)
 {
-    const int e = tensor_of(t, blockIdx.x);
+    int64_t i0;
+    int n;
+    const int e = tensor_of(t, blockIdx.x, i0, n), to = t.types[e] >> 4;
     const float q = max_norm / (*norm + 1e-6f), f = q < 1.f ? q : (q == q ? 1.f : q);
     if (f == 1.f && t.in[e] == t.out[e]) return;
-    const int64_t i0 = (int64_t)(blockIdx.x - t.first[e]) * BLOCK_ELEMS, i1 = t.n[e] - i0 < BLOCK_ELEMS ? t.n[e] : i0 + BLOCK_ELEMS;
-    for (int64_t i = i0 + threadIdx.x; i < i1; i += 256) {
-        const float v = elem(t.in[e], t.dtype[e], i) * f;
-        if (t.out_dtype[e] == NIRRT_NN_F32) ((float *)t.out[e])[i] = v;
-        else if (t.out_dtype[e] == NIRRT_NN_BF16) ((bf16_t *)t.out[e])[i] = (bf16_t)v;
-        else ((f16_t *)t.out[e])[i] = (f16_t)v;
-    }
+    void *out = t.out[e];
+    for_packs_of(t.in[e], t.types[e] & 15, i0, n, [&](const float *v, int cnt, int i) {
+        if (to == NIRRT_NN_F32) put_pack((float *)out + i0 + i, v, f, cnt);
+        else if (to == NIRRT_NN_BF16) put_pack((bf16_t *)out + i0 + i, v, f, cnt);
+        else put_pack((f16_t *)out + i0 + i, v, f, cnt);
+    });
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------------------
@@ -573,25 +1117,19 @@ int status() { return hipGetLastError() == hipSuccess ? 0 : -2; }
 int elem_size(int dtype) { return dtype == NIRRT_NN_F32 ? 4 : 2; }
 bool good_type(int dtype) { return dtype == NIRRT_NN_F32 || dtype == NIRRT_NN_BF16 || dtype == NIRRT_NN_F16; }
 
-template <class T> Operand<T> kc(const T *p, int64_t ld, int64_t rows)
-{
-    return {p, ld, (int)rows, ((uintptr_t)p % 16 == 0 && ld * (int64_t)sizeof(T) % 16 == 0) ? 1 : 0, nullptr};
-}
-template <class T> Operand<T> rc(const T *p, int64_t ld, int64_t rows, const float *skip = nullptr)
-{
-    return {p, ld, (int)rows, ((uintptr_t)p % (4 * sizeof(T)) == 0 && ld % 4 == 0) ? 1 : 0, skip};
-}
+template <class T> Operand<T> op(const T *p, int64_t ld, int64_t rows) { return {p, ld, (int)rows}; }
 
-// tile edge and parts of the reduction.  A GPU of 256 CUs wants some 500 workgroups of four waves: 128 x 128 tiles where that many exist,
-// else 64 x 64; where even these are fewer and the reduction is long, it is cut (at least four steps per part, at most 32 parts).
+// Tile edge and parts of the reduction.  A GPU of 256 CUs wants a workgroup of eight waves per CU (256 x 256 tiles) or two of four waves
+// (128 x 128): the largest tile that still gives every CU one; 64 x 64 where there are fewer, and where even these are few and the
+// reduction is long, it is cut (at least four steps per part, at most 32 parts).  256 x 256 needs operands of whole aligned chunks.
 struct Plan { int edge, parts, part; };
 Plan plan(int dtype, int64_t m, int64_t n, int64_t k)
 {
     Plan p;
-    const int64_t big = ceil_div(m, 128) * ceil_div(n, 128), step = ROW_BYTES / elem_size(dtype), steps = ceil_div(k, step);
-    p.edge = big >= 256 ? 128 : 64;
+    const int64_t step = ROW_BYTES / elem_size(dtype), steps = ceil_div(k, step);
+    p.edge = ceil_div(m, 256) * ceil_div(n, 256) >= 224 ? 256 : ceil_div(m, 128) * ceil_div(n, 128) >= 256 ? 128 : 64;
     const int64_t tiles = ceil_div(m, p.edge) * ceil_div(n, p.edge);      // (0 for an empty result)
-    int64_t parts = tiles >= 256 || tiles == 0 ? 1 : 512 / tiles;
+    int64_t parts = p.edge == 256 || tiles >= 256 || tiles == 0 ? 1 : 512 / tiles;
     if (parts > steps / 4) parts = steps / 4;
     if (parts > 32) parts = 32;
     if (parts < 1) parts = 1;
@@ -602,18 +1140,31 @@ Plan plan(int dtype, int64_t m, int64_t n, int64_t k)
 }
 int64_t plan_bytes(const Plan &p, int64_t m, int64_t n) { return p.parts > 1 ? round256(4 * m * n * p.parts) : 0; }
 
+// whole aligned chunks (see DirectOperand): rows and base on 16 bytes, for KC a reduction of whole chunks, offsets inside a step below 2^31
+template <class T, bool RC> bool direct(const Operand<T> &o, int64_t k)
+{
+    const int64_t row_bytes = o.ld * (int64_t)sizeof(T);
+    if ((uintptr_t)o.p % 16 || row_bytes % 16) return false;
+    return RC ? row_bytes <= (1 << 24) : k % Elem<T>::PER_CHUNK == 0 && row_bytes <= (1 << 22);
+}
+
 template <class T, bool RCA, bool RCB, class Epi>
 int gemm(const Operand<T> &a, const Operand<T> &b, int64_t m, int64_t n, int64_t k, const Plan &p, float *partial, const Epi &epi, hipStream_t st)
 {
-    const int64_t tiles = ceil_div(m, p.edge) * ceil_div(n, p.edge);
+    const bool fast = direct<T, RCA>(a, k) && direct<T, RCB>(b, k);
+    const int edge = fast || p.edge < 256 ? p.edge : 128;
+    const int64_t tiles = ceil_div(m, edge) * ceil_div(n, edge);
     if (tiles > DIM_MAX) return -1;
     const dim3 grid((unsigned)tiles, (unsigned)p.parts);
-    if (p.edge == 128)
-        hipLaunchKernelGGL((k_gemm<T, 128, 128, 2, 2, RCA, RCB, Epi>), grid, dim3(256), 0, st, a, b, (int)m, (int)n, (int)k, p.part, partial, epi);
-    else
-        hipLaunchKernelGGL((k_gemm<T, 64, 64, 2, 2, RCA, RCB, Epi>), grid, dim3(256), 0, st, a, b, (int)m, (int)n, (int)k, p.part, partial, epi);
+#define LAUNCH(TILE, EDGE, WM, WN)                                                                                                               \
+    hipLaunchKernelGGL((k_gemm<T, EDGE, EDGE, TILE<T, EDGE, EDGE, WM, WN, RCA, RCB>, Epi>), grid, dim3(64 * WM * WN), 0, st, a, b, (int)m, (int)n, \
+                       (int)k, p.part, partial, epi)
+    if (edge == 256) LAUNCH(DirectTile, 256, 2, 4);
+    else if (edge == 128) { if (fast) LAUNCH(DirectTile, 128, 2, 2); else LAUNCH(Tile, 128, 2, 2); }
+    else { if (fast) LAUNCH(DirectTile, 64, 2, 2); else LAUNCH(Tile, 64, 2, 2); }
+#undef LAUNCH
     if (p.parts > 1) {
-        const int64_t blocks = ceil_div(m * n, 256);
+        const int64_t blocks = ceil_div(m * ceil_div(n, 4), 256);
         hipLaunchKernelGGL((k_join<Epi>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, partial, p.parts, (int)m, (int)n, epi);
     }
     return status();
@@ -621,8 +1172,24 @@ int gemm(const Operand<T> &a, const Operand<T> &b, int64_t m, int64_t n, int64_t
 
 bool good_dims(int64_t a, int64_t b, int64_t c) { return a >= 0 && b >= 0 && c >= 0 && a <= DIM_MAX - 256 && b <= DIM_MAX - 256 && c <= DIM_MAX - 256; }
 
-constexpr int COLUMN_PARTS = 256;
-int column_chunk(int64_t m) { const int64_t c = ceil_div(m, COLUMN_PARTS); return (int)(c > 32 ? c : 32); }
+// k_dz: lanes per row, rows per workgroup and chunks so that some 2000 workgroups share a large matrix and a chunk is no shorter than 4 passes
+struct Columns { int lanes, blocks, chunk, parts; };
+Columns columns(int dtype, int64_t m, int64_t n)
+{
+    Columns c;
+    const int64_t packs = ceil_div(n, 16 / elem_size(dtype));
+    c.lanes = 1;
+    while (c.lanes < 64 && c.lanes < packs) c.lanes *= 2;
+    c.blocks = (int)ceil_div(packs, c.lanes);
+    const int64_t step = 256 / c.lanes;
+    int64_t parts = ceil_div(2048, c.blocks > 0 ? c.blocks : 1), most = ceil_div(m, 4 * step);
+    if (parts > most) parts = most;
+    if (parts > 512) parts = 512;
+    if (parts < 1) parts = 1;
+    c.chunk = (int)(m > 0 ? ceil_div(m, parts) : 1);
+    c.parts = (int)ceil_div(m, c.chunk);
+    return c;
+}
 
 struct LinearBackward { Plan px, pw; int64_t dz, sums, part, total; };
 LinearBackward linear_backward_layout(int dtype, int act, int64_t m, int64_t n, int64_t k)
@@ -631,7 +1198,7 @@ LinearBackward linear_backward_layout(int dtype, int act, int64_t m, int64_t n, 
     l.px = plan(dtype, m, k, n);
     l.pw = plan(dtype, n, k, m);
     l.dz = act == NIRRT_NN_ACT_NONE ? 0 : round256(m * n * elem_size(dtype));
-    l.sums = round256(4 * n * ceil_div(m, column_chunk(m)));
+    l.sums = round256(4 * n * columns(dtype, m, n).parts);
     const int64_t bx = plan_bytes(l.px, m, k), bw = plan_bytes(l.pw, n, k);
     l.part = bx > bw ? bx : bw;
     l.total = l.dz + l.sums + l.part;
@@ -643,7 +1210,7 @@ int linear_t(int dtype, int act, const void *x, int64_t ldx, const void *w, int6
              int64_t ldy, void *z, int64_t m, int64_t n, int64_t k, void *ws, hipStream_t st)
 {
     const EpiLinear<T> epi = {(const T *)b, (const T *)r, (T *)y, (T *)z, ldr, ldy, act, (int)n};
-    return gemm<T, false, false>(kc((const T *)x, ldx, m), kc((const T *)w, ldw, n), m, n, k, plan(dtype, m, n, k), (float *)ws, epi, st);
+    return gemm<T, false, false>(op((const T *)x, ldx, m), op((const T *)w, ldw, n), m, n, k, plan(dtype, m, n, k), (float *)ws, epi, st);
 }
 
 template <class T>
@@ -655,35 +1222,73 @@ int linear_backward_t(int dtype, int act, const void *x, int64_t ldx, const void
     float *sums = (float *)(ws + l.dz), *part = (float *)(ws + l.dz + l.sums);
     const bool own_dz = act != NIRRT_NN_ACT_NONE;
     if (own_dz || db) {
-        const int chunk = column_chunk(m), parts = (int)ceil_div(m, chunk);
-        if (m > 0) {
-            hipLaunchKernelGGL((k_dz<T>), dim3((unsigned)ceil_div(n, 256), (unsigned)parts), dim3(256), 0, st, (const T *)z, (const T *)dy, lddy,
-                               own_dz && (dx || dw) ? dz : (T *)nullptr, db ? sums : nullptr, (int)m, (int)n, chunk, act);
-        }
-        if (db) hipLaunchKernelGGL((k_column_join<T>), dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, st, sums, m > 0 ? parts : 0, (T *)db, (int)n);
+        const Columns c = columns(dtype, m, n);
+        if (m > 0)
+            hipLaunchKernelGGL((k_dz<T>), dim3((unsigned)c.blocks, (unsigned)c.parts), dim3(256), 0, st, (const T *)z, (const T *)dy, lddy,
+                               own_dz && (dx || dw) ? dz : (T *)nullptr, db ? sums : nullptr, (int)m, (int)n, c.chunk, c.lanes, act);
+        if (db)
+            hipLaunchKernelGGL((k_column_join<T>), dim3((unsigned)ceil_div(n, 64)), dim3(256), 0, st, sums, c.parts, (const float *)nullptr, 1.f, (T *)db, n);
         if (int rc_ = status()) return rc_;
     }
     const T *d = own_dz ? dz : (const T *)dy;
     const int64_t ldd = own_dz ? n : lddy;
     if (dx && m > 0 && k > 0) {
         const EpiPlain<T> epi = {(T *)dx, nullptr, 1.f, (int)k};
-        if (int rc_ = gemm<T, false, true>(kc(d, ldd, m), rc((const T *)w, ldw, k), m, k, n, l.px, part, epi, st)) return rc_;
+        if (int rc_ = gemm<T, false, true>(op(d, ldd, m), op((const T *)w, ldw, k), m, k, n, l.px, part, epi, st)) return rc_;
     }
     if (dw && n > 0 && k > 0) {
         const EpiPlain<T> epi = {(T *)dw, nullptr, 1.f, (int)k};
-        if (int rc_ = gemm<T, true, true>(rc(d, ldd, n), rc((const T *)x, ldx, k), n, k, m, l.pw, part, epi, st)) return rc_;
+        if (int rc_ = gemm<T, true, true>(op(d, ldd, n), op((const T *)x, ldx, k), n, k, m, l.pw, part, epi, st)) return rc_;
     }
     return 0;
 }
 
-// cross entropy: parts of the classes, so that row tiles x parts fill the GPU
-struct CeForward { int edge, parts, part; int64_t stats, score, sums, total; };
-CeForward ce_layout(int64_t rows, int64_t classes)
+// few classes (k_ce_few): up to 8, and a row on at most 64 lanes x 4 packs
+struct Few { int lanes, packs, classes, blocks, lds, lds_backward; };
+bool few_layout(int dtype, int64_t rows, int64_t classes, int64_t k, Few &f)
+{
+    const int p = 16 / elem_size(dtype);
+    const int64_t packs = ceil_div(k > 0 ? k : 1, p);
+    if (classes > 8 || packs > 256) return false;
+    f.lanes = 1;
+    while (f.lanes < 64 && f.lanes < packs) f.lanes *= 2;
+    const int64_t per_lane = ceil_div(packs, f.lanes);
+    f.packs = per_lane <= 1 ? 1 : per_lane <= 2 ? 2 : 4;
+    f.classes = classes <= 2 ? 2 : classes <= 4 ? 4 : 8;
+    if (f.classes * f.packs * p > 128) return false;      // registers of dw
+    const int kp = f.packs * f.lanes * p, per = 256 / f.lanes;
+    const int64_t blocks = ceil_div(rows, 4 * per);       // (at least four rows per lane group, at most two workgroups per CU)
+    f.blocks = (int)(blocks < 512 ? (blocks > 0 ? blocks : 1) : 512);
+    f.lds = (int)(4 * (classes * kp + 8));
+    f.lds_backward = f.lds > 4 * per * kp ? f.lds : 4 * per * kp;
+    return true;
+}
+#define FEW_LAUNCH(KERNEL, LDS, ...)                                                                                     \
+    do {                                                                                                                 \
+        if (f.classes == 2) { if (f.packs == 1) FEW_ONE(KERNEL, 2, 1, LDS, __VA_ARGS__); else if (f.packs == 2) FEW_ONE(KERNEL, 2, 2, LDS, __VA_ARGS__); else FEW_ONE(KERNEL, 2, 4, LDS, __VA_ARGS__); } \
+        else if (f.classes == 4) { if (f.packs == 1) FEW_ONE(KERNEL, 4, 1, LDS, __VA_ARGS__); else if (f.packs == 2) FEW_ONE(KERNEL, 4, 2, LDS, __VA_ARGS__); else FEW_ONE(KERNEL, 4, 4, LDS, __VA_ARGS__); } \
+        else { if (f.packs == 1) FEW_ONE(KERNEL, 8, 1, LDS, __VA_ARGS__); else if (f.packs == 2) FEW_ONE(KERNEL, 8, 2, LDS, __VA_ARGS__); else FEW_ONE(KERNEL, 8, 4, LDS, __VA_ARGS__); } \
+    } while (0)
+#define FEW_ONE(KERNEL, V, NC, LDS, ...) hipLaunchKernelGGL((KERNEL<T, V, NC>), dim3((unsigned)f.blocks), dim3(256), LDS, st, __VA_ARGS__)
+
+// cross entropy: tile edge, and parts of the classes so that row tiles x parts fill the GPU; x and w whose rows are no whole aligned chunks
+// are copied into such (k_ce_rows_copy): the products read them many times
+int64_t padded(int dtype, int64_t k) { const int64_t c = 16 / elem_size(dtype); return (k + c - 1) / c * c; }
+bool whole_rows(int dtype, const void *p, int64_t ld, int64_t k) { return (uintptr_t)p % 16 == 0 && ld * elem_size(dtype) % 16 == 0 && k == padded(dtype, k); }
+template <class T> void copy_rows(const void *x, int64_t ldx, const float *coef, T *out, int64_t ld, int64_t rows, int64_t k, hipStream_t st)
+{
+    const int64_t blocks = ceil_div(rows * (ld * (int64_t)sizeof(T) / 16), 256);
+    if (blocks > 0)
+        hipLaunchKernelGGL((k_ce_rows_copy<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, (const T *)x, ldx, coef, out, ld, (int)rows, (int)k);
+}
+struct CeForward { int edge, parts, part; int64_t stats, score, sums, xs, ws, total; };
+CeForward ce_layout(int dtype, int64_t rows, int64_t classes, int64_t k)
 {
     CeForward f;
-    f.edge = ceil_div(rows, 128) * ceil_div(classes, 128) >= 256 ? 128 : 64;
+    const int64_t big = ceil_div(rows, 128) * ceil_div(classes, 128);
+    f.edge = big >= 1024 ? 256 : big >= 256 ? 128 : 64;
     const int64_t row_tiles = ceil_div(rows, f.edge), class_tiles = ceil_div(classes, f.edge);
-    int64_t parts = ceil_div(512, row_tiles > 0 ? row_tiles : 1);
+    int64_t parts = ceil_div(f.edge == 256 ? 256 : 512, row_tiles > 0 ? row_tiles : 1);
     if (parts > class_tiles) parts = class_tiles;
     if (parts < 1) parts = 1;
     const int64_t per = ceil_div(class_tiles, parts);
@@ -691,29 +1296,41 @@ CeForward ce_layout(int64_t rows, int64_t classes)
     f.parts = (int)(class_tiles > 0 ? ceil_div(class_tiles, per) : 1);
     f.stats = round256(8 * rows * f.parts);
     f.score = round256(4 * rows);
-    f.sums = round256(16 * ceil_div(rows, 256));
-    f.total = f.stats + f.score + f.sums;
+    f.sums = round256(16 * (ceil_div(rows, 256) + 512));
+    f.xs = round256(rows * padded(dtype, k) * elem_size(dtype));
+    f.ws = round256(classes * padded(dtype, k) * elem_size(dtype));
+    f.total = f.stats + f.score + f.sums + f.xs + f.ws;
     return f;
 }
 template <class T>
-int ce_forward_t(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *b, const int64_t *target, const float *cw, int64_t ignore,
+int ce_forward_t(int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw, const void *b, const int64_t *target, const float *cw, int64_t ignore,
                  float *lse, float *nll, float *total, int64_t rows, int64_t classes, int64_t k, char *ws, hipStream_t st)
 {
-    const CeForward f = ce_layout(rows, classes);
-    float2 *stats = (float2 *)ws;
-    float *score = (float *)(ws + f.stats);
-    double *sums = (double *)(ws + f.stats + f.score);
-    const int64_t row_tiles = ceil_div(rows, f.edge), blocks = ceil_div(rows, 256);
-    if (rows > 0) {
-        const dim3 grid((unsigned)row_tiles, (unsigned)f.parts);
-        const Operand<T> ow = kc((const T *)w, ldw, classes), ox = kc((const T *)x, ldx, rows);
-        if (f.edge == 128)
-            hipLaunchKernelGGL((k_ce_stats<T, 128, 128, 2, 2>), grid, dim3(256), 0, st, ow, ox, (const T *)b, target, (int)rows, (int)classes, (int)k,
-                               f.part, stats, score);
-        else
-            hipLaunchKernelGGL((k_ce_stats<T, 64, 64, 2, 2>), grid, dim3(256), 0, st, ow, ox, (const T *)b, target, (int)rows, (int)classes, (int)k,
-                               f.part, stats, score);
-        hipLaunchKernelGGL(k_ce_rows, dim3((unsigned)blocks), dim3(256), 0, st, stats, f.parts, score, target, cw, ignore, (int)rows, (int)classes,
+    const CeForward l = ce_layout(dtype, rows, classes, k);
+    double *sums = (double *)ws;
+    float *score = (float *)(ws + l.sums);
+    float2 *stats = (float2 *)(ws + l.sums + l.score);
+    T *xs = (T *)(ws + l.sums + l.score + l.stats), *wsp = (T *)((char *)xs + l.xs);
+    int64_t blocks = 0;
+    Few f;
+    if (rows > 0 && few_layout(dtype, rows, classes, k, f)) {
+        blocks = f.blocks;
+        FEW_LAUNCH(k_ce_few, f.lds, (const T *)x, ldx, (const T *)w, ldw, (const T *)b, target, cw, ignore, (int)rows, (int)classes, (int)k, f.lanes, lse,
+                   nll, sums);
+    } else if (rows > 0) {
+        blocks = ceil_div(rows, 256);
+        const int64_t kp = padded(dtype, k), row_tiles = ceil_div(rows, l.edge);
+        if (!whole_rows(dtype, x, ldx, k)) { copy_rows(x, ldx, nullptr, xs, kp, rows, k, st); x = xs; ldx = kp; }
+        if (!whole_rows(dtype, w, ldw, k)) { copy_rows(w, ldw, nullptr, wsp, kp, classes, k, st); w = wsp; ldw = kp; }
+        const dim3 grid((unsigned)row_tiles, (unsigned)l.parts);
+        const Operand<T> ow = op((const T *)w, ldw, classes), ox = op((const T *)x, ldx, rows);
+        if (!direct<T, false>(ow, kp) || !direct<T, false>(ox, kp)) return -1;   // (rows of more than 4 MB)
+#define LAUNCH(EDGE, WM, WN)                                                                                                                \
+    hipLaunchKernelGGL((k_ce_stats<T, EDGE, EDGE, DirectTile<T, EDGE, EDGE, WM, WN, false, false>>), grid, dim3(64 * WM * WN), 0, st, ow, ox, \
+                       (const T *)b, target, (int)rows, (int)classes, (int)kp, l.part, stats, score)
+        if (l.edge == 256) LAUNCH(256, 2, 4); else if (l.edge == 128) LAUNCH(128, 2, 2); else LAUNCH(64, 2, 2);
+#undef LAUNCH
+        hipLaunchKernelGGL(k_ce_rows, dim3((unsigned)blocks), dim3(256), 0, st, stats, l.parts, score, target, cw, ignore, (int)rows, (int)classes,
                            lse, nll, sums);
     }
     hipLaunchKernelGGL(k_ce_total, dim3(1), dim3(256), 0, st, sums, (int)blocks, total);
@@ -721,22 +1338,36 @@ int ce_forward_t(const void *x, int64_t ldx, const void *w, int64_t ldw, const v
 }
 
 constexpr int64_t G_ELEMS = 1ll << 27;    // of g' at a time: pieces of the classes
-struct CeBackward { int64_t piece, ldg; Plan px, pw; int64_t g, rel, acc, part, total; };
+struct CeBackward { int64_t piece, ldg; Plan pg, px, pw; int64_t coef, tops, xs, ws, g, acc, part, total; };
 CeBackward ce_backward_layout(int dtype, int64_t rows, int64_t classes, int64_t k)
 {
     CeBackward l;
-    l.ldg = (rows + 7) / 8 * 8;
-    l.piece = l.ldg > 0 ? G_ELEMS / l.ldg / 128 * 128 : classes;
-    if (l.piece < 128) l.piece = 128;
+    Few f;
+    if (few_layout(dtype, rows, classes, k, f)) {
+        l = CeBackward{};
+        l.part = round256(4 * (k + 1) * classes * f.blocks);
+        l.total = l.part;
+        return l;
+    }
+    const int64_t e = elem_size(dtype);
+    l.ldg = padded(dtype, rows);
+    l.piece = l.ldg > 0 ? G_ELEMS / l.ldg / 256 * 256 : classes;
+    if (l.piece < 256) l.piece = 256;
     if (l.piece > classes) l.piece = classes;
+    l.pg = plan(dtype, l.piece, rows, k);
+    l.pg.parts = 1;                    // (the scores are not cut: the softmax needs whole ones)
+    l.pg.part = (int)(padded(dtype, k) > 0 ? padded(dtype, k) : 1);
     l.px = plan(dtype, rows, k, l.piece);
     l.pw = plan(dtype, l.piece, k, rows);
-    l.g = round256(l.ldg * l.piece * elem_size(dtype));
-    l.rel = round256(4 * rows) + 256;
+    l.coef = round256(4 * rows) + 256;
+    l.tops = round256(4 * ceil_div(rows, 256));
+    l.xs = round256(rows * padded(dtype, k) * e);
+    l.ws = round256(classes * padded(dtype, k) * e);
+    l.g = round256(l.ldg * l.piece * e);
     l.acc = l.piece < classes ? round256(4 * rows * k) : 0;
     const int64_t bx = plan_bytes(l.px, rows, k), bw = plan_bytes(l.pw, l.piece, k);
     l.part = bx > bw ? bx : bw;
-    l.total = l.g + l.rel + l.acc + l.part;
+    l.total = l.coef + l.tops + l.xs + l.ws + l.g + l.acc + l.part;
     return l;
 }
 template <class T>
@@ -745,36 +1376,52 @@ int ce_backward_t(int dtype, const void *x, int64_t ldx, const void *w, int64_t 
                   int64_t classes, int64_t k, char *ws, hipStream_t st)
 {
     const CeBackward l = ce_backward_layout(dtype, rows, classes, k);
-    T *g = (T *)ws;
-    float *scale = (float *)(ws + l.g), *rel = scale + 64, *acc = (float *)(ws + l.g + l.rel), *part = (float *)(ws + l.g + l.rel + l.acc);
-    hipLaunchKernelGGL(k_ce_coefficients, dim3(1), dim3(1024), 0, st, dloss, stride, total, target, cw, ignore, (int)rows, (int)classes, rel, scale);
+    Few f;
+    if (few_layout(dtype, rows, classes, k, f)) {
+        float *sw = (float *)ws, *sb = sw + k * classes * f.blocks;
+        FEW_LAUNCH(k_ce_few_backward, f.lds_backward, (const T *)x, ldx, (const T *)w, ldw, (const T *)b, target, cw, ignore, lse, dloss, stride, total, (T *)dx,
+                   sw, sb, (int)rows, (int)classes, (int)k, f.lanes);
+        if (dw && k > 0)
+            hipLaunchKernelGGL((k_column_join<T>), dim3((unsigned)ceil_div(classes * k, 64)), dim3(256), 0, st, sw, f.blocks, (const float *)nullptr, 1.f,
+                               (T *)dw, classes * k);
+        if (db)
+            hipLaunchKernelGGL((k_column_join<T>), dim3((unsigned)ceil_div(classes, 64)), dim3(256), 0, st, sb, f.blocks, (const float *)nullptr, 1.f, (T *)db,
+                               classes);
+        return status();
+    }
+    float *scale = (float *)ws, *coef = scale + 64, *tops = (float *)(ws + l.coef);
+    T *xs = (T *)(ws + l.coef + l.tops), *wsp = (T *)((char *)xs + l.xs), *g = (T *)((char *)wsp + l.ws);
+    float *acc = (float *)((char *)g + l.g), *part = (float *)((char *)acc + l.acc);
+    const int64_t kp = padded(dtype, k), blocks = ceil_div(rows, 256);
+    if (blocks > 0)
+        hipLaunchKernelGGL(k_ce_coefficients, dim3((unsigned)blocks), dim3(256), 0, st, dloss, stride, total, target, cw, ignore, (int)rows, (int)classes, coef, tops);
+    hipLaunchKernelGGL(k_ce_scale, dim3(1), dim3(256), 0, st, tops, (int)blocks, scale);
+    copy_rows(x, ldx, coef, xs, kp, rows, k, st);
+    if (!whole_rows(dtype, w, ldw, k)) { copy_rows(w, ldw, nullptr, wsp, kp, classes, k, st); w = wsp; ldw = kp; }
     const float unlift = 1.f / Factor<T>::VALUE;
     for (int64_t v0 = 0; v0 < classes; v0 += l.piece) {
         const int64_t nv = classes - v0 < l.piece ? classes - v0 : l.piece;
         const T *wp = (const T *)w + v0 * ldw;
         if (rows > 0) {
-            const EpiSoftmaxGrad<T> eg = {g, l.ldg, (const T *)b, lse, rel, target, v0};
-            Plan pg = plan(dtype, nv, rows, k);
-            pg.parts = 1;                    // (the scores are not cut: the softmax needs whole ones)
-            pg.part = (int)(k > 0 ? k : 1);
-            if (int rc_ = gemm<T, false, false>(kc(wp, ldw, nv), kc((const T *)x, ldx, rows), nv, rows, k, pg, nullptr, eg, st)) return rc_;
+            const EpiSoftmaxGrad<T> eg = {g, l.ldg, (const T *)b, lse, coef, scale, target, v0};
+            if (int rc = gemm<T, false, false>(op(wp, ldw, nv), op((const T *)xs, kp, rows), nv, rows, kp, l.pg, nullptr, eg, st)) return rc;
         }
         if (db) hipLaunchKernelGGL((k_ce_bias<T>), dim3((unsigned)ceil_div(nv, 4)), dim3(256), 0, st, (const T *)g, l.ldg, (int)rows, (int)nv, scale, (T *)db + v0);
         if (dx && rows > 0 && k > 0) {
-            const Operand<T> og = rc((const T *)g, l.ldg, rows), ow = rc(wp, ldw, k);
-            int rc_;
-            if (l.acc) rc_ = gemm<T, true, true>(og, ow, rows, k, nv, l.px, part, EpiAccumulate{acc, (int)k, v0 == 0}, st);
-            else rc_ = gemm<T, true, true>(og, ow, rows, k, nv, l.px, part, EpiPlain<T>{(T *)dx, scale, unlift, (int)k}, st);
-            if (rc_) return rc_;
+            const Operand<T> og = op((const T *)g, l.ldg, rows), ow = op(wp, ldw, k);
+            int rc;
+            if (l.acc) rc = gemm<T, true, true>(og, ow, rows, k, nv, l.px, part, EpiAccumulate<T>{acc, (int)k, v0 == 0}, st);
+            else rc = gemm<T, true, true>(og, ow, rows, k, nv, l.px, part, EpiPlain<T>{(T *)dx, scale, unlift, (int)k}, st);
+            if (rc) return rc;
         }
         if (dw && k > 0) {
             const EpiPlain<T> ep = {(T *)dw + v0 * k, scale, unlift, (int)k};
-            if (int rc_ = gemm<T, false, true>(kc((const T *)g, l.ldg, nv), rc((const T *)x, ldx, k, rel), nv, k, rows, l.pw, part, ep, st)) return rc_;
+            if (int rc = gemm<T, false, true>(op((const T *)g, l.ldg, nv), op((const T *)xs, kp, k), nv, k, rows, l.pw, part, ep, st)) return rc;
         }
     }
     if (dx && l.acc && rows > 0 && k > 0) {
-        const int64_t blocks = ceil_div(rows * k, 256);
-        hipLaunchKernelGGL((k_cast<T>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st, acc, scale, unlift, (T *)dx, rows * k);
+        const int64_t cast = ceil_div(rows * k, 256);
+        hipLaunchKernelGGL((k_cast<T>), dim3((unsigned)(cast < 8192 ? cast : 8192)), dim3(256), 0, st, acc, scale, unlift, (T *)dx, rows * k);
     }
     return status();
 }
@@ -802,6 +1449,7 @@ template <class F> int64_t for_tables(const nirrt_nn_tensor *t, int32_t count, F
         const int64_t b = i < count ? ceil_div(t[i].n, BLOCK_ELEMS) : 0;
         if (b > DIM_MAX / 2) return -1;
         if (tab.count == TABLE || (i == count && tab.count > 0) || (tab.count > 0 && blocks + b > DIM_MAX / 2)) {
+            tab.first[tab.count] = (int)blocks;
             if (launch(tab, done, blocks)) return -2;
             done += blocks;
             blocks = 0;
@@ -811,10 +1459,9 @@ template <class F> int64_t for_tables(const nirrt_nn_tensor *t, int32_t count, F
         const int c = tab.count++;
         tab.in[c] = t[i].data;
         tab.out[c] = t[i].out;
-        tab.n[c] = t[i].n;
         tab.first[c] = (int)blocks;
-        tab.dtype[c] = (uint8_t)t[i].dtype;
-        tab.out_dtype[c] = (uint8_t)t[i].out_dtype;
+        tab.last[c] = (uint16_t)((t[i].n - 1) % BLOCK_ELEMS);
+        tab.types[c] = (uint8_t)(t[i].dtype | t[i].out_dtype << 4);
         blocks += b;
     }
     return done;
@@ -861,7 +1508,7 @@ extern "C" int nirrt_nn_linear_backward(int dtype, int act, const void *x, int64
 extern "C" int64_t nirrt_nn_cross_entropy_workspace(int dtype, int64_t rows, int64_t classes, int64_t k)
 {
     if (!good_type(dtype) || !good_dims(rows, classes, k) || classes < 1) return -1;
-    return ce_layout(rows, classes).total;
+    return ce_layout(dtype, rows, classes, k).total;
 }
 
 extern "C" int nirrt_nn_cross_entropy(int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw, const void *b, const int64_t *target,
@@ -870,7 +1517,7 @@ extern "C" int nirrt_nn_cross_entropy(int dtype, const void *x, int64_t ldx, con
 {
     if (!good_type(dtype) || !good_dims(rows, classes, k) || classes < 1 || !total || ldx < k || ldw < k) return -1;
     if (rows > 0 && (!target || !lse || !nll || !workspace || (k > 0 && (!x || !w)))) return -1;
-#define CALL(T) ce_forward_t<T>(x, ldx, w, ldw, b, target, class_weight, ignore_index, lse, nll, total, rows, classes, k, (char *)workspace, (hipStream_t)stream)
+#define CALL(T) ce_forward_t<T>(dtype, x, ldx, w, ldw, b, target, class_weight, ignore_index, lse, nll, total, rows, classes, k, (char *)workspace, (hipStream_t)stream)
     return BY_TYPE(dtype, CALL);
 #undef CALL
 }
@@ -915,7 +1562,7 @@ extern "C" int nirrt_nn_norm(const nirrt_nn_tensor *tensors, int32_t count, floa
         return status();
     });
     if (blocks < 0) return (int)blocks;
-    hipLaunchKernelGGL(k_norm_total, dim3(1), dim3(256), 0, st, parts, blocks, norm);
+    hipLaunchKernelGGL(k_norm_total, dim3(1), dim3(1024), 0, st, parts, blocks, norm);
     return status();
 }
 

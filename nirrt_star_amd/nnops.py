@@ -10,6 +10,7 @@ float32, bfloat16 and float16; sums are held in 32 bits and rounded once.  Tenso
 there is no other implementation); rows may have any stride, other layouts are copied.  Results are the same bits for the same input
 (no atomics).  Backward passes are differentiable once.
 """
+import contextlib
 import ctypes as C
 
 import numpy as np
@@ -44,8 +45,11 @@ def _lib():
     return L
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # (the stream object costs 2 us per call)
+
+
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(device.index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 def _check(rc, what):
@@ -53,9 +57,12 @@ def _check(rc, what):
         raise RuntimeError("libnirrt_hip %s failed (%d)" % (what, rc))
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(device):
     """the C functions launch on the calling thread's current device"""
-    return torch.cuda.device(device)
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def _need(name, first, **others):
@@ -261,13 +268,13 @@ def _tensor_list(name, tensors):
     ts = [t for t in tensors if t is not None]
     if not ts:
         raise ValueError("%s: no tensors" % name)
-    dev = ts[0].device
-    if dev.type != "cuda":
+    # (sets of small values instead of one comparison per tensor: hundreds of tensors are a case where the host's time counts)
+    where = {t.get_device() for t in ts}
+    if where == {-1}:
         raise RuntimeError("nirrt_star_amd.nnops.%s got a CPU tensor: the package only has the HIP kernels (move it to 'cuda')" % name)
-    for t in ts:
-        if t.device != dev or t.dtype not in _TYPES or t.layout != torch.strided:
-            raise ValueError("%s: dense float32, bfloat16 or float16 tensors of one device, not %s %s on %s" % (name, t.layout, t.dtype, t.device))
-    return ts, dev
+    if len(where) != 1 or {t.layout for t in ts} != {torch.strided} or not {t.dtype for t in ts} <= _TYPES.keys():
+        raise ValueError("%s: dense float32, bfloat16 or float16 tensors of one device" % name)
+    return ts, ts[0].device
 
 
 def _table(ts, outs=None):
@@ -318,15 +325,17 @@ def clip_grad_norm_(grads, max_norm, out=None):
         dst = src
     else:
         dst, dev_o = _tensor_list(name, out)
-        if dev_o != dev or any(o.shape != t.shape or not o.is_contiguous() for o, t in zip(dst, ts)):
+        if dev_o != dev or [o.shape for o in dst] != [t.shape for t in ts] or not all([o.is_contiguous() for o in dst]):
             raise ValueError("%s: outputs must be contiguous, of the gradients' shapes and on their device" % name)
     tab = _table(src, dst)
-    full = tab[tab["n"] > 0]
-    if len(np.unique(full["out"])) != len(full):
+    full = tab[tab["n"] > 0] if (tab["n"] == 0).any() else tab
+    places = set(full["out"].tolist())
+    if len(places) != len(full):
         raise ValueError("%s: a tensor is named twice" % name)
     if out is not None:
         own = full["out"] == full["data"]
-        if np.isin(full["out"][~own], full["data"]).any() or (full["dtype"][own] != full["out_dtype"][own]).any():
+        if places & set(full["data"][~own].tolist()) or (places & set(full["data"][own].tolist())
+                                                         and ((full["dtype"] != full["out_dtype"]) & own).any()):
             raise ValueError("%s: an output shares memory with another gradient, or with its own of another type" % name)
     with _on(dev):
         norm = _norm(tab, dev)
