@@ -208,15 +208,31 @@ template <class T, int BM, int BN, int WM, int WN, bool RCA, bool RCB> struct Ti
 // out-of-range offsets give zeros.  The LDS place of a lane's chunk is fixed (base + 16 lane), so the swizzle is applied to the global
 // address.  A KC operand lies as in Tile; an RC operand lies as it is, STEP rows of k with R elements each, and is transposed on its way
 // out: 16-bit by the transposing LDS read (4 k x 16 rows per 16 lanes), 32-bit because an MFMA operand is one element per lane anyway.
-// Two stages: one is multiplied while the other is on its way; one barrier per step.
+// Four stages of 64 bytes of k per row, in a ring: one is multiplied, the next has arrived (its first operands are read during the last
+// products of this one), two are on their way - a stage's loads have two steps of products to arrive in, and the barrier between steps finds
+// every wave's products still running.  (Two stages of 128 bytes, each waited for whole: 58 % of the MFMA cycles busy, 600 us for
+// 16384 x 4096 x 4096 in bf16.)
+constexpr int STAGES = 4, RING_BYTES = 64, RING_CHUNKS = RING_BYTES / 16;
+__device__ __forceinline__ int ring_sw(int row) { return (row >> 2) & 3; }   // 16 lanes on 16 rows: 16 places of 16 bytes
 constexpr unsigned NOWHERE = 0x7ffffff0u;   // an offset beyond every buffer (direct() keeps them below)
 
+// 16 bytes per lane from buffer + offset to lds + 16 lane.  Written out, because the compiler does not know which part of the LDS a load of its own
+// writes and waits for all of them before every transposing read (902 us instead of 567 for dw of 16384 x 4096 x 4096).  It has no
+// result register; the waits are arrive() below, which every use of the LDS stands behind.
+__device__ __forceinline__ void load_to_lds(u32x4 buffer, const u32x4 *lds, unsigned offset)
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    const unsigned where = (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void *)lds;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(where), "v"(offset), "s"(buffer) : "memory");
+#endif
+}
+
 template <class T, int R, int NT, bool RC> struct DirectOperand {
-    static constexpr int CE = Elem<T>::PER_CHUNK, STEP = Elem<T>::STEP, N = R * CHUNKS / NT, PER_K = R / CE;
+    static constexpr int CE = Elem<T>::PER_CHUNK, STEP = RING_BYTES / sizeof(T), N = R * RING_CHUNKS / NT, PER_K = R / CE;
     const char *base;          // of the step to load next
     int64_t bytes, advance;    // valid bytes from base on, per step
     unsigned at[N];            // a lane's offset in a step
-    int first;                 // KC: the first k of its chunk (the same in all N: rows NT / 8 apart have the same swizzle)
+    int first;                 // KC: the first k of its chunk (the same in all N: rows NT / 4 apart have the same swizzle)
 
     // 16-byte blocks of an RC row are moved by whole bank groups: 64 bytes by k mod 4 (16-bit: a transposing read takes 4 k x 64 bytes at
     // a time), 128 bytes by k / 4 (32-bit: the halves of a wave read k 4 apart)
@@ -229,7 +245,7 @@ template <class T, int R, int NT, bool RC> struct DirectOperand {
             const int rows = o.rows - r0 < R ? o.rows - r0 : R;
             base = (const char *)(o.p + (int64_t)r0 * o.ld + k0);
             bytes = (rows - 1) * row_bytes + (int64_t)(k1 - k0) * sizeof(T);
-            advance = ROW_BYTES;
+            advance = RING_BYTES;
         } else {
             base = (const char *)(o.p + (int64_t)k0 * o.ld + r0);
             // (whole 4-byte words count as in or out of range: the last one belongs to the row even if only half of it does)
@@ -240,7 +256,7 @@ template <class T, int R, int NT, bool RC> struct DirectOperand {
         for (int i = 0; i < N; i++) {
             const int p = i * NT + tid;
             if constexpr (!RC) {
-                const int r = p >> 3, c = (p & 7) ^ sw(r);
+                const int r = p / RING_CHUNKS, c = (p % RING_CHUNKS) ^ ring_sw(r);
                 at[i] = (unsigned)(r * row_bytes + c * 16);
                 first = c * CE;
             } else {
@@ -250,33 +266,32 @@ template <class T, int R, int NT, bool RC> struct DirectOperand {
             }
         }
     }
-    // left: k still to come, this step's included
-    __device__ __forceinline__ void load(u32x4 *lds, int left, int wave)
+    // one of the N loads of a step (left: k still to come, this step's included); next() moves on
+    __device__ __forceinline__ void load(const u32x4 *lds, int i, int left, int wave) const
     {
-#ifdef __HIP_DEVICE_COMPILE__   // (the host pass does not know the buffer and LDS types)
-        const int64_t lim = bytes < (int64_t)NOWHERE ? bytes : (int64_t)NOWHERE;
-        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)(lim > 0 ? lim : 0), 0x00020000);
-#pragma unroll
-        for (int i = 0; i < N; i++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)(lds + i * NT + wave * 64), 16,
-                                                     RC || first < left ? at[i] : NOWHERE, 0, 0, 0);
-#endif
+        const int64_t lim = bytes < (int64_t)NOWHERE ? bytes : (int64_t)NOWHERE;      // (below zero behind the end: an empty buffer)
+        const u32x4 buffer = {(unsigned)(uintptr_t)base, (unsigned)((uintptr_t)base >> 32) & 0xffffu, (unsigned)(lim > 0 ? lim : 0), 0x00020000u};
+        load_to_lds(buffer, lds + i * NT + wave * 64, RC || first < left ? at[i] : NOWHERE);
+    }
+    __device__ __forceinline__ void next()
+    {
         base += advance;
         bytes -= advance;
     }
 };
 
-// reads the operands of an MFMA group (32 bytes of k, s = 0 .. 3) for M blocks of 32 rows: the lane's byte offsets in the operand's part of
-// a stage, so that everything else is a constant in the instruction
+// reads the operands of an MFMA group (32 bytes of k, two per stage) for M blocks of 32 rows: the lane's byte offsets in the operand's part
+// of a stage, so that everything else is a constant in the instruction
 template <class T, int R, bool RC, int M> struct Reader {
-    int at[RC ? M : CHUNKS / 2];
+    static constexpr int GROUPS = RING_CHUNKS / 2;
+    int at[RC ? M : GROUPS];
 
     __device__ __forceinline__ void start(int row0, int lane, int where)
     {
         if constexpr (!RC) {
-            const int r = row0 + (lane & 31), c = (lane >> 5) ^ sw(r);
+            const int r = row0 + (lane & 31), c = (lane >> 5) ^ ring_sw(r);
 #pragma unroll
-            for (int s = 0; s < CHUNKS / 2; s++) at[s] = where + r * ROW_BYTES + (c ^ (2 * s)) * 16;
+            for (int s = 0; s < GROUPS; s++) at[s] = where + r * RING_BYTES + (c ^ (2 * s)) * 16;
         } else {
             typedef DirectOperand<T, R, 64, true> Op;
             const int i = lane & 15, k = sizeof(T) == 2 ? 8 * (lane >> 5) + (i >> 2) : 4 * (lane >> 5);
@@ -285,17 +300,12 @@ template <class T, int R, bool RC, int M> struct Reader {
             for (int m = 0; m < M; m++) at[m] = where + k * (R * (int)sizeof(T)) + (((row + 32 * m) * (int)sizeof(T)) ^ (Op::turn(k) * 16));
         }
     }
-    __device__ __forceinline__ void flip(int stage)
-    {
-#pragma unroll
-        for (int i = 0; i < (RC ? M : CHUNKS / 2); i++) at[i] ^= stage;
-    }
-    __device__ __forceinline__ u32x4 read(const u32x4 *lds, int m, int s) const
+    __device__ __forceinline__ u32x4 read(const u32x4 *lds, int stage, int m, int s) const
     {
 #ifdef __HIP_DEVICE_COMPILE__
-        const __attribute__((address_space(3))) char *p = (const __attribute__((address_space(3))) char *)lds;
+        const __attribute__((address_space(3))) char *p = (const __attribute__((address_space(3))) char *)lds + stage;
         if constexpr (!RC) {
-            return *(const __attribute__((address_space(3))) u32x4 *)(p + at[s] + m * 32 * ROW_BYTES);
+            return *(const __attribute__((address_space(3))) u32x4 *)(p + at[s] + m * 32 * RING_BYTES);
         } else if constexpr (sizeof(T) == 2) {
             typedef short s16x4 __attribute__((ext_vector_type(4)));
             s16x4 q[2];
@@ -317,13 +327,30 @@ template <class T, int R, bool RC, int M> struct Reader {
     }
 };
 
+// all but the newest `left` loads of every wave of the workgroup have arrived
+template <int left> __device__ __forceinline__ void arrive()
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(left) : "memory");
+#endif
+}
+
 template <class T, int BM, int BN, int WM, int WN, bool RCA, bool RCB> struct DirectTile {
-    static constexpr int NT = 64 * WM * WN, WAVES_M = WM, WAVES_N = WN, MI = BM / WM / 32, NI = BN / WN / 32, STAGE = (BM + BN) * CHUNKS;
-    static constexpr int LDS_CHUNKS = 2 * STAGE;
+    static constexpr int NT = 64 * WM * WN, WAVES_M = WM, WAVES_N = WN, MI = BM / WM / 32, NI = BN / WN / 32;
+    static constexpr int STAGE = (BM + BN) * RING_CHUNKS, LDS_CHUNKS = STAGES * STAGE, STEP = RING_BYTES / sizeof(T);
     f32x16 acc[MI][NI];
 
     static __device__ __forceinline__ int row(int wave, int lane, int mi, int e) { return (wave / WN) * (BM / WM) + mi * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3); }
     static __device__ __forceinline__ int col(int wave, int lane, int ni) { return (wave % WN) * (BN / WN) + ni * 32 + (lane & 31); }
+
+    typedef DirectOperand<T, BM, NT, RCA> OpA;
+    typedef DirectOperand<T, BN, NT, RCB> OpB;
+    static constexpr int LOADS = OpA::N + OpB::N;      // per wave and stage
+    static __device__ __forceinline__ void load(const OpA &oa, const OpB &ob, u32x4 *stage, int i, int left, int wave)
+    {
+        if (i < OpA::N) oa.load(stage, i, left, wave);
+        else ob.load(stage + BM * RING_CHUNKS, i - OpA::N, left, wave);
+    }
 
     __device__ __forceinline__ void mainloop(const Operand<T> &a, const Operand<T> &b, int i0, int j0, int k0, int k1, u32x4 *lds)
     {
@@ -335,48 +362,58 @@ template <class T, int BM, int BN, int WM, int WN, bool RCA, bool RCB> struct Di
 #pragma unroll
                 for (int e = 0; e < 16; e++) acc[mi][ni][e] = 0.f;
         if (k0 >= k1) return;
-        DirectOperand<T, BM, NT, RCA> oa;
-        DirectOperand<T, BN, NT, RCB> ob;
+        OpA oa;
+        OpB ob;
         oa.start(a, i0, k0, k1, tid);
         ob.start(b, j0, k0, k1, tid);
-        __syncthreads();                     // (a tile before this one has been read)
-        oa.load(lds, k1 - k0, wave);
-        ob.load(lds + BM * CHUNKS, k1 - k0, wave);
         Reader<T, BM, RCA, MI> xa;
         Reader<T, BN, RCB, NI> xb;
         xa.start((wave / WN) * (BM / WM), lane, 0);
-        xb.start((wave % WN) * (BN / WN), lane, BM * ROW_BYTES);
-        int other = STAGE;
-        for (int k = k0; k < k1; k += Elem<T>::STEP) {
-            __syncthreads();                 // this step has arrived, and the stage of the one before has been read
-            const int left = k1 - k - Elem<T>::STEP;
-            if (left > 0) {
-                oa.load(lds + other, left, wave);
-                ob.load(lds + other + BM * CHUNKS, left, wave);
-            }
-            // operands of the next group are read while this one is multiplied
-            u32x4 fa[2][MI], fb[2][NI];
+        xb.start((wave % WN) * (BN / WN), lane, BM * RING_BYTES);
+        __syncthreads();                     // (a tile before this one has been read)
+        int left = k1 - k0;                  // k that have not been asked for; behind the end the loads give zeros, the count stays even
 #pragma unroll
-            for (int mi = 0; mi < MI; mi++) fa[0][mi] = xa.read(lds, mi, 0);
+        for (int p = 0; p < STAGES - 1; p++) {
 #pragma unroll
-            for (int ni = 0; ni < NI; ni++) fb[0][ni] = xb.read(lds, ni, 0);
-#pragma unroll
-            for (int s = 0; s < CHUNKS / 2; s++) {
-                if (s + 1 < CHUNKS / 2) {
-#pragma unroll
-                    for (int mi = 0; mi < MI; mi++) fa[(s + 1) & 1][mi] = xa.read(lds, mi, s + 1);
-#pragma unroll
-                    for (int ni = 0; ni < NI; ni++) fb[(s + 1) & 1][ni] = xb.read(lds, ni, s + 1);
-                }
-#pragma unroll
-                for (int mi = 0; mi < MI; mi++)
-#pragma unroll
-                    for (int ni = 0; ni < NI; ni++) acc[mi][ni] = mma((T)0.f, fa[s & 1][mi], fb[s & 1][ni], acc[mi][ni]);
-            }
-            xa.flip(STAGE * 16);
-            xb.flip(STAGE * 16);
-            other ^= STAGE;
+            for (int i = 0; i < LOADS; i++) load(oa, ob, lds + p * STAGE, i, left, wave);
+            oa.next();
+            ob.next();
+            left -= STEP;
         }
+        arrive<LOADS>();
+        u32x4 fa[2][MI], fb[2][NI];
+#pragma unroll
+        for (int mi = 0; mi < MI; mi++) fa[0][mi] = xa.read(lds, 0, mi, 0);
+#pragma unroll
+        for (int ni = 0; ni < NI; ni++) fb[0][ni] = xb.read(lds, 0, ni, 0);
+        int now = 0;                         // this stage's place in the ring, in chunks
+        for (int k = k0; k < k1; k += STEP) {
+            const int next = now + STAGE == LDS_CHUNKS ? 0 : now + STAGE, free = now == 0 ? LDS_CHUNKS - STAGE : now - STAGE;
+            // a row of products at a time, with the operands of the next group and the loads of three stages on in between (the memory
+            // pipe takes a load of a wave in 16 cycles: all of a step's at once hold up the products behind them)
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+#pragma unroll
+                for (int mi = 0; mi < MI; mi++) {
+                    fa[1 - s][mi] = xa.read(lds, (s ? next : now) * 16, mi, 1 - s);
+#pragma unroll
+                    for (int ni = 0; ni < NI; ni++)
+                        if (ni * MI / NI == mi) fb[1 - s][ni] = xb.read(lds, (s ? next : now) * 16, ni, 1 - s);
+#pragma unroll
+                    for (int i = 0; i < LOADS; i++)
+                        if (i * 2 * MI / LOADS == s * MI + mi) load(oa, ob, lds + free, i, left, wave);
+                    __builtin_amdgcn_sched_barrier(0);      // (left alone, the compiler reads behind the products and waits)
+#pragma unroll
+                    for (int ni = 0; ni < NI; ni++) acc[mi][ni] = mma((T)0.f, fa[s][mi], fb[s][ni], acc[mi][ni]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            oa.next();
+            ob.next();
+            left -= STEP;
+            arrive<LOADS>();
+            now = next;
+        }
+        arrive<0>();                         // (the loads behind the end)
     }
 };
 
@@ -433,7 +470,7 @@ __device__ __forceinline__ float act_slope(int act, float z)
     }
 }
 
-// ---- what a product does with four neighbouring elements C[i, j ..] (n of them, 1 .. 4, exist) ---------------------------------------
+// ---- what a product does with four neighbouring elements C[i, j ..] of Q rows (row q: i + q step; rows of them exist, n columns) ---------
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 template <class T> __device__ __forceinline__ f32x4 load4(const T *p, int n)
 {
@@ -456,16 +493,32 @@ template <class T> struct EpiLinear {
     T *y, *z;
     int64_t ldr, ldy;
     int act, n;
-    __device__ __forceinline__ void put(f32x4 c, int i, int j, int cnt) const
+    template <int Q> __device__ __forceinline__ void put(f32x4 (&c)[Q], int i, int step, int rows, int j, int cnt) const
     {
-        if (b) c += load4(b + j, cnt);
-        if (z) store4(z + (int64_t)i * n + j, c, cnt);
+        if (b) {
+            const f32x4 add = load4(b + j, cnt);
+#pragma unroll
+            for (int q = 0; q < Q; q++) c[q] += add;
+        }
+        if (z) {
+#pragma unroll
+            for (int q = 0; q < Q; q++)
+                if (q < rows) store4(z + (int64_t)(i + q * step) * n + j, c[q], cnt);
+        }
         if (act != NIRRT_NN_ACT_NONE) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) c[e] = act_value(act, c[e]);
+            for (int q = 0; q < Q; q++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) c[q][e] = act_value(act, c[q][e]);
         }
-        if (r) c += load4(r + (int64_t)i * ldr + j, cnt);
-        store4(y + (int64_t)i * ldy + j, c, cnt);
+        if (r) {
+#pragma unroll
+            for (int q = 0; q < Q; q++)
+                if (q < rows) c[q] += load4(r + (int64_t)(i + q * step) * ldr + j, cnt);
+        }
+#pragma unroll
+        for (int q = 0; q < Q; q++)
+            if (q < rows) store4(y + (int64_t)(i + q * step) * ldy + j, c[q], cnt);
     }
 };
 // out = scale C (contiguous rows of n); scale on the device or 1
@@ -474,16 +527,39 @@ template <class T> struct EpiPlain {
     const float *scale;
     float factor;
     int n;
-    __device__ __forceinline__ void put(f32x4 c, int i, int j, int cnt) const { store4(out + (int64_t)i * n + j, c * (scale ? *scale * factor : factor), cnt); }
+    template <int Q> __device__ __forceinline__ void put(f32x4 (&c)[Q], int i, int step, int rows, int j, int cnt) const
+    {
+        const float f = scale ? *scale * factor : factor;
+#pragma unroll
+        for (int q = 0; q < Q; q++)
+            if (q < rows) store4(out + (int64_t)(i + q * step) * n + j, c[q] * f, cnt);
+    }
 };
 // acc (+)= C in fp32: the sum over pieces of the reduction that are multiplied one after the other
 template <class T> struct EpiAccumulate {
     float *out;
     int n, first;
-    __device__ __forceinline__ void put(f32x4 c, int i, int j, int cnt) const
+    template <int Q> __device__ __forceinline__ void put(f32x4 (&c)[Q], int i, int step, int rows, int j, int cnt) const
     {
-        float *q = out + (int64_t)i * n + j;
-        store4(q, first ? c : c + load4(q, cnt), cnt);
+        if (!first) {
+#pragma unroll
+            for (int q = 0; q < Q; q++)
+                if (q < rows) c[q] += load4(out + (int64_t)(i + q * step) * n + j, cnt);
+        }
+#pragma unroll
+        for (int q = 0; q < Q; q++)
+            if (q < rows) store4(out + (int64_t)(i + q * step) * n + j, c[q], cnt);
+    }
+};
+// a part of a cut reduction: part p at out + p m n
+struct EpiPart {
+    float *out;
+    int n;
+    template <int Q> __device__ __forceinline__ void put(f32x4 (&c)[Q], int i, int step, int rows, int j, int cnt) const
+    {
+#pragma unroll
+        for (int q = 0; q < Q; q++)
+            if (q < rows) store4(out + (int64_t)(i + q * step) * n + j, c[q], cnt);
     }
 };
 
@@ -501,9 +577,11 @@ __global__ __launch_bounds__(Tl::NT) void k_gemm(Operand<T> a, Operand<T> b, int
     const int k0 = blockIdx.y * part, k1 = k - k0 < part ? k : k0 + part;
     t.mainloop(a, b, ti * BM, tj * BN, k0, k1, lds);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    float *pp = gridDim.y > 1 ? partial + (int64_t)blockIdx.y * m * n : nullptr;
     const int i0 = ti * BM + Tl::row(wave, 0, 0, 0), j0 = tj * BN + Tl::col(wave, 0, 0);
     float *slab = (float *)(lds + wave * SLAB);
+    constexpr int PER_ROW = COLS / 4, STEP = 64 / PER_ROW, Q = 32 / STEP;     // lanes per row, rows per pass, passes
+    const int r = lane / PER_ROW, c = lane % PER_ROW * 4, j = j0 + c, cnt = n - j < 4 ? n - j : 4;
+    const EpiPart part_out = {partial + (int64_t)blockIdx.y * m * n, n};
     __syncthreads();                        // (the last step has been read)
 #pragma unroll
     for (int mi = 0; mi < Tl::MI; mi++) {
@@ -513,16 +591,13 @@ __global__ __launch_bounds__(Tl::NT) void k_gemm(Operand<T> a, Operand<T> b, int
             for (int e = 0; e < 16; e++) slab[(8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * LD + ni * 32 + (lane & 31)] = t.acc[mi][ni][e];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-#pragma unroll 2
-        for (int q = 0; q < COLS / 8; q++) {
-            const int at = q * 64 + lane, r = at / (COLS / 4), c = at % (COLS / 4) * 4, i = i0 + 32 * mi + r, j = j0 + c;
-            const f32x4 v = *(const f32x4 *)(slab + r * LD + c);
-            if (i < m && j < n) {
-                const int cnt = n - j < 4 ? n - j : 4;
-                if (pp) store4(pp + (int64_t)i * n + j, v, cnt);
-                else epi.put(v, i, j, cnt);
-            }
-        }
+        f32x4 v[Q];
+#pragma unroll
+        for (int q = 0; q < Q; q++) v[q] = *(const f32x4 *)(slab + (q * STEP + r) * LD + c);
+        const int i = i0 + 32 * mi + r, left = m - i, rows = left <= 0 || cnt <= 0 ? 0 : (left - 1) / STEP + 1;
+        if (gridDim.y > 1) part_out.put(v, i, STEP, rows, j, cnt);
+        else if (rows >= Q && cnt == 4) epi.put(v, i, STEP, Q, j, 4);         // (nothing to check)
+        else if (rows > 0) epi.put(v, i, STEP, rows, j, cnt);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
@@ -534,10 +609,10 @@ template <class Epi> __global__ __launch_bounds__(256) void k_join(const float *
     for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < all; at += (int64_t)gridDim.x * 256) {
         const int i = (int)(at / quads), j = (int)(at - i * quads) * 4, cnt = n - j < 4 ? n - j : 4;
         const float *p = partial + (int64_t)i * n + j;
-        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+        f32x4 s[1] = {{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll 4
-        for (int q = 0; q < parts; q++) s += load4(p + q * size, cnt);
-        epi.put(s, i, j, cnt);
+        for (int q = 0; q < parts; q++) s[0] += load4(p + q * size, cnt);
+        epi.put(s, i, 0, 1, j, cnt);
     }
 }
 
@@ -692,18 +767,29 @@ __global__ __launch_bounds__(Tl::NT) void k_ce_stats(Operand<T> w, Operand<T> x,
         if (r0 + c < rows) stats[(int64_t)blockIdx.y * rows + r0 + c] = make_float2(top, sum);
     }
 }
-// parts of a row's statistics -> lse, weighted loss; the block's sums of loss and weight (in double) for k_ce_total
+// parts of a row's statistics (eight lanes per row) -> lse, weighted loss; the block's sums of loss and weight (in double) for k_ce_total
+constexpr int CE_ROWS = 32;
 __global__ __launch_bounds__(256) void k_ce_rows(const float2 *stats, int parts, const float *target_score, const int64_t *target, const float *cw,
                                                  int64_t ignore, int rows, int classes, float *lse, float *nll, double *sums)
 {
     __shared__ double part[2][4];
-    const int r = blockIdx.x * 256 + threadIdx.x;
+    const int r = blockIdx.x * CE_ROWS + threadIdx.x / 8, p0 = threadIdx.x & 7;
     double a = 0., b = 0.;
-    if (r < rows) {
-        float top = -__builtin_inff(), sum = 0.f;
-        for (int p = 0; p < parts; p++) top = fmaxf(top, stats[(int64_t)p * rows + r].x);
-        const float ref = top == -__builtin_inff() ? 0.f : top;
-        for (int p = 0; p < parts; p++) { const float2 q = stats[(int64_t)p * rows + r]; sum += q.y * __builtin_amdgcn_exp2f(q.x - ref); }
+    float top = -__builtin_inff(), sum = 0.f;
+    if (r < rows)
+        for (int p = p0; p < parts; p += 8) {
+            const float2 q = stats[(int64_t)p * rows + r];
+            const float hi = fmaxf(top, q.x), ref = hi == -__builtin_inff() ? 0.f : hi;
+            sum = sum * __builtin_amdgcn_exp2f(top - ref) + q.y * __builtin_amdgcn_exp2f(q.x - ref);
+            top = hi;
+        }
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) {
+        const float t2 = __shfl_xor(top, d), s2 = __shfl_xor(sum, d), hi = fmaxf(top, t2), ref = hi == -__builtin_inff() ? 0.f : hi;
+        sum = sum * __builtin_amdgcn_exp2f(top - ref) + s2 * __builtin_amdgcn_exp2f(t2 - ref);
+        top = hi;
+    }
+    if (r < rows && p0 == 0) {
         const float l = (top + __builtin_amdgcn_logf(sum)) * LN2;
         const int64_t t = target[r];
         const float wt = row_weight(cw, t, ignore, classes);
@@ -777,18 +863,18 @@ __global__ __launch_bounds__(256) void k_ce_scale(const float *tops, int blocks,
         scale[1] = usable ? 1.f / top : 1.f;
     }
 }
-// x with the rows that do not count set to zero (whatever they hold: 0 x NaN must not reach dw) and its rows padded with zeros to ld, so
-// that whole aligned chunks can be read; one pass over x, a small part of the products behind it
+// x with the rows that do not count set to zero (whatever they hold: 0 x NaN must not reach dw), padded with zeros to ld columns and
+// rows_out rows, so that whole aligned chunks can be read; one pass over x, a small part of the products behind it
 template <class T>
-__global__ __launch_bounds__(256) void k_ce_rows_copy(const T *x, int64_t ldx, const float *coef, T *out, int64_t ld, int rows, int k)
+__global__ __launch_bounds__(256) void k_ce_rows_copy(const T *x, int64_t ldx, const float *coef, T *out, int64_t ld, int rows, int rows_out, int k)
 {
     constexpr int V = 16 / sizeof(T);
-    const int64_t per = ld / V, all = rows * per;
+    const int64_t per = ld / V, all = rows_out * per;
     for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < all; at += (int64_t)gridDim.x * 256) {
         const int64_t r = at / per;
         const int c = (int)(at - r * per) * V;
         Pack<T, V> v = {};
-        if (!coef || coef[r] != 0.f) v = load_some<T, V>(x + r * ldx + c, k - c);
+        if (r < rows && (!coef || coef[r] != 0.f)) v = load_some<T, V>(x + r * ldx + c, k - c);
         store_pack(out + r * ld + c, v);
     }
 }
@@ -804,18 +890,28 @@ template <class T> struct EpiSoftmaxGrad {
     const float *lse, *coef, *scale;
     const int64_t *target;
     int64_t v0;
-    __device__ __forceinline__ void put(f32x4 c, int i, int j, int cnt) const
+    int rows;
+    template <int Q> __device__ __forceinline__ void put(f32x4 (&c)[Q], int i, int step, int rows_here, int j, int cnt) const
     {
-        const float add = b ? (float)b[v0 + i] : 0.f, lift = scale[1] * Factor<T>::VALUE;
-        const f32x4 l = load4(lse + j, cnt), w = load4(coef + j, cnt);
-        f32x4 o;
+        const float lift = scale[1] * Factor<T>::VALUE;
+        const int real = rows - j < cnt ? rows - j : cnt;        // (columns behind the last row of x pad g with zeros)
+        const f32x4 l = load4(lse + j, real), w = load4(coef + j, real);
+        int64_t t[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            float p = __expf(c[e] + add - l[e]);
-            if (e < cnt && target[j + e] == v0 + i) p -= 1.f;
-            o[e] = w[e] == 0.f ? 0.f : p * (w[e] * lift);
-        }
-        store4(g + (int64_t)i * ldg + j, o, cnt);
+        for (int e = 0; e < 4; e++) t[e] = e < real ? target[j + e] - v0 - i : -1;
+#pragma unroll
+        for (int q = 0; q < Q; q++)
+            if (q < rows_here) {
+                const float add = b ? (float)b[v0 + i + q * step] : 0.f;
+                f32x4 o;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float p = __expf(c[q][e] + add - l[e]);
+                    if (t[e] == q * step) p -= 1.f;
+                    o[e] = w[e] == 0.f ? 0.f : p * (w[e] * lift);
+                }
+                store4(g + (int64_t)(i + q * step) * ldg + j, o, cnt);
+            }
     }
 };
 // db[v] = scale / FACTOR sum_r g'[v, r]: a wave per class
@@ -1275,11 +1371,13 @@ bool few_layout(int dtype, int64_t rows, int64_t classes, int64_t k, Few &f)
 // are copied into such (k_ce_rows_copy): the products read them many times
 int64_t padded(int dtype, int64_t k) { const int64_t c = 16 / elem_size(dtype); return (k + c - 1) / c * c; }
 bool whole_rows(int dtype, const void *p, int64_t ld, int64_t k) { return (uintptr_t)p % 16 == 0 && ld * elem_size(dtype) % 16 == 0 && k == padded(dtype, k); }
-template <class T> void copy_rows(const void *x, int64_t ldx, const float *coef, T *out, int64_t ld, int64_t rows, int64_t k, hipStream_t st)
+template <class T>
+void copy_rows(const void *x, int64_t ldx, const float *coef, T *out, int64_t ld, int64_t rows, int64_t rows_out, int64_t k, hipStream_t st)
 {
-    const int64_t blocks = ceil_div(rows * (ld * (int64_t)sizeof(T) / 16), 256);
+    const int64_t blocks = ceil_div(rows_out * (ld * (int64_t)sizeof(T) / 16), 256);
     if (blocks > 0)
-        hipLaunchKernelGGL((k_ce_rows_copy<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, (const T *)x, ldx, coef, out, ld, (int)rows, (int)k);
+        hipLaunchKernelGGL((k_ce_rows_copy<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, (const T *)x, ldx, coef, out, ld,
+                           (int)rows, (int)rows_out, (int)k);
 }
 struct CeForward { int edge, parts, part; int64_t stats, score, sums, xs, ws, total; };
 CeForward ce_layout(int dtype, int64_t rows, int64_t classes, int64_t k)
@@ -1296,7 +1394,7 @@ CeForward ce_layout(int dtype, int64_t rows, int64_t classes, int64_t k)
     f.parts = (int)(class_tiles > 0 ? ceil_div(class_tiles, per) : 1);
     f.stats = round256(8 * rows * f.parts);
     f.score = round256(4 * rows);
-    f.sums = round256(16 * (ceil_div(rows, 256) + 512));
+    f.sums = round256(16 * (ceil_div(rows, CE_ROWS) + 512));
     f.xs = round256(rows * padded(dtype, k) * elem_size(dtype));
     f.ws = round256(classes * padded(dtype, k) * elem_size(dtype));
     f.total = f.stats + f.score + f.sums + f.xs + f.ws;
@@ -1318,10 +1416,10 @@ int ce_forward_t(int dtype, const void *x, int64_t ldx, const void *w, int64_t l
         FEW_LAUNCH(k_ce_few, f.lds, (const T *)x, ldx, (const T *)w, ldw, (const T *)b, target, cw, ignore, (int)rows, (int)classes, (int)k, f.lanes, lse,
                    nll, sums);
     } else if (rows > 0) {
-        blocks = ceil_div(rows, 256);
+        blocks = ceil_div(rows, CE_ROWS);
         const int64_t kp = padded(dtype, k), row_tiles = ceil_div(rows, l.edge);
-        if (!whole_rows(dtype, x, ldx, k)) { copy_rows(x, ldx, nullptr, xs, kp, rows, k, st); x = xs; ldx = kp; }
-        if (!whole_rows(dtype, w, ldw, k)) { copy_rows(w, ldw, nullptr, wsp, kp, classes, k, st); w = wsp; ldw = kp; }
+        if (!whole_rows(dtype, x, ldx, k)) { copy_rows(x, ldx, nullptr, xs, kp, rows, rows, k, st); x = xs; ldx = kp; }
+        if (!whole_rows(dtype, w, ldw, k)) { copy_rows(w, ldw, nullptr, wsp, kp, classes, classes, k, st); w = wsp; ldw = kp; }
         const dim3 grid((unsigned)row_tiles, (unsigned)l.parts);
         const Operand<T> ow = op((const T *)w, ldw, classes), ox = op((const T *)x, ldx, rows);
         if (!direct<T, false>(ow, kp) || !direct<T, false>(ox, kp)) return -1;   // (rows of more than 4 MB)
@@ -1354,14 +1452,14 @@ CeBackward ce_backward_layout(int dtype, int64_t rows, int64_t classes, int64_t 
     l.piece = l.ldg > 0 ? G_ELEMS / l.ldg / 256 * 256 : classes;
     if (l.piece < 256) l.piece = 256;
     if (l.piece > classes) l.piece = classes;
-    l.pg = plan(dtype, l.piece, rows, k);
+    l.pg = plan(dtype, l.piece, l.ldg, k);
     l.pg.parts = 1;                    // (the scores are not cut: the softmax needs whole ones)
     l.pg.part = (int)(padded(dtype, k) > 0 ? padded(dtype, k) : 1);
     l.px = plan(dtype, rows, k, l.piece);
-    l.pw = plan(dtype, l.piece, k, rows);
+    l.pw = plan(dtype, l.piece, k, l.ldg);
     l.coef = round256(4 * rows) + 256;
     l.tops = round256(4 * ceil_div(rows, 256));
-    l.xs = round256(rows * padded(dtype, k) * e);
+    l.xs = round256(l.ldg * padded(dtype, k) * e);
     l.ws = round256(classes * padded(dtype, k) * e);
     l.g = round256(l.ldg * l.piece * e);
     l.acc = l.piece < classes ? round256(4 * rows * k) : 0;
@@ -1396,15 +1494,15 @@ int ce_backward_t(int dtype, const void *x, int64_t ldx, const void *w, int64_t 
     if (blocks > 0)
         hipLaunchKernelGGL(k_ce_coefficients, dim3((unsigned)blocks), dim3(256), 0, st, dloss, stride, total, target, cw, ignore, (int)rows, (int)classes, coef, tops);
     hipLaunchKernelGGL(k_ce_scale, dim3(1), dim3(256), 0, st, tops, (int)blocks, scale);
-    copy_rows(x, ldx, coef, xs, kp, rows, k, st);
-    if (!whole_rows(dtype, w, ldw, k)) { copy_rows(w, ldw, nullptr, wsp, kp, classes, k, st); w = wsp; ldw = kp; }
+    copy_rows(x, ldx, coef, xs, kp, rows, l.ldg, k, st);
+    if (!whole_rows(dtype, w, ldw, k)) { copy_rows(w, ldw, nullptr, wsp, kp, classes, classes, k, st); w = wsp; ldw = kp; }
     const float unlift = 1.f / Factor<T>::VALUE;
     for (int64_t v0 = 0; v0 < classes; v0 += l.piece) {
         const int64_t nv = classes - v0 < l.piece ? classes - v0 : l.piece;
         const T *wp = (const T *)w + v0 * ldw;
         if (rows > 0) {
-            const EpiSoftmaxGrad<T> eg = {g, l.ldg, (const T *)b, lse, coef, scale, target, v0};
-            if (int rc = gemm<T, false, false>(op(wp, ldw, nv), op((const T *)xs, kp, rows), nv, rows, kp, l.pg, nullptr, eg, st)) return rc;
+            const EpiSoftmaxGrad<T> eg = {g, l.ldg, (const T *)b, lse, coef, scale, target, v0, (int)rows};
+            if (int rc = gemm<T, false, false>(op(wp, ldw, nv), op((const T *)xs, kp, l.ldg), nv, l.ldg, kp, l.pg, nullptr, eg, st)) return rc;
         }
         if (db) hipLaunchKernelGGL((k_ce_bias<T>), dim3((unsigned)ceil_div(nv, 4)), dim3(256), 0, st, (const T *)g, l.ldg, (int)rows, (int)nv, scale, (T *)db + v0);
         if (dx && rows > 0 && k > 0) {
@@ -1416,7 +1514,7 @@ int ce_backward_t(int dtype, const void *x, int64_t ldx, const void *w, int64_t 
         }
         if (dw && k > 0) {
             const EpiPlain<T> ep = {(T *)dw + v0 * k, scale, unlift, (int)k};
-            if (int rc = gemm<T, false, true>(op((const T *)g, l.ldg, nv), op((const T *)xs, kp, k), nv, k, rows, l.pw, part, ep, st)) return rc;
+            if (int rc = gemm<T, false, true>(op((const T *)g, l.ldg, nv), op((const T *)xs, kp, k), nv, k, l.ldg, l.pw, part, ep, st)) return rc;
         }
     }
     if (dx && l.acc && rows > 0 && k > 0) {
