@@ -19,15 +19,17 @@ enum { NIRRT_NN_F32 = 0, NIRRT_NN_BF16 = 1, NIRRT_NN_F16 = 2 };
 enum { NIRRT_NN_ACT_NONE = 0, NIRRT_NN_ACT_RELU = 1, NIRRT_NN_ACT_GELU = 2, NIRRT_NN_ACT_SILU = 3 };
 
 /* y = act(x w^T + b) + r: x (m, k), w (n, k), b (n,) or NULL, r (m, n) or NULL, y (m, n).  z (m, n) contiguous or NULL receives the
- * pre-activation x w^T + b for nirrt_nn_linear_backward.  workspace may be NULL if its size is 0. */
-int64_t nirrt_nn_linear_workspace(int dtype, int64_t m, int64_t n, int64_t k);
+ * pre-activation x w^T + b for nirrt_nn_linear_backward.  The workspace's size depends on the operands' addresses and strides (whole aligned
+ * 16-byte chunks or not); workspace may be NULL if it is 0. */
+int64_t nirrt_nn_linear_workspace(int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t m, int64_t n, int64_t k);
 int nirrt_nn_linear(int dtype, int act, const void *x, int64_t ldx, const void *w, int64_t ldw, const void *b, const void *r, int64_t ldr,
                     void *y, int64_t ldy, void *z, int64_t m, int64_t n, int64_t k, void *workspace, void *stream);
 
 /* Gradients of nirrt_nn_linear: dz = dy act'(z) (rounded to the element type), dx = dz w, dw = dz^T x, db = column sums of dz.  z as the
  * forward pass left it (NULL for NIRRT_NN_ACT_NONE; the forward's y may stand for z with NIRRT_NN_ACT_RELU and no r); dy (m, n).  dx
  * (m, k), dw (n, k) contiguous, db (n,): each may be NULL (not wanted).  The gradient of r is dy itself. */
-int64_t nirrt_nn_linear_backward_workspace(int dtype, int act, int64_t m, int64_t n, int64_t k);
+int64_t nirrt_nn_linear_backward_workspace(int dtype, int act, const void *x, int64_t ldx, const void *w, int64_t ldw, const void *dy, int64_t lddy,
+                                           int64_t m, int64_t n, int64_t k);
 int nirrt_nn_linear_backward(int dtype, int act, const void *x, int64_t ldx, const void *w, int64_t ldw, const void *z, const void *dy,
                              int64_t lddy, void *dx, void *dw, void *db, int64_t m, int64_t n, int64_t k, void *workspace, void *stream);
 

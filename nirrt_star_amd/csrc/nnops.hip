@@ -48,11 +48,11 @@ __device__ __forceinline__ f32x16 mma(float, u32x4 a, u32x4 b, f32x16 c)
     return c;
 }
 
-// one operand: element (r, k) at p[r * ld + k] (KC) or p[k * ld + r] (RC)
+// one operand: element (r, k) at p[r * ld + k] (KC) or p[k * ld + r] (RC); an RC operand counts as zeros from k = depth on
 template <class T> struct Operand {
     const T *p;
     int64_t ld;
-    int rows;
+    int rows, depth;
 };
 
 // N elements from any address of their type (the hardware takes vector loads off their alignment)
@@ -117,7 +117,7 @@ template <class T, int R, int NT, bool RC> struct Stage {
                     T f[VR];
 #pragma unroll
                     for (int s = 0; s < VR; s++) f[s] = (T)0.f;
-                    if (k + j < k1 && row < o.rows) {
+                    if (k + j < k1 && k + j < o.depth && row < o.rows) {
                         if (row + VR <= o.rows) __builtin_memcpy(f, q, VR * sizeof(T));
                         else {
 #pragma unroll
@@ -249,7 +249,7 @@ template <class T, int R, int NT, bool RC> struct DirectOperand {
         } else {
             base = (const char *)(o.p + (int64_t)k0 * o.ld + r0);
             // (whole 4-byte words count as in or out of range: the last one belongs to the row even if only half of it does)
-            bytes = ((int64_t)(k1 - k0 - 1) * row_bytes + (int64_t)(o.rows - r0) * sizeof(T) + 3) & ~3ll;
+            bytes = ((int64_t)((k1 < o.depth ? k1 : o.depth) - k0 - 1) * row_bytes + (int64_t)(o.rows - r0) * sizeof(T) + 3) & ~3ll;
             advance = STEP * row_bytes;
         }
 #pragma unroll
@@ -602,6 +602,78 @@ __global__ __launch_bounds__(Tl::NT) void k_gemm(Operand<T> a, Operand<T> b, int
         __builtin_amdgcn_wave_barrier();
     }
 }
+// ---- few rows (m <= 32): every weight is read for a handful of rows, so what bounds the product is reading w ---------------------------------
+// A workgroup of eight waves owns 16 columns; each wave takes every eighth step of 64 bytes per row of w, eight steps in flight (8 KB per
+// wave: some 64 KB per CU cover the latency), multiplies them on 16 x 16 MFMA with the rows of x straight from memory, and the waves' sums
+// meet in the LDS.  One launch, nothing cut, no workspace.
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4_t mma16(bf16_t, u32x4 a, u32x4 b, f32x4_t c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4_t mma16(f16_t, u32x4 a, u32x4 b, f32x4_t c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4_t mma16(float, u32x4 a, u32x4 b, f32x4_t c)
+{
+#pragma unroll
+    for (int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
+    return c;
+}
+template <class T> __device__ __forceinline__ u32x4 chunk_of(const T *row, int at, int k)
+{
+    constexpr int P = 16 / sizeof(T);
+    Pack<T, P> v = {};
+    if (at < k) v = load_some<T, P>(row + at, k - at);
+    return __builtin_bit_cast(u32x4, v);
+}
+template <class T, int MT, class Epi>
+__global__ __launch_bounds__(512) void k_few_rows(const T *x, int64_t ldx, const T *w, int64_t ldw, int m, int n, int k, Epi epi)
+{
+    constexpr int P = 16 / sizeof(T), STEP = 4 * P, DEPTH = 8, ROUND = 8 * STEP;     // elements: a wave's step, all waves' steps
+    __shared__ f32x4_t meet[8][MT][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, c = wave * STEP + (lane >> 4) * P, j0 = blockIdx.x * 16;
+    // (rows behind the last are the last once more: their results go nowhere)
+    const T *wr = w + (int64_t)(j0 + r < n ? j0 + r : n - 1) * ldw + c, *xr[MT];
+#pragma unroll
+    for (int t = 0; t < MT; t++) xr[t] = x + (int64_t)(16 * t + r < m ? 16 * t + r : m - 1) * ldx + c;
+    f32x4_t acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; t++) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    int k0 = 0;
+    for (; k0 + DEPTH * ROUND <= k; k0 += DEPTH * ROUND) {       // whole steps of all waves: nothing to check
+        u32x4 a[MT][DEPTH], b[DEPTH];
+#pragma unroll
+        for (int d = 0; d < DEPTH; d++) b[d] = __builtin_bit_cast(u32x4, load_pack<T, P>(wr + k0 + d * ROUND));
+#pragma unroll
+        for (int t = 0; t < MT; t++)
+#pragma unroll
+            for (int d = 0; d < DEPTH; d++) a[t][d] = __builtin_bit_cast(u32x4, load_pack<T, P>(xr[t] + k0 + d * ROUND));
+#pragma unroll
+        for (int d = 0; d < DEPTH; d++)
+#pragma unroll
+            for (int t = 0; t < MT; t++) acc[t] = mma16((T)0.f, a[t][d], b[d], acc[t]);
+    }
+    for (; k0 < k; k0 += ROUND) {
+        const u32x4 b = chunk_of(wr, k0, k - c);
+#pragma unroll
+        for (int t = 0; t < MT; t++) acc[t] = mma16((T)0.f, chunk_of(xr[t], k0, k - c), b, acc[t]);
+    }
+#pragma unroll
+    for (int t = 0; t < MT; t++) meet[wave][t][lane] = acc[t];
+    __syncthreads();
+    // element (row, column) of a 16 x 16 block: register row % 4 of lane 16 (row / 4) + column
+    if (threadIdx.x < 64 * MT) {
+        const int t = threadIdx.x >> 6, row = (threadIdx.x & 63) >> 2, cc = (threadIdx.x & 3) * 4, i = 16 * t + row, j = j0 + cc;
+        f32x4 v[1] = {{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int p = 0; p < 8; p++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[0][e] += meet[p][t][16 * (row >> 2) + cc + e][row & 3];
+        if (i < m && j < n) epi.put(v, i, 0, 1, j, n - j < 4 ? n - j : 4);
+    }
+}
 // the parts of a cut reduction, added in their order
 template <class Epi> __global__ __launch_bounds__(256) void k_join(const float *partial, int parts, int m, int n, Epi epi)
 {
@@ -620,7 +692,7 @@ template <class Epi> __global__ __launch_bounds__(256) void k_join(const float *
 // grid (column blocks, row chunks).  A row's 16-byte packs lie on `lanes` (a power of two) neighbouring lanes, 256 / lanes rows at a time;
 // a lane keeps the sums of its columns over the chunk, the rows' lanes meet in the LDS: sums (chunk, column), joined by k_column_join.
 template <class T>
-__global__ __launch_bounds__(256) void k_dz(const T *z, const T *dy, int64_t lddy, T *dz, float *sums, int m, int n, int chunk, int lanes, int act)
+__global__ __launch_bounds__(256) void k_dz(const T *z, const T *dy, int64_t lddy, T *dz, int64_t lddz, float *sums, int m, int n, int chunk, int lanes, int act)
 {
     constexpr int V = 16 / sizeof(T);
     __shared__ float meet[256 * V];
@@ -641,11 +713,11 @@ __global__ __launch_bounds__(256) void k_dz(const T *z, const T *dy, int64_t ldd
                     s[e] += v;
                     d.e[e] = (T)v;
                 }
-                if (dz) store_some(dz + (int64_t)i * n + j, d, cnt);
             } else {
 #pragma unroll
                 for (int e = 0; e < V; e++) s[e] += (float)d.e[e];
             }
+            if (dz) store_pack(dz + (int64_t)i * lddz + j, d);               // (rows of whole packs, zeros behind column n)
         }
     if (!sums) return;
 #pragma unroll
@@ -671,6 +743,22 @@ template <class T> __global__ __launch_bounds__(256) void k_column_join(const fl
     __syncthreads();
     if (threadIdx.x < 64 && j < n)
         out[j] = (T)(((meet[0][threadIdx.x] + meet[1][threadIdx.x]) + (meet[2][threadIdx.x] + meet[3][threadIdx.x])) * (scale ? *scale * factor : factor));
+}
+
+// x with the rows that do not count set to zero (whatever they hold: 0 x NaN must not reach dw), padded with zeros to ld columns and
+// rows_out rows, so that whole aligned chunks can be read; one pass over x, a small part of the products behind it
+template <class T>
+__global__ __launch_bounds__(256) void k_rows_copy(const T *x, int64_t ldx, const float *coef, T *out, int64_t ld, int rows, int rows_out, int k)
+{
+    constexpr int V = 16 / sizeof(T);
+    const int64_t per = ld / V, all = rows_out * per;
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < all; at += (int64_t)gridDim.x * 256) {
+        const int64_t r = at / per;
+        const int c = (int)(at - r * per) * V;
+        Pack<T, V> v = {};
+        if (r < rows && (!coef || coef[r] != 0.f)) v = load_some<T, V>(x + r * ldx + c, k - c);
+        store_pack(out + r * ld + c, v);
+    }
 }
 
 // ---- cross entropy -----------------------------------------------------------------------------------------------------------------
@@ -861,21 +949,6 @@ __global__ __launch_bounds__(256) void k_ce_scale(const float *tops, int blocks,
         const bool usable = top > 1e-30f && top < __builtin_inff();
         scale[0] = usable ? top : 1.f;
         scale[1] = usable ? 1.f / top : 1.f;
-    }
-}
-// x with the rows that do not count set to zero (whatever they hold: 0 x NaN must not reach dw), padded with zeros to ld columns and
-// rows_out rows, so that whole aligned chunks can be read; one pass over x, a small part of the products behind it
-template <class T>
-__global__ __launch_bounds__(256) void k_ce_rows_copy(const T *x, int64_t ldx, const float *coef, T *out, int64_t ld, int rows, int rows_out, int k)
-{
-    constexpr int V = 16 / sizeof(T);
-    const int64_t per = ld / V, all = rows_out * per;
-    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < all; at += (int64_t)gridDim.x * 256) {
-        const int64_t r = at / per;
-        const int c = (int)(at - r * per) * V;
-        Pack<T, V> v = {};
-        if (r < rows && (!coef || coef[r] != 0.f)) v = load_some<T, V>(x + r * ldx + c, k - c);
-        store_pack(out + r * ld + c, v);
     }
 }
 // g' = c_r / scale (exp(l - lse_r) - [v = target]) FACTOR in the element type, stored (v, r): the product C[v, r] again.  16-bit products
@@ -1127,24 +1200,24 @@ __device__ __forceinline__ int tensor_of(const TensorTable &t, int block, int64_
     n = block + 1 == t.first[lo + 1] ? t.last[lo] + 1 : BLOCK_ELEMS;
     return lo;
 }
-// f(eight elements as fp32, how many of them exist, index) over the range, packs of eight neighbouring elements per thread
-template <class T, class F> __device__ __forceinline__ void for_packs(const T *p, int n, F f)
+// f(P elements as fp32, how many of them exist, index) over the range, neighbouring packs on neighbouring lanes
+template <int P, class T, class F> __device__ __forceinline__ void for_packs(const T *p, int n, F f)
 {
-#pragma unroll 4
-    for (int i = threadIdx.x * 8; i < n; i += 256 * 8) {
-        float v[8];
-        const int cnt = n - i < 8 ? n - i : 8;
-        const Pack<T, 8> q = load_some<T, 8>(p + i, cnt);
+#pragma unroll 8
+    for (int i = threadIdx.x * P; i < n; i += 256 * P) {
+        float v[P];
+        const int cnt = n - i < P ? n - i : P;
+        const Pack<T, P> q = load_some<T, P>(p + i, cnt);
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = (float)q.e[e];
+        for (int e = 0; e < P; e++) v[e] = (float)q.e[e];
         f(v, cnt, i);
     }
 }
-template <class F> __device__ __forceinline__ void for_packs_of(const void *p, int dtype, int64_t i0, int n, F f)
+template <int P, class F> __device__ __forceinline__ void for_packs_of(const void *p, int dtype, int64_t i0, int n, F f)
 {
-    if (dtype == NIRRT_NN_F32) for_packs((const float *)p + i0, n, f);
-    else if (dtype == NIRRT_NN_BF16) for_packs((const bf16_t *)p + i0, n, f);
-    else for_packs((const f16_t *)p + i0, n, f);
+    if (dtype == NIRRT_NN_F32) for_packs<4>((const float *)p + i0, n, f);
+    else if (dtype == NIRRT_NN_BF16) for_packs<P>((const bf16_t *)p + i0, n, f);
+    else for_packs<P>((const f16_t *)p + i0, n, f);
 }
 // squares are summed in double: no overflow below the largest element squared, and the order does not matter to the last bits of the norm
 __global__ __launch_bounds__(256) void k_norm_parts(TensorTable t, double *parts)
@@ -1154,10 +1227,11 @@ __global__ __launch_bounds__(256) void k_norm_parts(TensorTable t, double *parts
     int n;
     const int e = tensor_of(t, blockIdx.x, i0, n);
     double s = 0.;
-    for_packs_of(t.in[e], t.types[e] & 15, i0, n, [&](const float *v, int, int) {
+    for_packs_of<8>(t.in[e], t.types[e] & 15, i0, n, [&](const auto &v, int, int) {
+        constexpr int P = sizeof(v) / sizeof(float);
         double a = 0.;
 #pragma unroll
-        for (int q = 0; q < 8; q++) a = __builtin_fma((double)v[q], (double)v[q], a);
+        for (int q = 0; q < P; q++) a = __builtin_fma((double)v[q], (double)v[q], a);
         s += a;
     });
 #pragma unroll
@@ -1183,11 +1257,11 @@ __global__ __launch_bounds__(1024) void k_norm_total(const double *parts, int64_
         *norm = (float)sqrt(s);
     }
 }
-template <class T> __device__ __forceinline__ void put_pack(T *o, const float *v, float f, int cnt)
+template <class T, int P> __device__ __forceinline__ void put_pack(T *o, const float (&v)[P], float f, int cnt)
 {
-    Pack<T, 8> q;
+    Pack<T, P> q;
 #pragma unroll
-    for (int e = 0; e < 8; e++) q.e[e] = (T)(v[e] * f);
+    for (int e = 0; e < P; e++) q.e[e] = (T)(v[e] * f);
     store_some(o, q, cnt);
 }
 __global__ __launch_bounds__(256) void k_scale(TensorTable t, const float *norm, float max_norm)
@@ -1197,8 +1271,9 @@ __global__ __launch_bounds__(256) void k_scale(TensorTable t, const float *norm,
     const int e = tensor_of(t, blockIdx.x, i0, n), to = t.types[e] >> 4;
     const float q = max_norm / (*norm + 1e-6f), f = q < 1.f ? q : (q == q ? 1.f : q);
     if (f == 1.f && t.in[e] == t.out[e]) return;
+    // (four elements per lane: both sides of a 16-bit -> 32-bit scaling are whole lines per instruction)
     void *out = t.out[e];
-    for_packs_of(t.in[e], t.types[e] & 15, i0, n, [&](const float *v, int cnt, int i) {
+    for_packs_of<4>(t.in[e], t.types[e] & 15, i0, n, [&](const auto &v, int cnt, int i) {
         if (to == NIRRT_NN_F32) put_pack((float *)out + i0 + i, v, f, cnt);
         else if (to == NIRRT_NN_BF16) put_pack((bf16_t *)out + i0 + i, v, f, cnt);
         else put_pack((f16_t *)out + i0 + i, v, f, cnt);
@@ -1213,28 +1288,55 @@ int status() { return hipGetLastError() == hipSuccess ? 0 : -2; }
 int elem_size(int dtype) { return dtype == NIRRT_NN_F32 ? 4 : 2; }
 bool good_type(int dtype) { return dtype == NIRRT_NN_F32 || dtype == NIRRT_NN_BF16 || dtype == NIRRT_NN_F16; }
 
-template <class T> Operand<T> op(const T *p, int64_t ld, int64_t rows) { return {p, ld, (int)rows}; }
+template <class T> Operand<T> op(const T *p, int64_t ld, int64_t rows, int64_t depth = DIM_MAX) { return {p, ld, (int)rows, (int)depth}; }
 
-// Tile edge and parts of the reduction.  A GPU of 256 CUs wants a workgroup of eight waves per CU (256 x 256 tiles) or two of four waves
-// (128 x 128): the largest tile that still gives every CU one; 64 x 64 where there are fewer, and where even these are few and the
-// reduction is long, it is cut (at least four steps per part, at most 32 parts).  256 x 256 needs operands of whole aligned chunks.
-struct Plan { int edge, parts, part; };
-Plan plan(int dtype, int64_t m, int64_t n, int64_t k)
+// Tile edge and parts of the reduction, by the time they are expected to take.  A step is 64 bytes of k; a CU with q tiles of a kind to do takes
+// max(lat ceil(q / fit), q work) us per step (fit: tiles resident at once), 0.3 ns per element for the epilogue, and parts are joined at 4 bytes
+// per element, part and way.  Measured on one box, us per step, 256 CUs with 1 / 2 / 4 tiles each (x w^T): 16-bit 256: 0.94 2.0 4.4, 128: 0.39
+// 0.67 1.33, 64: 0.28 0.33 0.62; 32-bit 256: 4.2, 128: 1.07, 64: 0.31 per tile.  slow = 1 + the number of RC operands: operands that are no whole
+// aligned chunks take the register-staged tile (4097 x 321 x 515 in bf16, edge 64: 14 us with none, 22 with one, 37 with two); 0: they are.
+struct Plan { int edge, parts, part; double us; };
+struct TileCost { int edge, fit; double lat, work; };
+Plan plan(int dtype, int64_t m, int64_t n, int64_t k, int slow = 0, int64_t most_parts = 32)
 {
-    Plan p;
-    const int64_t step = ROW_BYTES / elem_size(dtype), steps = ceil_div(k, step);
-    p.edge = ceil_div(m, 256) * ceil_div(n, 256) >= 224 ? 256 : ceil_div(m, 128) * ceil_div(n, 128) >= 256 ? 128 : 64;
-    const int64_t tiles = ceil_div(m, p.edge) * ceil_div(n, p.edge);      // (0 for an empty result)
-    int64_t parts = p.edge == 256 || tiles >= 256 || tiles == 0 ? 1 : 512 / tiles;
-    if (parts > steps / 4) parts = steps / 4;
-    if (parts > 32) parts = 32;
-    if (parts < 1) parts = 1;
-    const int64_t per = ceil_div(steps, parts);
-    p.part = (int)(per * step < DIM_MAX ? (per > 0 ? per * step : step) : DIM_MAX);
-    p.parts = (int)(steps > 0 ? ceil_div(steps, per) : 1);
-    return p;
+    static const TileCost fast16[] = {{256, 1, 0.94, 1.03}, {128, 2, 0.38, 0.33}, {64, 5, 0.28, 0.155}};
+    static const TileCost fast32[] = {{256, 1, 3.7, 4.2}, {128, 2, 1.05, 1.07}, {64, 5, 0.36, 0.31}};
+    static const TileCost slow16[] = {{128, 3, 1.0, 0.6}, {64, 6, 0.5, 0.25}};
+    static const TileCost slow32[] = {{128, 3, 1.5, 1.25}, {64, 6, 0.6, 0.36}};
+    const bool f32 = dtype == NIRRT_NN_F32;
+    const TileCost *cost = slow ? (f32 ? slow32 : slow16) : (f32 ? fast32 : fast16);
+    const double rc = slow <= 1 ? 1. : f32 ? (slow == 2 ? 1.2 : 1.5) : (slow == 2 ? 1.7 : 3.);
+    const int64_t step = 64 / elem_size(dtype), steps = ceil_div(k, step);
+    Plan best = {64, 1, (int)(steps > 0 ? steps * step : step), 0.};
+    if (m <= 0 || n <= 0 || k <= 0) return best;
+    best.us = 1e30;
+    for (int c = slow ? 1 : 2; c >= 0; c--) {
+        const double tiles = (double)ceil_div(m, cost[c].edge) * (double)ceil_div(n, cost[c].edge), elems = (double)cost[c].edge * cost[c].edge;
+        for (int64_t parts = 1; parts <= most_parts && parts * 8 <= steps + 7; parts++) {
+            const int64_t per = ceil_div(steps, parts);
+            if (parts > 1 && ceil_div(steps, per) != parts) continue;
+            const double q = ceil(tiles * parts / 256.), waves = ceil(q / cost[c].fit);
+            const double run = (cost[c].lat * waves > q * cost[c].work ? cost[c].lat * waves : q * cost[c].work) * rc * per;
+            const double us = run + 2. * waves + q * elems * 3e-4 + (parts > 1 ? 5. + (double)m * n * 4. * (2 * parts + 1) / 4e6 : 0.);
+            if (us < best.us) best = {cost[c].edge, (int)parts, (int)(per * step), us};
+        }
+    }
+    return best;
 }
 int64_t plan_bytes(const Plan &p, int64_t m, int64_t n) { return p.parts > 1 ? round256(4 * m * n * p.parts) : 0; }
+// the time that copying rows into whole chunks takes: 3 TB/s and a launch
+double copy_us(int dtype, int64_t rows, int64_t k) { return 4. + (double)rows * k * 2 * elem_size(dtype) / 3e6; }
+int64_t padded(int dtype, int64_t k) { const int64_t c = 16 / elem_size(dtype); return (k + c - 1) / c * c; }
+bool whole_rows(int dtype, const void *p, int64_t ld, int64_t k) { return (uintptr_t)p % 16 == 0 && ld * elem_size(dtype) % 16 == 0 && k == padded(dtype, k); }
+bool aligned_rows(int dtype, const void *p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld * elem_size(dtype) % 16 == 0; }
+template <class T>
+void copy_rows(const void *x, int64_t ldx, const float *coef, T *out, int64_t ld, int64_t rows, int64_t rows_out, int64_t k, hipStream_t st)
+{
+    const int64_t blocks = ceil_div(rows_out * (ld * (int64_t)sizeof(T) / 16), 256);
+    if (blocks > 0)
+        hipLaunchKernelGGL((k_rows_copy<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, (const T *)x, ldx, coef, out, ld,
+                           (int)rows, (int)rows_out, (int)k);
+}
 
 // whole aligned chunks (see DirectOperand): rows and base on 16 bytes, for KC a reduction of whole chunks, offsets inside a step below 2^31
 template <class T, bool RC> bool direct(const Operand<T> &o, int64_t k)
@@ -1248,7 +1350,7 @@ template <class T, bool RCA, bool RCB, class Epi>
 int gemm(const Operand<T> &a, const Operand<T> &b, int64_t m, int64_t n, int64_t k, const Plan &p, float *partial, const Epi &epi, hipStream_t st)
 {
     const bool fast = direct<T, RCA>(a, k) && direct<T, RCB>(b, k);
-    const int edge = fast || p.edge < 256 ? p.edge : 128;
+    const int edge = fast || p.edge < 256 ? p.edge : 128;   // (a plan for whole chunks, and operands beyond direct()'s row length)
     const int64_t tiles = ceil_div(m, edge) * ceil_div(n, edge);
     if (tiles > DIM_MAX) return -1;
     const dim3 grid((unsigned)tiles, (unsigned)p.parts);
@@ -1287,54 +1389,112 @@ Columns columns(int dtype, int64_t m, int64_t n)
     return c;
 }
 
-struct LinearBackward { Plan px, pw; int64_t dz, sums, part, total; };
-LinearBackward linear_backward_layout(int dtype, int act, int64_t m, int64_t n, int64_t k)
+// x w^T: few rows go to k_few_rows; operands that are no whole aligned chunks are copied into such where that is expected to pay
+struct Linear { bool few, copy_x, copy_w; Plan p; int64_t kp, xs, ws, part, total; };
+Linear linear_layout(int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t m, int64_t n, int64_t k)
 {
-    LinearBackward l;
-    l.px = plan(dtype, m, k, n);
-    l.pw = plan(dtype, n, k, m);
-    l.dz = act == NIRRT_NN_ACT_NONE ? 0 : round256(m * n * elem_size(dtype));
-    l.sums = round256(4 * n * columns(dtype, m, n).parts);
-    const int64_t bx = plan_bytes(l.px, m, k), bw = plan_bytes(l.pw, n, k);
-    l.part = bx > bw ? bx : bw;
-    l.total = l.dz + l.sums + l.part;
+    Linear l = {};
+    l.few = m <= 32;
+    l.kp = k;
+    if (l.few) return l;
+    l.copy_x = !whole_rows(dtype, x, ldx, k);
+    l.copy_w = !whole_rows(dtype, w, ldw, k);
+    if (l.copy_x || l.copy_w) {
+        const Plan slow = plan(dtype, m, n, k, 1), fast = plan(dtype, m, n, padded(dtype, k));
+        if (fast.us + (l.copy_x ? copy_us(dtype, m, k) : 0.) + (l.copy_w ? copy_us(dtype, n, k) : 0.) >= slow.us) {
+            l.copy_x = l.copy_w = false;
+            l.p = slow;
+        } else {
+            l.p = fast;
+            l.kp = padded(dtype, k);
+        }
+    } else l.p = plan(dtype, m, n, k);
+    l.xs = l.copy_x ? round256(m * l.kp * elem_size(dtype)) : 0;
+    l.ws = l.copy_w ? round256(n * l.kp * elem_size(dtype)) : 0;
+    l.part = plan_bytes(l.p, m, n);
+    l.total = l.xs + l.ws + l.part;
     return l;
 }
-
 template <class T>
 int linear_t(int dtype, int act, const void *x, int64_t ldx, const void *w, int64_t ldw, const void *b, const void *r, int64_t ldr, void *y,
-             int64_t ldy, void *z, int64_t m, int64_t n, int64_t k, void *ws, hipStream_t st)
+             int64_t ldy, void *z, int64_t m, int64_t n, int64_t k, char *ws, hipStream_t st)
 {
+    const Linear l = linear_layout(dtype, x, ldx, w, ldw, m, n, k);
     const EpiLinear<T> epi = {(const T *)b, (const T *)r, (T *)y, (T *)z, ldr, ldy, act, (int)n};
-    return gemm<T, false, false>(op((const T *)x, ldx, m), op((const T *)w, ldw, n), m, n, k, plan(dtype, m, n, k), (float *)ws, epi, st);
+    if (l.few) {
+        const dim3 grid((unsigned)ceil_div(n, 16));
+        if (m <= 16) hipLaunchKernelGGL((k_few_rows<T, 1, EpiLinear<T>>), grid, dim3(512), 0, st, (const T *)x, ldx, (const T *)w, ldw, (int)m, (int)n, (int)k, epi);
+        else hipLaunchKernelGGL((k_few_rows<T, 2, EpiLinear<T>>), grid, dim3(512), 0, st, (const T *)x, ldx, (const T *)w, ldw, (int)m, (int)n, (int)k, epi);
+        return status();
+    }
+    T *xs = (T *)ws, *wsp = (T *)(ws + l.xs);
+    if (l.copy_x) { copy_rows(x, ldx, nullptr, xs, l.kp, m, m, k, st); x = xs; ldx = l.kp; }
+    if (l.copy_w) { copy_rows(w, ldw, nullptr, wsp, l.kp, n, n, k, st); w = wsp; ldw = l.kp; }
+    return gemm<T, false, false>(op((const T *)x, ldx, m), op((const T *)w, ldw, n), m, n, l.kp, l.p, (float *)(ws + l.xs + l.ws), epi, st);
 }
 
+// dx = dz w (m, k; reduction n), dw = dz^T x (n, k; reduction m).  dz is written in rows of whole chunks (also for ACT_NONE where dy's are not); w
+// and x are copied into such where that is expected to pay.
+struct LinearBackward { bool own_dz, copy_x, copy_w; Plan px, pw; int64_t np, kp, dz, xs, ws, sums, part, total; };
+LinearBackward linear_backward_layout(int dtype, int act, const void *x, int64_t ldx, const void *w, int64_t ldw, const void *dy, int64_t lddy, int64_t m,
+                                      int64_t n, int64_t k, bool dx, bool dw)
+{
+    LinearBackward l = {};
+    const int e = elem_size(dtype);
+    l.np = padded(dtype, n);
+    l.kp = padded(dtype, k);
+    l.px = plan(dtype, m, k, l.np);
+    l.pw = plan(dtype, n, k, m);
+    l.copy_w = dx && !aligned_rows(dtype, w, ldw);
+    l.copy_x = dw && !aligned_rows(dtype, x, ldx);
+    const double relay_dy = act == NIRRT_NN_ACT_NONE && (dx || dw) && !whole_rows(dtype, dy, lddy, n) ? copy_us(dtype, m, n) : 0.;
+    const Plan sx = plan(dtype, m, k, n, 2), sw_ = plan(dtype, n, k, m, 3);
+    const bool slow_x = dx && (l.copy_w || relay_dy > 0.) && l.px.us + (l.copy_w ? copy_us(dtype, n, k) : 0.) + relay_dy / 2 >= sx.us;
+    const bool slow_w = dw && (l.copy_x || relay_dy > 0.) && l.pw.us + (l.copy_x ? copy_us(dtype, m, k) : 0.) + relay_dy / 2 >= sw_.us;
+    if (slow_x) { l.px = sx; l.copy_w = false; }
+    if (slow_w) { l.pw = sw_; l.copy_x = false; }
+    l.own_dz = act != NIRRT_NN_ACT_NONE || (relay_dy > 0. && ((dx && !slow_x) || (dw && !slow_w)));
+    l.dz = l.own_dz && (dx || dw) ? round256(m * l.np * e) : 0;
+    l.xs = l.copy_x ? round256(m * l.kp * e) : 0;
+    l.ws = l.copy_w ? round256(n * l.kp * e) : 0;
+    l.sums = round256(4 * n * columns(dtype, m, n).parts);
+    const int64_t bx = dx ? plan_bytes(l.px, m, k) : 0, bw = dw ? plan_bytes(l.pw, n, k) : 0;
+    l.part = bx > bw ? bx : bw;
+    l.total = l.dz + l.xs + l.ws + l.sums + l.part;
+    return l;
+}
 template <class T>
 int linear_backward_t(int dtype, int act, const void *x, int64_t ldx, const void *w, int64_t ldw, const void *z, const void *dy, int64_t lddy,
                       void *dx, void *dw, void *db, int64_t m, int64_t n, int64_t k, char *ws, hipStream_t st)
 {
-    const LinearBackward l = linear_backward_layout(dtype, act, m, n, k);
-    T *dz = (T *)ws;
-    float *sums = (float *)(ws + l.dz), *part = (float *)(ws + l.dz + l.sums);
-    const bool own_dz = act != NIRRT_NN_ACT_NONE;
-    if (own_dz || db) {
+    const LinearBackward l = linear_backward_layout(dtype, act, x, ldx, w, ldw, dy, lddy, m, n, k, dx != nullptr, dw != nullptr);
+    T *dz = (T *)ws, *xs = (T *)(ws + l.dz), *wsp = (T *)((char *)xs + l.xs);
+    float *sums = (float *)((char *)wsp + l.ws), *part = (float *)((char *)sums + l.sums);
+    if (l.own_dz || db) {
         const Columns c = columns(dtype, m, n);
         if (m > 0)
             hipLaunchKernelGGL((k_dz<T>), dim3((unsigned)c.blocks, (unsigned)c.parts), dim3(256), 0, st, (const T *)z, (const T *)dy, lddy,
-                               own_dz && (dx || dw) ? dz : (T *)nullptr, db ? sums : nullptr, (int)m, (int)n, c.chunk, c.lanes, act);
+                               l.dz ? dz : (T *)nullptr, l.np, db ? sums : nullptr, (int)m, (int)n, c.chunk, c.lanes, act);
         if (db)
             hipLaunchKernelGGL((k_column_join<T>), dim3((unsigned)ceil_div(n, 64)), dim3(256), 0, st, sums, c.parts, (const float *)nullptr, 1.f, (T *)db, n);
         if (int rc_ = status()) return rc_;
     }
-    const T *d = own_dz ? dz : (const T *)dy;
-    const int64_t ldd = own_dz ? n : lddy;
+    const T *d = l.dz ? dz : (const T *)dy;
+    const int64_t ldd = l.dz ? l.np : lddy;
     if (dx && m > 0 && k > 0) {
         const EpiPlain<T> epi = {(T *)dx, nullptr, 1.f, (int)k};
-        if (int rc_ = gemm<T, false, true>(op(d, ldd, m), op((const T *)w, ldw, k), m, k, n, l.px, part, epi, st)) return rc_;
+        const T *wp = (const T *)w;
+        int64_t ld = ldw;
+        if (l.copy_w) { copy_rows(w, ldw, nullptr, wsp, l.kp, n, n, k, st); wp = wsp; ld = l.kp; }
+        // (own dz: a reduction of whole chunks, zeros behind n)
+        if (int rc_ = gemm<T, false, true>(op(d, ldd, m), op(wp, ld, k, n), m, k, l.dz ? l.np : n, l.px, part, epi, st)) return rc_;
     }
     if (dw && n > 0 && k > 0) {
         const EpiPlain<T> epi = {(T *)dw, nullptr, 1.f, (int)k};
-        if (int rc_ = gemm<T, true, true>(op(d, ldd, n), op((const T *)x, ldx, k), n, k, m, l.pw, part, epi, st)) return rc_;
+        const T *xp = (const T *)x;
+        int64_t ld = ldx;
+        if (l.copy_x) { copy_rows(x, ldx, nullptr, xs, l.kp, m, m, k, st); xp = xs; ld = l.kp; }
+        if (int rc_ = gemm<T, true, true>(op(d, ldd, n), op(xp, ld, k), n, k, m, l.pw, part, epi, st)) return rc_;
     }
     return 0;
 }
@@ -1368,17 +1528,7 @@ bool few_layout(int dtype, int64_t rows, int64_t classes, int64_t k, Few &f)
 #define FEW_ONE(KERNEL, V, NC, LDS, ...) hipLaunchKernelGGL((KERNEL<T, V, NC>), dim3((unsigned)f.blocks), dim3(256), LDS, st, __VA_ARGS__)
 
 // cross entropy: tile edge, and parts of the classes so that row tiles x parts fill the GPU; x and w whose rows are no whole aligned chunks
-// are copied into such (k_ce_rows_copy): the products read them many times
-int64_t padded(int dtype, int64_t k) { const int64_t c = 16 / elem_size(dtype); return (k + c - 1) / c * c; }
-bool whole_rows(int dtype, const void *p, int64_t ld, int64_t k) { return (uintptr_t)p % 16 == 0 && ld * elem_size(dtype) % 16 == 0 && k == padded(dtype, k); }
-template <class T>
-void copy_rows(const void *x, int64_t ldx, const float *coef, T *out, int64_t ld, int64_t rows, int64_t rows_out, int64_t k, hipStream_t st)
-{
-    const int64_t blocks = ceil_div(rows_out * (ld * (int64_t)sizeof(T) / 16), 256);
-    if (blocks > 0)
-        hipLaunchKernelGGL((k_ce_rows_copy<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, (const T *)x, ldx, coef, out, ld,
-                           (int)rows, (int)rows_out, (int)k);
-}
+// are copied into such (k_rows_copy): the products read them many times
 struct CeForward { int edge, parts, part; int64_t stats, score, sums, xs, ws, total; };
 CeForward ce_layout(int dtype, int64_t rows, int64_t classes, int64_t k)
 {
@@ -1452,9 +1602,7 @@ CeBackward ce_backward_layout(int dtype, int64_t rows, int64_t classes, int64_t 
     l.piece = l.ldg > 0 ? G_ELEMS / l.ldg / 256 * 256 : classes;
     if (l.piece < 256) l.piece = 256;
     if (l.piece > classes) l.piece = classes;
-    l.pg = plan(dtype, l.piece, l.ldg, k);
-    l.pg.parts = 1;                    // (the scores are not cut: the softmax needs whole ones)
-    l.pg.part = (int)(padded(dtype, k) > 0 ? padded(dtype, k) : 1);
+    l.pg = plan(dtype, l.piece, l.ldg, padded(dtype, k), 0, 1);     // (the scores are not cut: the softmax needs whole ones)
     l.px = plan(dtype, rows, k, l.piece);
     l.pw = plan(dtype, l.piece, k, l.ldg);
     l.coef = round256(4 * rows) + 256;
@@ -1567,37 +1715,48 @@ template <class F> int64_t for_tables(const nirrt_nn_tensor *t, int32_t count, F
 
 }   // namespace
 
-extern "C" int64_t nirrt_nn_linear_workspace(int dtype, int64_t m, int64_t n, int64_t k)
+static bool good_linear(int dtype, int act, int64_t ldx, int64_t ldw, int64_t m, int64_t n, int64_t k)
 {
-    if (!good_type(dtype) || !good_dims(m, n, k)) return -1;
-    return plan_bytes(plan(dtype, m, n, k), m, n);
+    return good_type(dtype) && act >= 0 && act <= NIRRT_NN_ACT_SILU && good_dims(m, n, k) && ldx >= k && ldw >= k;
+}
+
+extern "C" int64_t nirrt_nn_linear_workspace(int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t m, int64_t n, int64_t k)
+{
+    if (!good_linear(dtype, 0, ldx, ldw, m, n, k)) return -1;
+    return linear_layout(dtype, x, ldx, w, ldw, m, n, k).total;
 }
 
 extern "C" int nirrt_nn_linear(int dtype, int act, const void *x, int64_t ldx, const void *w, int64_t ldw, const void *b, const void *r, int64_t ldr,
                                void *y, int64_t ldy, void *z, int64_t m, int64_t n, int64_t k, void *workspace, void *stream)
 {
-    if (!good_type(dtype) || act < 0 || act > NIRRT_NN_ACT_SILU || !good_dims(m, n, k)) return -1;
+    if (!good_linear(dtype, act, ldx, ldw, m, n, k)) return -1;
     if (m == 0 || n == 0) return 0;
-    if (!y || (k > 0 && (!x || !w)) || ldx < k || ldw < k || ldy < n || (r && ldr < n)) return -1;
-    if (nirrt_nn_linear_workspace(dtype, m, n, k) > 0 && !workspace) return -1;
-#define CALL(T) linear_t<T>(dtype, act, x, ldx, w, ldw, b, r, ldr, y, ldy, z, m, n, k, workspace, (hipStream_t)stream)
+    if (!y || (k > 0 && (!x || !w)) || ldy < n || (r && ldr < n)) return -1;
+    if (!workspace && nirrt_nn_linear_workspace(dtype, x, ldx, w, ldw, m, n, k) > 0) return -1;
+#define CALL(T) linear_t<T>(dtype, act, x, ldx, w, ldw, b, r, ldr, y, ldy, z, m, n, k, (char *)workspace, (hipStream_t)stream)
     return BY_TYPE(dtype, CALL);
 #undef CALL
 }
 
-extern "C" int64_t nirrt_nn_linear_backward_workspace(int dtype, int act, int64_t m, int64_t n, int64_t k)
+extern "C" int64_t nirrt_nn_linear_backward_workspace(int dtype, int act, const void *x, int64_t ldx, const void *w, int64_t ldw, const void *dy,
+                                                      int64_t lddy, int64_t m, int64_t n, int64_t k)
 {
-    if (!good_type(dtype) || act < 0 || act > NIRRT_NN_ACT_SILU || !good_dims(m, n, k)) return -1;
-    return linear_backward_layout(dtype, act, m, n, k).total;
+    if (!good_linear(dtype, act, ldx, ldw, m, n, k) || lddy < n) return -1;
+    int64_t most = 0;                       // of what a call may leave out
+    for (int want = 0; want < 4; want++) {
+        const int64_t t = linear_backward_layout(dtype, act, x, ldx, w, ldw, dy, lddy, m, n, k, want & 1, want & 2).total;
+        most = t > most ? t : most;
+    }
+    return most;
 }
 
 extern "C" int nirrt_nn_linear_backward(int dtype, int act, const void *x, int64_t ldx, const void *w, int64_t ldw, const void *z, const void *dy,
                                         int64_t lddy, void *dx, void *dw, void *db, int64_t m, int64_t n, int64_t k, void *workspace, void *stream)
 {
-    if (!good_type(dtype) || act < 0 || act > NIRRT_NN_ACT_SILU || !good_dims(m, n, k)) return -1;
-    if (m > 0 && n > 0 && (!dy || lddy < n || (act != NIRRT_NN_ACT_NONE && !z))) return -1;
-    if (((dx || dw) && (ldx < k || ldw < k)) || (dx && m > 0 && n > 0 && k > 0 && !w) || (dw && m > 0 && n > 0 && k > 0 && !x)) return -1;
-    if (!workspace && linear_backward_layout(dtype, act, m, n, k).total > 0) return -1;
+    if (!good_linear(dtype, act, ldx, ldw, m, n, k) || lddy < n) return -1;
+    if (m > 0 && n > 0 && (!dy || (act != NIRRT_NN_ACT_NONE && !z))) return -1;
+    if ((dx && m > 0 && n > 0 && k > 0 && !w) || (dw && m > 0 && n > 0 && k > 0 && !x)) return -1;
+    if (!workspace && linear_backward_layout(dtype, act, x, ldx, w, ldw, dy, lddy, m, n, k, dx != nullptr, dw != nullptr).total > 0) return -1;
 #define CALL(T) linear_backward_t<T>(dtype, act, x, ldx, w, ldw, z, dy, lddy, dx, dw, db, m, n, k, (char *)workspace, (hipStream_t)stream)
     return BY_TYPE(dtype, CALL);
 #undef CALL

@@ -21,14 +21,18 @@ ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 _DIM_MAX = 0x7fffffff - 256
 
 
+_library = None
+
+
 def _lib():
-    from . import _hip
-    L = _hip.load()
-    if not hasattr(L, "_nn_ready"):
+    global _library
+    if _library is None:
+        from . import _hip
+        L = _hip.load()
         vp, i, l, f = C.c_void_p, C.c_int, C.c_int64, C.c_float
-        L.nirrt_nn_linear_workspace.argtypes = [i, l, l, l]
+        L.nirrt_nn_linear_workspace.argtypes = [i, vp, l, vp, l, l, l, l]
         L.nirrt_nn_linear.argtypes = [i, i, vp, l, vp, l, vp, vp, l, vp, l, vp, l, l, l, vp, vp]
-        L.nirrt_nn_linear_backward_workspace.argtypes = [i, i, l, l, l]
+        L.nirrt_nn_linear_backward_workspace.argtypes = [i, i, vp, l, vp, l, vp, l, l, l, l]
         L.nirrt_nn_linear_backward.argtypes = [i, i, vp, l, vp, l, vp, vp, l, vp, vp, vp, l, l, l, vp, vp]
         L.nirrt_nn_cross_entropy_workspace.argtypes = [i, l, l, l]
         L.nirrt_nn_cross_entropy.argtypes = [i, vp, l, vp, l, vp, vp, vp, l, vp, vp, vp, l, l, l, vp, vp]
@@ -41,8 +45,8 @@ def _lib():
             getattr(L, "nirrt_nn_%s_workspace" % name).restype = l
             getattr(L, "nirrt_nn_%s" % name).restype = i
         L.nirrt_nn_scale_by_norm.restype = i
-        L._nn_ready = True
-    return L
+        _library = L
+    return _library
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # (the stream object costs 2 us per call)
@@ -82,13 +86,16 @@ def _need(name, first, **others):
 
 def _rows(t):
     """(..., k) -> (rows, k) with unit column stride and rows that do not overlap (a copy if need be), and its row stride"""
-    k = t.shape[-1]
     if t.dim() != 2:
+        k = t.shape[-1]
         t = t.reshape(t.numel() // k if k else _prod(t.shape[:-1]), k)
-    m = t.shape[0]
+    m, k = t.shape
+    ld, one = t.stride()
+    if one == 1 and ld >= k > 0:
+        return t, ld
     if m <= 1 or k == 0:
-        return (t if k <= 1 or t.stride(1) == 1 else t.contiguous()), max(k, 1)
-    if (k > 1 and t.stride(1) != 1) or t.stride(0) < k:
+        return (t if k <= 1 or one == 1 else t.contiguous()), max(k, 1)
+    if k > 1 or ld < k:
         t = t.contiguous()
     return t, t.stride(0)
 
@@ -118,19 +125,21 @@ def _sizes_ok(name, *dims):
 # ---- linear layer ---------------------------------------------------------------------------------------------------------------------
 def _linear_forward(x, w, b, r, act, keep):
     """-> y, z (what the backward pass needs of the pre-activation: None, y itself, or a tensor of its own)"""
-    m, n, k = _prod(x.shape[:-1]), w.shape[0], w.shape[1]
+    n, k = w.shape
     x2, ldx = _rows(x)
     w2, ldw = _rows(w)
-    y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
+    m = x2.shape[0]
+    device, dtype = x.device, x.dtype
+    y = torch.empty((m, n) if x.dim() == 2 else x.shape[:-1] + (n,), dtype=dtype, device=device)
     r2, ldr = _rows(r) if r is not None else (None, n)
     z = None
     if keep and act:
-        z = y if act == 1 and r is None else torch.empty(m, n, dtype=x.dtype, device=x.device)
+        z = y if act == 1 and r is None else torch.empty(m, n, dtype=dtype, device=device)
     if m and n:
-        L, dt = _lib(), _TYPES[x.dtype]
-        ws = _workspace(L.nirrt_nn_linear_workspace(dt, m, n, k), x.device)
-        _check(L.nirrt_nn_linear(dt, act, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b), _ptr(r2), ldr, y.data_ptr(), n,
-                                 None if z is None or z is y else z.data_ptr(), m, n, k, _ptr(ws), _stream(x.device)), "linear")
+        L, dt, px, pw = _lib(), _TYPES[dtype], x2.data_ptr(), w2.data_ptr()
+        ws = _workspace(L.nirrt_nn_linear_workspace(dt, px, ldx, pw, ldw, m, n, k), device)
+        _check(L.nirrt_nn_linear(dt, act, px, ldx, pw, ldw, None if b is None else b.data_ptr(), None if r2 is None else r2.data_ptr(), ldr, y.data_ptr(), n,
+                                 None if z is None or z is y else z.data_ptr(), m, n, k, _ptr(ws), _stream(device)), "linear")
     return y, z
 
 
@@ -163,7 +172,8 @@ class _Linear(torch.autograd.Function):
                 x2, ldx = _rows(x)
                 w2, ldw = _rows(w)
                 L, dt = _lib(), _TYPES[x.dtype]
-                ws = _workspace(L.nirrt_nn_linear_backward_workspace(dt, ctx.act, m, n, k), x.device)
+                ws = _workspace(L.nirrt_nn_linear_backward_workspace(dt, ctx.act, x2.data_ptr(), ldx, w2.data_ptr(), ldw, dy2.data_ptr(), lddy,
+                                                                     m, n, k), x.device)
                 if n:
                     _check(L.nirrt_nn_linear_backward(dt, ctx.act, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(z), dy2.data_ptr(), lddy, _ptr(dx),
                                                       _ptr(dw), _ptr(db), m, n, k, _ptr(ws), _stream(x.device)), "linear_backward")
@@ -265,26 +275,30 @@ _TENSOR = np.dtype([("data", "<u8"), ("out", "<u8"), ("n", "<i8"), ("dtype", "<i
 
 
 def _tensor_list(name, tensors):
+    """-> the tensors that are not None, their device, their element types if they differ (else the one they share)"""
     ts = [t for t in tensors if t is not None]
     if not ts:
         raise ValueError("%s: no tensors" % name)
-    # (sets of small values instead of one comparison per tensor: hundreds of tensors are a case where the host's time counts)
+    # (one pass per property into a set: with hundreds of small tensors the host's time is what counts)
     where = {t.get_device() for t in ts}
     if where == {-1}:
         raise RuntimeError("nirrt_star_amd.nnops.%s got a CPU tensor: the package only has the HIP kernels (move it to 'cuda')" % name)
-    if len(where) != 1 or {t.layout for t in ts} != {torch.strided} or not {t.dtype for t in ts} <= _TYPES.keys():
+    types = [t.dtype for t in ts]
+    kinds = set(types)
+    if len(where) != 1 or {t.layout for t in ts} != {torch.strided} or not kinds <= _TYPES.keys():
         raise ValueError("%s: dense float32, bfloat16 or float16 tensors of one device" % name)
-    return ts, ts[0].device
+    return ts, ts[0].device, _TYPES[types[0]] if len(kinds) == 1 else [_TYPES[t] for t in types]
 
 
-def _table(ts, outs=None):
+def _dense(ts):
+    return ts if all([t.is_contiguous() for t in ts]) else [t if t.is_contiguous() else t.contiguous() for t in ts]
+
+
+def _table(ts, types):
     tab = np.zeros(len(ts), dtype=_TENSOR)
     tab["data"] = [t.data_ptr() for t in ts]
     tab["n"] = [t.numel() for t in ts]
-    tab["dtype"] = [_TYPES[t.dtype] for t in ts]
-    if outs is not None:
-        tab["out"] = [t.data_ptr() for t in outs]
-        tab["out_dtype"] = [_TYPES[t.dtype] for t in outs]
+    tab["dtype"] = types
     return tab
 
 
@@ -299,15 +313,15 @@ def _norm(tab, dev):
 @torch.no_grad()
 def grad_norm(tensors):
     """2-norm of all elements of the tensors (None entries are skipped), summed in 64 bits in a fixed order -> float32 scalar on their device"""
-    ts, dev = _tensor_list("grad_norm", tensors)
+    ts, dev, types = _tensor_list("grad_norm", tensors)
     with _on(dev):
-        return _norm(_table([t.contiguous() for t in ts]), dev)
+        return _norm(_table(_dense(ts), types), dev)
 
 
 @torch.no_grad()
 def clip_grad_norm_(grads, max_norm, out=None):
     """scales the tensors by min(1, max_norm / (norm + 1e-6)), norm as grad_norm gives it, and returns the norm (float32 scalar on their
-    device; nothing waits for it).  In place, or into `out`: as many contiguous tensors of the same shapes, of any of the three types
+    device; nothing waits for it).  In place, or into `out`: as many contiguous tensors of as many elements each, of any of the three types
     (half-precision gradients into float32 ones, say).  None entries are skipped (in `out` too).  A tensor may be named once only, and an
     `out` tensor may share memory with its own gradient (of the same type) but not with another one."""
     name = "clip_grad_norm_"
@@ -319,23 +333,23 @@ def clip_grad_norm_(grads, max_norm, out=None):
         out = list(out)
         if len(out) != len(grads) or any((g is None) != (o is None) for g, o in zip(grads, out)):
             raise ValueError("%s: %d gradients, %d outputs (None where the gradient is)" % (name, len(grads), len(out)))
-    ts, dev = _tensor_list(name, grads)
-    src = [t if t.is_contiguous() else t.contiguous() for t in ts]
+    ts, dev, types = _tensor_list(name, grads)
+    src = _dense(ts)
+    tab = _table(src, types)
     if out is None:
-        dst = src
+        tab["out"], tab["out_dtype"] = tab["data"], tab["dtype"]
     else:
-        dst, dev_o = _tensor_list(name, out)
-        if dev_o != dev or [o.shape for o in dst] != [t.shape for t in ts] or not all([o.is_contiguous() for o in dst]):
-            raise ValueError("%s: outputs must be contiguous, of the gradients' shapes and on their device" % name)
-    tab = _table(src, dst)
-    full = tab[tab["n"] > 0] if (tab["n"] == 0).any() else tab
+        dst, dev_o, types = _tensor_list(name, out)
+        if dev_o != dev or [o.numel() for o in dst] != tab["n"].tolist() or not all([o.is_contiguous() for o in dst]):
+            raise ValueError("%s: outputs must be contiguous, of as many elements as the gradients and on their device" % name)
+        tab["out"], tab["out_dtype"] = [o.data_ptr() for o in dst], types
+    full = tab[tab["n"] > 0]
     places = set(full["out"].tolist())
     if len(places) != len(full):
         raise ValueError("%s: a tensor is named twice" % name)
-    if out is not None:
+    if out is not None and not places.isdisjoint(full["data"].tolist()):
         own = full["out"] == full["data"]
-        if places & set(full["data"][~own].tolist()) or (places & set(full["data"][own].tolist())
-                                                         and ((full["dtype"] != full["out_dtype"]) & own).any()):
+        if not places.isdisjoint(full["data"][~own].tolist()) or ((full["dtype"] != full["out_dtype"]) & own).any():
             raise ValueError("%s: an output shares memory with another gradient, or with its own of another type" % name)
     with _on(dev):
         norm = _norm(tab, dev)

@@ -61,8 +61,8 @@ def test_c_entry_points_refuse_bad_arguments():
     from nirrt_star_amd import nnops
     L = nnops._lib()
     p = C.c_void_p(4096)            # (never read: every call is refused by its other arguments)
-    assert L.nirrt_nn_linear_workspace(3, 1, 1, 1) == -1 and L.nirrt_nn_linear_workspace(0, -1, 1, 1) == -1
-    assert L.nirrt_nn_linear_workspace(0, 1 << 31, 1, 1) == -1
+    assert L.nirrt_nn_linear_workspace(3, p, 1, p, 1, 1, 1, 1) == -1 and L.nirrt_nn_linear_workspace(0, p, 1, p, 1, -1, 1, 1) == -1
+    assert L.nirrt_nn_linear_workspace(0, p, 1, p, 1, 1 << 31, 1, 1) == -1
     assert L.nirrt_nn_linear(7, 0, p, 4, p, 4, None, None, 4, p, 4, None, 4, 4, 4, p, None) == -1       # element type
     assert L.nirrt_nn_linear(0, 4, p, 4, p, 4, None, None, 4, p, 4, None, 4, 4, 4, p, None) == -1       # activation
     assert L.nirrt_nn_linear(0, 0, p, 3, p, 4, None, None, 4, p, 4, None, 4, 4, 4, p, None) == -1       # row stride below the row
@@ -70,10 +70,10 @@ def test_c_entry_points_refuse_bad_arguments():
     assert L.nirrt_nn_linear(0, 0, p, 4, p, 4, None, p, 3, p, 4, None, 4, 4, 4, p, None) == -1          # residual stride
     assert L.nirrt_nn_linear(0, 0, p, 4, p, 4, None, None, 4, p, 4, None, 0, 4, 4, None, None) == 0     # nothing to do
     big = 1 << 16
-    assert L.nirrt_nn_linear_workspace(0, 8, 64, big) > 0
-    assert L.nirrt_nn_linear(0, 0, p, big, p, big, None, None, 64, p, 64, None, 8, 64, big, None, None) == -1   # workspace missing
+    assert L.nirrt_nn_linear_workspace(0, p, big, p, big, 64, 64, big) > 0
+    assert L.nirrt_nn_linear(0, 0, p, big, p, big, None, None, 64, p, 64, None, 64, 64, big, None, None) == -1   # workspace missing
     for m, n, k in ((0, 4, 4), (4, 0, 4), (4, 4, 0), (0, 0, 0)):                                         # empty sizes have a size too
-        assert L.nirrt_nn_linear_workspace(0, m, n, k) == 0 and L.nirrt_nn_linear_backward_workspace(0, 1, m, n, k) >= 0
+        assert L.nirrt_nn_linear_workspace(0, p, 4, p, 4, m, n, k) == 0 and L.nirrt_nn_linear_backward_workspace(0, 1, p, 4, p, 4, p, 4, m, n, k) >= 0
         assert L.nirrt_nn_cross_entropy_workspace(0, m, 4, k) >= 0 and L.nirrt_nn_cross_entropy_backward_workspace(0, m, 4, k) >= 0
     assert L.nirrt_nn_linear_backward(0, 2, p, 4, p, 4, None, p, 4, p, p, p, 4, 4, 4, p, None) == -1    # z missing
     assert L.nirrt_nn_cross_entropy_workspace(0, 4, 0, 4) == -1                                          # no classes
