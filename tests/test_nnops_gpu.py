@@ -128,11 +128,11 @@ def test_linear_empty_and_special_values():
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("act", ["none", "gelu", "silu"])
 @pytest.mark.parametrize("m,k,n", [(1, 128, 128), (7, 515, 321), (130, 96, 36), (257, 33, 70), (2000, 260, 132), (5000, 16, 8), (3, 1, 2)])
-def test_linear_gradients(m, k, n, act, dt):
+def test_linear_gradients(m, k, n, act, dt, dy=None):
     from nirrt_star_amd import nnops
     g = gen(m + k * 3 + n)
     x, w, b, r = randn((m, k), g, dt), randn((n, k), g, dt, k ** -0.5), randn((n,), g, dt), randn((m, n), g, dt)
-    dy = randn((m, n), g, dt)
+    dy = randn((m, n), g, dt) if dy is None else dy
     leaves = [t.clone().requires_grad_(True) for t in (x, w, b, r)]
     y = nnops.linear_act(*leaves, activation=act)
     dx, dw, db, dr = torch.autograd.grad(y, leaves, dy)
@@ -546,3 +546,44 @@ def test_more_than_two_to_the_31_elements():
     within(y[-3:], want, ey, torch.float16)
     assert (y[:-3] == 0).all()
     assert abs(float(nnops.grad_norm([x])) / float(x[-3:].double().norm()) - 1) < 1e-6
+
+
+# ---- sizes at which the kernels change ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("m,k,n", [(16, 515, 321), (17, 4096, 40), (32, 7, 16), (33, 515, 321), (31, 1, 4100)])
+def test_linear_few_rows(m, k, n, dt):
+    test_linear_gradients(m, k, n, "gelu", dt)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("m,k,n,act", [(4000, 328, 4064, "silu"), (4000, 4064, 328, "gelu"), (328, 4064, 4000, "relu"), (4000, 329, 4063, "silu"),
+                                       (4003, 4063, 327, "none"), (3000, 1000, 24, "none"), (300, 9000, 264, "gelu"), (777, 515, 1029, "none")])
+def test_linear_large_tiles_and_parts(m, k, n, act, dt):
+    """the largest tiles in each of the three products with ragged edges, reductions in parts, odd operands copied into whole chunks"""
+    if act == "relu":                  # (no slope at a rounded 0: the forward product only)
+        from nirrt_star_amd import nnops
+        g = gen(m + k)
+        x, w, b = randn((m, k), g, dt), randn((n, k), g, dt, k ** -0.5), randn((n,), g, dt)
+        _, _, y, ey = linear64(x, w, b, None, act)
+        within(nnops.linear_act(x, w, b, activation=act), y, ey, dt)
+        act = "silu"
+    test_linear_gradients(m, k, n, act, dt)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_linear_layouts_of_the_incoming_gradient(act, dt):
+    """gradients that arrive transposed, as columns of a wider tensor, off 16 bytes, or as one value for all (a sum's)"""
+    g = gen(17)
+    for m, k, n in ((70, 40, 48), (129, 33, 35)):
+        for dy in (randn((n, m), g, dt).t(), randn((m, n + 9), g, dt)[:, 3:3 + n], randn((m, 2 * n), g, dt)[:, ::2], randn((1, 1), g, dt).expand(m, n),
+                   randn((1, n), g, dt).expand(m, n)):
+            test_linear_gradients(m, k, n, act, dt, dy)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("rows,k,v", [(64, 31, 3), (256, 128, 5), (257, 200, 8), (255, 129, 9), (128, 64, 64), (130, 8, 65), (2100, 515, 1031), (3000, 264, 4100),
+                                      (33, 1030, 257), (1500, 1, 6)])
+def test_cross_entropy_more_sizes(rows, k, v, dt):
+    test_cross_entropy(rows, k, v, "mean", True, True, dt)
+    test_cross_entropy(rows, k, v, "none", False, False, dt)

@@ -42,7 +42,7 @@ def test_step_equals_the_plain_evaluation():
     loss, norm = train_step(m, opt, x, labels, cw, max_norm=0.25, fps_starts=starts)
     hook.remove()
     # head and loss from the features the step saw, in 64 bits
-    h = seen["h"].relu().permute(0, 2, 1).reshape(-1, 128).double()
+    h = seen["h"].relu().double()
     w, b = before["conv2.weight"].squeeze(2).double(), before["conv2.bias"].double()
     t = labels.reshape(-1)
     keep = t >= 0
@@ -93,3 +93,12 @@ def test_without_clipping_the_gradients_stay():
     loss, norm = train_step(m, opt, x, labels, fps_starts=starts)
     total = float(torch.stack([p.grad.double().square().sum() for p in m.parameters()]).sum().sqrt())
     assert torch.isfinite(loss) and abs(float(norm) - total) <= 1e-6 * total
+
+
+def test_a_folded_model_in_eval_mode_is_refused():
+    m = _model(6).eval().fold()
+    x, labels, starts = _batch(1, 1100, 4)
+    with pytest.raises(RuntimeError):
+        m.loss(x, labels)
+    m.train()
+    assert torch.isfinite(m.loss(x, labels, None, starts))
