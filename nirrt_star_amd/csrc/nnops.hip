@@ -701,23 +701,35 @@ __global__ __launch_bounds__(256) void k_dz(const T *z, const T *dy, int64_t ldd
     float s[V];
 #pragma unroll
     for (int e = 0; e < V; e++) s[e] = 0.f;
-    if (cnt > 0)
-#pragma unroll 4
-        for (int i = i0 + rr; i < i1; i += step) {
-            Pack<T, V> d = load_some<T, V>(dy + (int64_t)i * lddy + j, cnt);
-            if (act != NIRRT_NN_ACT_NONE) {
-                const Pack<T, V> q = load_some<T, V>(z + (int64_t)i * n + j, cnt);
+    const auto one = [&](Pack<T, V> d, const Pack<T, V> &q, int i) {
+        if (act != NIRRT_NN_ACT_NONE) {
 #pragma unroll
-                for (int e = 0; e < V; e++) {
-                    const float v = (float)d.e[e] * act_slope(act, (float)q.e[e]);
-                    s[e] += v;
-                    d.e[e] = (T)v;
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < V; e++) s[e] += (float)d.e[e];
+            for (int e = 0; e < V; e++) {
+                const float v = (float)d.e[e] * act_slope(act, (float)q.e[e]);
+                s[e] += v;
+                d.e[e] = (T)v;
             }
-            if (dz) store_pack(dz + (int64_t)i * lddz + j, d);               // (rows of whole packs, zeros behind column n)
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; e++) s[e] += (float)d.e[e];
+        }
+        if (dz) store_pack(dz + (int64_t)i * lddz + j, d);                   // (rows of whole packs, zeros behind column n)
+    };
+    int i = i0 + rr;
+    if (cnt >= V)                                                            // whole packs: four rows' loads on their way at once
+        for (; i + 3 * step < i1; i += 4 * step) {
+            Pack<T, V> d[4], q[4];
+#pragma unroll
+            for (int g = 0; g < 4; g++) d[g] = load_pack<T, V>(dy + (int64_t)(i + g * step) * lddy + j);
+#pragma unroll
+            for (int g = 0; g < 4; g++) q[g] = act != NIRRT_NN_ACT_NONE ? load_pack<T, V>(z + (int64_t)(i + g * step) * n + j) : d[g];
+#pragma unroll
+            for (int g = 0; g < 4; g++) one(d[g], q[g], i + g * step);
+        }
+    if (cnt > 0)
+        for (; i < i1; i += step) {
+            const Pack<T, V> d = load_some<T, V>(dy + (int64_t)i * lddy + j, cnt);
+            one(d, act != NIRRT_NN_ACT_NONE ? load_some<T, V>(z + (int64_t)i * n + j, cnt) : d, i);
         }
     if (!sums) return;
 #pragma unroll
