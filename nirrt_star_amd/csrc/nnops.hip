@@ -742,19 +742,22 @@ __global__ __launch_bounds__(256) void k_dz(const T *z, const T *dy, int64_t ldd
         if (col < n) sums[(int64_t)blockIdx.y * n + col] = a;
     }
 }
-// out[j] = factor scale sum over parts of sums[p, j], in a fixed order: 64 columns x 4 shares of the parts per workgroup
-template <class T> __global__ __launch_bounds__(256) void k_column_join(const float *sums, int parts, const float *scale, float factor, T *out, int64_t n)
+// out[j] = sum over parts of sums[p, j] for j < n, tail[j - n] for the n_tail columns behind them, in a fixed order: 64 columns x 4 shares of
+// the parts per workgroup
+template <class T> __global__ __launch_bounds__(256) void k_column_join(const float *sums, int parts, T *out, int64_t n, T *tail, int64_t n_tail)
 {
     __shared__ float meet[4][64];
     const int64_t j = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
     float s = 0.f;
-    if (j < n)
+    if (j < n + n_tail)
 #pragma unroll 8
-        for (int p = threadIdx.x >> 6; p < parts; p += 4) s += sums[p * n + j];
+        for (int p = threadIdx.x >> 6; p < parts; p += 4) s += sums[p * (n + n_tail) + j];
     meet[threadIdx.x >> 6][threadIdx.x & 63] = s;
     __syncthreads();
-    if (threadIdx.x < 64 && j < n)
-        out[j] = (T)(((meet[0][threadIdx.x] + meet[1][threadIdx.x]) + (meet[2][threadIdx.x] + meet[3][threadIdx.x])) * (scale ? *scale * factor : factor));
+    if (threadIdx.x < 64 && j < n + n_tail) {
+        T *to = j < n ? out + j : tail + (j - n);
+        if (j < n ? out : tail) *to = (T)((meet[0][threadIdx.x] + meet[1][threadIdx.x]) + (meet[2][threadIdx.x] + meet[3][threadIdx.x]));
+    }
 }
 
 // x with the rows that do not count set to zero (whatever they hold: 0 x NaN must not reach dw), padded with zeros to ld columns and
@@ -1072,11 +1075,11 @@ __global__ __launch_bounds__(256) void k_ce_few(const T *x, int64_t ldx, const T
     float *lb = few + classes * kp;
     few_weights(w, ldw, b, classes, k, kp, few, lb);
     double a = 0., n = 0.;
-    for (int r0 = blockIdx.x * per; r0 < rows; r0 += gridDim.x * per) {
-        const int r = r0 + threadIdx.x / G;
+    for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < rows; r0 += gridDim.x * per) {
+        const int64_t r = r0 + threadIdx.x / G;
         FewRow<T, V, NC> q;
         float l[V];
-        q.load(x + (int64_t)r * ldx, k, g, G, r < rows);
+        q.load(x + r * ldx, k, g, G, r < rows);
         q.scores(few, lb, kp, classes, g, G, l);
         if (r < rows && g == 0) {
             float top = -__builtin_inff(), sum = 0.f, mine = 0.f;
@@ -1103,11 +1106,11 @@ __global__ __launch_bounds__(256) void k_ce_few(const T *x, int64_t ldx, const T
     __syncthreads();
     if (threadIdx.x < 2) sums[2 * blockIdx.x + threadIdx.x] = (part[threadIdx.x][0] + part[threadIdx.x][1]) + (part[threadIdx.x][2] + part[threadIdx.x][3]);
 }
-// shares (workgroup, class, k) of dw and behind them (workgroup, class) of db, both fp32; dx written whole
+// sums: per workgroup its share (class, k) of dw and behind it (class) of db, fp32; dx written whole
 template <class T, int V, int NC>
 __global__ __launch_bounds__(256) void k_ce_few_backward(const T *x, int64_t ldx, const T *w, int64_t ldw, const T *b, const int64_t *target,
                                                          const float *cw, int64_t ignore, const float *lse, const float *dloss, int stride,
-                                                         const float *total, T *dx, float *dw, float *db, int rows, int classes, int k, int G)
+                                                         const float *total, T *dx, float *sums, int rows, int classes, int k, int G)
 {
     constexpr int P = FewRow<T, V, NC>::P;
     extern __shared__ float few[];           // classes x kp weights, V biases; later 256 / G x kp shares of one class
@@ -1121,15 +1124,24 @@ __global__ __launch_bounds__(256) void k_ce_few_backward(const T *x, int64_t ldx
 #pragma unroll
         for (int e = 0; e < NC * P; e++) aw[v][e] = 0.f;
     }
-    for (int r0 = blockIdx.x * per; r0 < rows; r0 += gridDim.x * per) {
-        const int r = r0 + threadIdx.x / G;
-        const float c = r < rows ? row_coefficient(dloss, stride, total, target, cw, ignore, classes, r) : 0.f;
-        FewRow<T, V, NC> q;
+    struct Ahead { FewRow<T, V, NC> q; float c, z; int64_t t; } next;          // the next row travels while this one is worked on
+    const auto fetch = [&](int64_t r) {
+        next.q.load(x + r * ldx, k, g, G, r < rows);
+        next.c = r < rows ? row_coefficient(dloss, stride, total, target, cw, ignore, classes, (int)r) : 0.f;
+        next.z = r < rows ? lse[r] : 0.f;
+        next.t = r < rows ? target[r] : -1;
+    };
+    fetch((int64_t)blockIdx.x * per + threadIdx.x / G);
+    for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < rows; r0 += gridDim.x * per) {
+        const int64_t r = r0 + threadIdx.x / G;
+        FewRow<T, V, NC> q = next.q;
+        const float c = next.c, z = next.z;
+        const int64_t t = next.t;
         float l[V], out[NC * P];
-        q.load(x + (int64_t)r * ldx, k, g, G, r < rows && c != 0.f);          // (a row that does not count is zeros, whatever it holds)
+        fetch(r + (int64_t)gridDim.x * per);
+#pragma unroll
+        for (int e = 0; e < NC * P; e++) q.x[e] = c != 0.f ? q.x[e] : 0.f;      // (a row that does not count is zeros, whatever it holds)
         q.scores(few, lb, kp, classes, g, G, l);
-        const float z = r < rows ? lse[r] : 0.f;
-        const int64_t t = r < rows ? target[r] : -1;
 #pragma unroll
         for (int e = 0; e < NC * P; e++) out[e] = 0.f;
 #pragma unroll
@@ -1149,7 +1161,7 @@ __global__ __launch_bounds__(256) void k_ce_few_backward(const T *x, int64_t ldx
 #pragma unroll
             for (int m = 0; m < NC; m++) {
                 const int at = (m * G + g) * P;
-                T *o = dx + (int64_t)r * k + at;
+                T *o = dx + r * k + at;
                 Pack<T, P> v;
 #pragma unroll
                 for (int e = 0; e < P; e++) v.e[e] = (T)out[m * P + e];
@@ -1170,7 +1182,7 @@ __global__ __launch_bounds__(256) void k_ce_few_backward(const T *x, int64_t ldx
         for (int c = threadIdx.x; c < k; c += 256) {
             float s = 0.f;
             for (int q = 0; q < per; q++) s += few[q * kp + c];
-            dw[((int64_t)blockIdx.x * classes + v) * k + c] = s;
+            sums[((int64_t)blockIdx.x * (k + 1)) * classes + (int64_t)v * k + c] = s;
         }
         __syncthreads();
         if (g == 0) few[threadIdx.x / G] = ab[v];
@@ -1178,7 +1190,7 @@ __global__ __launch_bounds__(256) void k_ce_few_backward(const T *x, int64_t ldx
         if (threadIdx.x == 0) {
             float s = 0.f;
             for (int q = 0; q < per; q++) s += few[q];
-            db[(int64_t)blockIdx.x * classes + v] = s;
+            sums[((int64_t)blockIdx.x * (k + 1) + k) * classes + v] = s;
         }
     }
 }
@@ -1503,7 +1515,7 @@ int linear_backward_t(int dtype, int act, const void *x, int64_t ldx, const void
             hipLaunchKernelGGL((k_dz<T>), dim3((unsigned)c.blocks, (unsigned)c.parts), dim3(256), 0, st, (const T *)z, (const T *)dy, lddy,
                                l.dz ? dz : (T *)nullptr, l.np, db ? sums : nullptr, (int)m, (int)n, c.chunk, c.lanes, act);
         if (db)
-            hipLaunchKernelGGL((k_column_join<T>), dim3((unsigned)ceil_div(n, 64)), dim3(256), 0, st, sums, c.parts, (const float *)nullptr, 1.f, (T *)db, n);
+            hipLaunchKernelGGL((k_column_join<T>), dim3((unsigned)ceil_div(n, 64)), dim3(256), 0, st, sums, c.parts, (T *)db, n, (T *)nullptr, (int64_t)0);
         if (int rc_ = status()) return rc_;
     }
     const T *d = l.dz ? dz : (const T *)dy;
@@ -1527,7 +1539,8 @@ int linear_backward_t(int dtype, int act, const void *x, int64_t ldx, const void
 }
 
 // few classes (k_ce_few): up to 8, and a row on at most 64 lanes x 4 packs
-struct Few { int lanes, packs, classes, blocks, lds, lds_backward; };
+struct Few { int lanes, packs, classes, blocks_forward, blocks, lds, lds_backward; };
+constexpr int FEW_BLOCKS = 2048;
 bool few_layout(int dtype, int64_t rows, int64_t classes, int64_t k, Few &f)
 {
     const int p = 16 / elem_size(dtype);
@@ -1540,19 +1553,22 @@ bool few_layout(int dtype, int64_t rows, int64_t classes, int64_t k, Few &f)
     f.classes = classes <= 2 ? 2 : classes <= 4 ? 4 : 8;
     if (f.classes * f.packs * p > 128) return false;      // registers of dw
     const int kp = f.packs * f.lanes * p, per = 256 / f.lanes;
-    const int64_t blocks = ceil_div(rows, 4 * per);       // (at least four rows per lane group, at most two workgroups per CU)
+    // forward eight workgroups per CU, so that enough rows are on their way; backward two, because each leaves a share of dw behind (and asks for
+    // its next rows ahead instead): at least two and four rows per lane group
+    const int64_t forward = ceil_div(rows, 2 * per), blocks = ceil_div(rows, 4 * per);
+    f.blocks_forward = (int)(forward < FEW_BLOCKS ? (forward > 0 ? forward : 1) : FEW_BLOCKS);
     f.blocks = (int)(blocks < 512 ? (blocks > 0 ? blocks : 1) : 512);
     f.lds = (int)(4 * (classes * kp + 8));
     f.lds_backward = f.lds > 4 * per * kp ? f.lds : 4 * per * kp;
     return true;
 }
-#define FEW_LAUNCH(KERNEL, LDS, ...)                                                                                     \
+#define FEW_LAUNCH(KERNEL, BLOCKS, LDS, ...)                                                                                     \
     do {                                                                                                                 \
-        if (f.classes == 2) { if (f.packs == 1) FEW_ONE(KERNEL, 2, 1, LDS, __VA_ARGS__); else if (f.packs == 2) FEW_ONE(KERNEL, 2, 2, LDS, __VA_ARGS__); else FEW_ONE(KERNEL, 2, 4, LDS, __VA_ARGS__); } \
-        else if (f.classes == 4) { if (f.packs == 1) FEW_ONE(KERNEL, 4, 1, LDS, __VA_ARGS__); else if (f.packs == 2) FEW_ONE(KERNEL, 4, 2, LDS, __VA_ARGS__); else FEW_ONE(KERNEL, 4, 4, LDS, __VA_ARGS__); } \
-        else { if (f.packs == 1) FEW_ONE(KERNEL, 8, 1, LDS, __VA_ARGS__); else if (f.packs == 2) FEW_ONE(KERNEL, 8, 2, LDS, __VA_ARGS__); else FEW_ONE(KERNEL, 8, 4, LDS, __VA_ARGS__); } \
+        if (f.classes == 2) { if (f.packs == 1) FEW_ONE(KERNEL, 2, 1, BLOCKS, LDS, __VA_ARGS__); else if (f.packs == 2) FEW_ONE(KERNEL, 2, 2, BLOCKS, LDS, __VA_ARGS__); else FEW_ONE(KERNEL, 2, 4, BLOCKS, LDS, __VA_ARGS__); } \
+        else if (f.classes == 4) { if (f.packs == 1) FEW_ONE(KERNEL, 4, 1, BLOCKS, LDS, __VA_ARGS__); else if (f.packs == 2) FEW_ONE(KERNEL, 4, 2, BLOCKS, LDS, __VA_ARGS__); else FEW_ONE(KERNEL, 4, 4, BLOCKS, LDS, __VA_ARGS__); } \
+        else { if (f.packs == 1) FEW_ONE(KERNEL, 8, 1, BLOCKS, LDS, __VA_ARGS__); else if (f.packs == 2) FEW_ONE(KERNEL, 8, 2, BLOCKS, LDS, __VA_ARGS__); else FEW_ONE(KERNEL, 8, 4, BLOCKS, LDS, __VA_ARGS__); } \
     } while (0)
-#define FEW_ONE(KERNEL, V, NC, LDS, ...) hipLaunchKernelGGL((KERNEL<T, V, NC>), dim3((unsigned)f.blocks), dim3(256), LDS, st, __VA_ARGS__)
+#define FEW_ONE(KERNEL, V, NC, BLOCKS, LDS, ...) hipLaunchKernelGGL((KERNEL<T, V, NC>), dim3((unsigned)BLOCKS), dim3(256), LDS, st, __VA_ARGS__)
 
 // cross entropy: tile edge, and parts of the classes so that row tiles x parts fill the GPU; x and w whose rows are no whole aligned chunks
 // are copied into such (k_rows_copy): the products read them many times
@@ -1571,7 +1587,7 @@ CeForward ce_layout(int dtype, int64_t rows, int64_t classes, int64_t k)
     f.parts = (int)(class_tiles > 0 ? ceil_div(class_tiles, per) : 1);
     f.stats = round256(8 * rows * f.parts);
     f.score = round256(4 * rows);
-    f.sums = round256(16 * (ceil_div(rows, CE_ROWS) + 512));
+    f.sums = round256(16 * (ceil_div(rows, CE_ROWS) + FEW_BLOCKS));
     f.xs = round256(rows * padded(dtype, k) * elem_size(dtype));
     f.ws = round256(classes * padded(dtype, k) * elem_size(dtype));
     f.total = f.stats + f.score + f.sums + f.xs + f.ws;
@@ -1589,8 +1605,8 @@ int ce_forward_t(int dtype, const void *x, int64_t ldx, const void *w, int64_t l
     int64_t blocks = 0;
     Few f;
     if (rows > 0 && few_layout(dtype, rows, classes, k, f)) {
-        blocks = f.blocks;
-        FEW_LAUNCH(k_ce_few, f.lds, (const T *)x, ldx, (const T *)w, ldw, (const T *)b, target, cw, ignore, (int)rows, (int)classes, (int)k, f.lanes, lse,
+        blocks = f.blocks_forward;
+        FEW_LAUNCH(k_ce_few, f.blocks_forward, f.lds, (const T *)x, ldx, (const T *)w, ldw, (const T *)b, target, cw, ignore, (int)rows, (int)classes, (int)k, f.lanes, lse,
                    nll, sums);
     } else if (rows > 0) {
         blocks = ceil_div(rows, CE_ROWS);
@@ -1651,15 +1667,12 @@ int ce_backward_t(int dtype, const void *x, int64_t ldx, const void *w, int64_t 
     const CeBackward l = ce_backward_layout(dtype, rows, classes, k);
     Few f;
     if (few_layout(dtype, rows, classes, k, f)) {
-        float *sw = (float *)ws, *sb = sw + k * classes * f.blocks;
-        FEW_LAUNCH(k_ce_few_backward, f.lds_backward, (const T *)x, ldx, (const T *)w, ldw, (const T *)b, target, cw, ignore, lse, dloss, stride, total, (T *)dx,
-                   sw, sb, (int)rows, (int)classes, (int)k, f.lanes);
-        if (dw && k > 0)
-            hipLaunchKernelGGL((k_column_join<T>), dim3((unsigned)ceil_div(classes * k, 64)), dim3(256), 0, st, sw, f.blocks, (const float *)nullptr, 1.f,
-                               (T *)dw, classes * k);
-        if (db)
-            hipLaunchKernelGGL((k_column_join<T>), dim3((unsigned)ceil_div(classes, 64)), dim3(256), 0, st, sb, f.blocks, (const float *)nullptr, 1.f, (T *)db,
-                               classes);
+        float *sums = (float *)ws;
+        FEW_LAUNCH(k_ce_few_backward, f.blocks, f.lds_backward, (const T *)x, ldx, (const T *)w, ldw, (const T *)b, target, cw, ignore, lse, dloss, stride, total, (T *)dx,
+                   sums, (int)rows, (int)classes, (int)k, f.lanes);
+        if (dw || db)
+            hipLaunchKernelGGL((k_column_join<T>), dim3((unsigned)ceil_div(classes * (k + 1), 64)), dim3(256), 0, st, sums, f.blocks, (T *)dw, classes * k,
+                               (T *)db, classes);
         return status();
     }
     float *scale = (float *)ws, *coef = scale + 64, *tops = (float *)(ws + l.coef);
