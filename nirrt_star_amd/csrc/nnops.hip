@@ -4,12 +4,15 @@
 //   cross entropy   softmax cross entropy of the scores x w^T + b without keeping them, and its gradients
 //   norm / scale    2-norm of many tensors, and the clipping by it
 //
-// All products run through one tile loop (class-free: mainloop below) on v_mfma_f32_32x32x*: a workgroup of 4 waves owns a tile
-// C[i, j] = sum_k A[i, k] B[j, k], K-steps of 128 bytes per row.  An operand is stored either with k contiguous ("KC": x, w in the forward
-// product) or with i contiguous ("RC": w in dx = dz w, dz and x in dw = dz^T x); an RC operand is transposed in registers on its way
-// into the LDS, so both look alike there: rows of eight 16-byte chunks along k, chunk c of row r at place c ^ sw(r).  A lane's 16-byte
-// read is one operand of a 16-bit MFMA (8 k) or four of a 32-bit one (4 x 1 k); the order of k inside a step is the same in A and B, so
-// the sum is the same whatever it is.  Accumulators and partial sums are fp32.
+// Products of more than 32 rows run on v_mfma_f32_32x32x*: a workgroup of 4 or 8 waves owns a tile C[i, j] = sum_k A[i, k] B[j, k].  An operand is
+// stored either with k contiguous ("KC": x, w in the forward product) or with i contiguous ("RC": w in dx = dz w, dz and x in dw = dz^T x).
+// Two tile loops: DirectTile for operands of whole aligned 16-byte chunks (memory -> LDS, a ring of four stages), Tile for all others
+// (memory -> registers -> LDS).  A lane's 16 bytes are one operand of a 16-bit MFMA (8 k) or four of a 32-bit one (4 x 1 k); the order of k
+// inside a step is the same in A and B, so the sum is the same whatever it is.  Accumulators and partial sums are fp32.
+//
+// Times are those of an MI355X that copies at 5.1 TB/s; its library's products reach 1135 - 1290 TFLOP/s (bf16) and 131 (fp32).  For 16384 x 4096 x
+// 4096 in bf16: 560 us forward (z, r and y in the epilogue: 590), 514 dx, 482 dw (1140 TFLOP/s; the library 425 - 480); under these kernels the
+// clock falls to 1.5 GHz (power), where MFMA alone reach 1313.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -81,7 +84,8 @@ template <class T, int N> __device__ __forceinline__ void store_some(T *p, const
         if (e < n) p[e] = v.e[e];
 }
 
-// a thread's share of one K-step of R rows: global memory -> registers -> LDS
+// a thread's share of one K-step (128 bytes per row) of R rows: global memory -> registers -> LDS.  There both kinds look alike: rows of
+// eight 16-byte chunks along k, chunk c of row r at place c ^ sw(r); an RC operand is transposed in registers on its way.
 template <class T, int R, int NT, bool RC> struct Stage {
     static constexpr int N = R * CHUNKS / NT, CE = Elem<T>::PER_CHUNK, VR = N % 4 == 0 ? 4 : 2;   // VR: rows of a transposed block
     static_assert(N % 2 == 0 && R % 4 == 0, "whole blocks per thread");
@@ -216,9 +220,9 @@ constexpr int STAGES = 4, RING_BYTES = 64, RING_CHUNKS = RING_BYTES / 16;
 __device__ __forceinline__ int ring_sw(int row) { return (row >> 2) & 3; }   // 16 lanes on 16 rows: 16 places of 16 bytes
 constexpr unsigned NOWHERE = 0x7ffffff0u;   // an offset beyond every buffer (direct() keeps them below)
 
-// 16 bytes per lane from buffer + offset to lds + 16 lane.  Written out, because the compiler does not know which part of the LDS a load of its own
-// writes and waits for all of them before every transposing read (902 us instead of 567 for dw of 16384 x 4096 x 4096).  It has no
-// result register; the waits are arrive() below, which every use of the LDS stands behind.
+// 16 bytes per lane from buffer + offset to lds + 16 lane.  Written out, because the compiler does not know which part of the LDS a load of its
+// own writes, and would wait for all of them before every read.  It has no result register; the waits are arrive() below, which every use of
+// the LDS stands behind.
 __device__ __forceinline__ void load_to_lds(u32x4 buffer, const u32x4 *lds, unsigned offset)
 {
 #ifdef __HIP_DEVICE_COMPILE__
@@ -605,7 +609,7 @@ __global__ __launch_bounds__(Tl::NT) void k_gemm(Operand<T> a, Operand<T> b, int
 // ---- few rows (m <= 32): every weight is read for a handful of rows, so what bounds the product is reading w ---------------------------------
 // A workgroup of eight waves owns 16 columns; each wave takes every eighth step of 64 bytes per row of w, eight steps in flight (8 KB per
 // wave: some 64 KB per CU cover the latency), multiplies them on 16 x 16 MFMA with the rows of x straight from memory, and the waves' sums
-// meet in the LDS.  One launch, nothing cut, no workspace.
+// meet in the LDS.  One launch, nothing cut, no workspace.  7 x 4096 x 4096 in fp16: 9.8 us, 3.4 TB/s of w (a cut 64-wide tile and its join: 9 + 4 us).
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ f32x4_t mma16(bf16_t, u32x4 a, u32x4 b, f32x4_t c)
 {
@@ -690,7 +694,8 @@ template <class Epi> __global__ __launch_bounds__(256) void k_join(const float *
 
 // ---- dz = dy act'(z) and its column sums -------------------------------------------------------------------------------------------
 // grid (column blocks, row chunks).  A row's 16-byte packs lie on `lanes` (a power of two) neighbouring lanes, 256 / lanes rows at a time;
-// a lane keeps the sums of its columns over the chunk, the rows' lanes meet in the LDS: sums (chunk, column), joined by k_column_join.
+// a lane keeps the sums of its columns over the chunk, the rows' lanes meet in the LDS: sums (chunk, column), joined by k_column_join.  Bound by
+// memory: 16384 x 4096 in bf16 93 us (4.3 TB/s; 106 with one row's loads at a time).
 template <class T>
 __global__ __launch_bounds__(256) void k_dz(const T *z, const T *dy, int64_t lddy, T *dz, int64_t lddz, float *sums, int m, int n, int chunk, int lanes, int act)
 {
@@ -787,7 +792,8 @@ __device__ __forceinline__ float row_weight(const float *cw, int64_t t, int64_t 
 constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
 
 // C[v, r] = w_v . x_r: a lane holds scores of NI rows r (its columns), so the running maximum and sum over the classes stay in the
-// lane; the two halves of a wave and the waves above one another meet once, at the end.  grid (row tiles, parts of the classes).
+// lane; the two halves of a wave and the waves above one another meet once, at the end.  grid (row tiles, parts of the classes).  Bound by the
+// products: 8192 x 1024 x 32003 in bf16 544 us (987 TFLOP/s; the library's product alone, scores written: 499).
 template <class T, int BM, int BN, class Tl>
 __global__ __launch_bounds__(Tl::NT) void k_ce_stats(Operand<T> w, Operand<T> x, const T *b, const int64_t *target, int rows, int classes,
                                                            int k, int part, float2 *stats, float *target_score)
@@ -968,7 +974,10 @@ __global__ __launch_bounds__(256) void k_ce_scale(const float *tops, int blocks,
 }
 // g' = c_r / scale (exp(l - lse_r) - [v = target]) FACTOR in the element type, stored (v, r): the product C[v, r] again.  16-bit products
 // need 16-bit operands; c / scale <= 1 keeps the range, and FACTOR 4096 in f16 lifts probabilities of large vocabularies (1e-5) out of
-// its subnormals.  Relative error of a rounding: 2^-9 (bf16), 2^-12 (f16) of the element, like the rounding of dz in the linear layer.
+// its subnormals.  A rounding is off by 2^-8 (bf16), 2^-11 (f16) of the element at most, like the rounding of dz in the linear layer.
+// The scores are multiplied out again rather than kept: at 1024 inputs in bf16 that costs 2 ps per score, writing and reading them in 32 bits
+// 1.6; in fp32 it costs 15 fs per input and score, so a head of many inputs pays for the memory it saves (991 x 1703 x 1320: 290 us
+// against 232 of the elementary form).
 template <class T> struct Factor { static constexpr float VALUE = 1.f; };
 template <> struct Factor<f16_t> { static constexpr float VALUE = 4096.f; };
 template <class T> struct EpiSoftmaxGrad {
@@ -1017,7 +1026,8 @@ template <class T> __global__ __launch_bounds__(256) void k_ce_bias(const T *g, 
 // Two classes and 128 inputs are what the guidance network's head has: a tile of 64 classes would be empty but for two, and what bounds the
 // operator is reading x (forward) and reading x and writing dx (backward).  A row's 16-byte packs lie on G neighbouring lanes (64 / G rows
 // per wave, NC packs per lane), the scores are summed over the G lanes with shuffles, everything in fp32; backward, a lane keeps dw of its
-// columns over all rows of the workgroup, and the workgroups' shares are joined in a fixed order.
+// columns over all rows of the workgroup, and the workgroups' shares are joined in a fixed order.  32768 x 128 in fp32, two classes: 13 us
+// forward, 20 + 7 backward, 140 a call with torch's autograd (on the tiles of many classes 317); at the copy's rate it is 3 and 7.
 template <class T, int V, int NC> struct FewRow {
     static constexpr int P = 16 / sizeof(T);
     float x[NC * P];
@@ -1258,7 +1268,8 @@ template <int P, class F> __device__ __forceinline__ void for_packs_of(const voi
     else if (dtype == NIRRT_NN_BF16) for_packs<P>((const bf16_t *)p + i0, n, f);
     else for_packs<P>((const f16_t *)p + i0, n, f);
 }
-// squares are summed in double: no overflow below the largest element squared, and the order does not matter to the last bits of the norm
+// squares are summed in double: no overflow below the largest element squared, and the order does not matter to the last bits of the norm.
+// 260 M bf16 elements: 134 us (3.9 TB/s); scaled into fp32: 286 us (5.4 TB/s, the last 256 MB read from the cache)
 __global__ __launch_bounds__(256) void k_norm_parts(TensorTable t, double *parts)
 {
     __shared__ double part[4];
