@@ -790,10 +790,13 @@ __device__ __forceinline__ float row_weight(const float *cw, int64_t t, int64_t 
 }
 
 constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
+// exp(a - b) for a <= b: the difference first, so that scores of any size (a mask of the type's lowest value) stay finite
+__device__ __forceinline__ float exp_less(float a, float b) { return __builtin_amdgcn_exp2f((a - b) * LOG2E); }
 
 // C[v, r] = w_v . x_r: a lane holds scores of NI rows r (its columns), so the running maximum and sum over the classes stay in the
 // lane; the two halves of a wave and the waves above one another meet once, at the end.  grid (row tiles, parts of the classes).  Bound by the
-// products: 8192 x 1024 x 32003 in bf16 544 us (987 TFLOP/s; the library's product alone, scores written: 499).
+// products: 8192 x 1024 x 32003 in bf16 561 us (957 TFLOP/s; the library's product alone, scores written: 499; 544 with scores in units of log2,
+// which a mask of the type's lowest value overflows).
 template <class T, int BM, int BN, class Tl>
 __global__ __launch_bounds__(Tl::NT) void k_ce_stats(Operand<T> w, Operand<T> x, const T *b, const int64_t *target, int rows, int classes,
                                                            int k, int part, float2 *stats, float *target_score)
@@ -801,9 +804,9 @@ __global__ __launch_bounds__(Tl::NT) void k_ce_stats(Operand<T> w, Operand<T> x,
     constexpr int WM = Tl::WAVES_M, WN = Tl::WAVES_N;
     __shared__ u32x4 lds[Tl::LDS_CHUNKS];
     __shared__ float2 meet[2 * WM][BN];
-    __shared__ __attribute__((aligned(16))) float add[BM];   // log2(e) b of the tile's classes, -inf behind the last
+    __shared__ __attribute__((aligned(16))) float add[BM];   // b of the tile's classes, -inf behind the last
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r0 = blockIdx.x * BN, top_row = Tl::row(wave, lane, 0, 0);
-    float m[Tl::NI], s[Tl::NI], mine[Tl::NI];                 // everything in units of log2: one fma and one exp2 per score
+    float m[Tl::NI], s[Tl::NI], mine[Tl::NI];
     int tg[Tl::NI];
 #pragma unroll
     for (int ni = 0; ni < Tl::NI; ni++) {
@@ -817,7 +820,7 @@ __global__ __launch_bounds__(Tl::NT) void k_ce_stats(Operand<T> w, Operand<T> x,
     for (int v0 = blockIdx.y * part; v0 < v_end; v0 += BM) {
         Tl t;
         __syncthreads();                                     // (the tile before has been added)
-        for (int c = threadIdx.x; c < BM; c += Tl::NT) add[c] = v0 + c < v_end ? (b ? LOG2E * (float)b[v0 + c] : 0.f) : -__builtin_inff();
+        for (int c = threadIdx.x; c < BM; c += Tl::NT) add[c] = v0 + c < v_end ? (b ? (float)b[v0 + c] : 0.f) : -__builtin_inff();
         t.mainloop(w, x, v0, r0, 0, k, lds);
         if (k == 0) __syncthreads();                         // (otherwise the products' barriers stand between)
 #pragma unroll
@@ -828,7 +831,7 @@ __global__ __launch_bounds__(Tl::NT) void k_ce_stats(Operand<T> w, Operand<T> x,
 #pragma unroll
                 for (int ni = 0; ni < Tl::NI; ni++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) t.acc[mi][ni][4 * q + e] = __builtin_fmaf(t.acc[mi][ni][4 * q + e], LOG2E, bb[e]);
+                    for (int e = 0; e < 4; e++) t.acc[mi][ni][4 * q + e] += bb[e];
             }
 #pragma unroll
         for (int ni = 0; ni < Tl::NI; ni++) {
@@ -849,8 +852,8 @@ __global__ __launch_bounds__(Tl::NT) void k_ce_stats(Operand<T> w, Operand<T> x,
 #pragma unroll
             for (int mi = 0; mi < Tl::MI; mi++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) sum[e & 3] += __builtin_amdgcn_exp2f(t.acc[mi][ni][e] - ref);
-            s[ni] = s[ni] * __builtin_amdgcn_exp2f(m[ni] - ref) + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+                for (int e = 0; e < 16; e++) sum[e & 3] += exp_less(t.acc[mi][ni][e], ref);
+            s[ni] = s[ni] * exp_less(m[ni], ref) + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
             m[ni] = top;
         }
     }
@@ -860,7 +863,7 @@ __global__ __launch_bounds__(Tl::NT) void k_ce_stats(Operand<T> w, Operand<T> x,
         const int in = tg[ni] - (int)blockIdx.y * part;
         if (tg[ni] >= 0 && in >= 0 && tg[ni] < v_end) {
             const int at = in % BM - top_row;
-            if (at >= 0 && at < Tl::MI * 32 && (at & 7) < 4) target_score[r0 + Tl::col(wave, lane, ni)] = mine[ni] * LN2;
+            if (at >= 0 && at < Tl::MI * 32 && (at & 7) < 4) target_score[r0 + Tl::col(wave, lane, ni)] = mine[ni];
         }
     }
 #pragma unroll
@@ -872,14 +875,14 @@ __global__ __launch_bounds__(Tl::NT) void k_ce_stats(Operand<T> w, Operand<T> x,
         for (int p = 0; p < 2 * WM; p++) top = fmaxf(top, meet[p][c].x);
         const float ref = top == -__builtin_inff() ? 0.f : top;
 #pragma unroll
-        for (int p = 0; p < 2 * WM; p++) sum += meet[p][c].y * __builtin_amdgcn_exp2f(meet[p][c].x - ref);
+        for (int p = 0; p < 2 * WM; p++) sum += meet[p][c].y * exp_less(meet[p][c].x, ref);
         if (r0 + c < rows) stats[(int64_t)blockIdx.y * rows + r0 + c] = make_float2(top, sum);
     }
 }
-// parts of a row's statistics (eight lanes per row) -> lse, weighted loss; the block's sums of loss and weight (in double) for k_ce_total
+// parts of a row's statistics (eight lanes per row) -> lse = (largest score, log of the sum of exp(l - it)), weighted loss; the block's sums of loss and weight (in double) for k_ce_total
 constexpr int CE_ROWS = 32;
 __global__ __launch_bounds__(256) void k_ce_rows(const float2 *stats, int parts, const float *target_score, const int64_t *target, const float *cw,
-                                                 int64_t ignore, int rows, int classes, float *lse, float *nll, double *sums)
+                                                 int64_t ignore, int rows, int classes, float2 *lse, float *nll, double *sums)
 {
     __shared__ double part[2][4];
     const int r = blockIdx.x * CE_ROWS + threadIdx.x / 8, p0 = threadIdx.x & 7;
@@ -889,21 +892,21 @@ __global__ __launch_bounds__(256) void k_ce_rows(const float2 *stats, int parts,
         for (int p = p0; p < parts; p += 8) {
             const float2 q = stats[(int64_t)p * rows + r];
             const float hi = fmaxf(top, q.x), ref = hi == -__builtin_inff() ? 0.f : hi;
-            sum = sum * __builtin_amdgcn_exp2f(top - ref) + q.y * __builtin_amdgcn_exp2f(q.x - ref);
+            sum = sum * exp_less(top, ref) + q.y * exp_less(q.x, ref);
             top = hi;
         }
 #pragma unroll
     for (int d = 1; d < 8; d <<= 1) {
         const float t2 = __shfl_xor(top, d), s2 = __shfl_xor(sum, d), hi = fmaxf(top, t2), ref = hi == -__builtin_inff() ? 0.f : hi;
-        sum = sum * __builtin_amdgcn_exp2f(top - ref) + s2 * __builtin_amdgcn_exp2f(t2 - ref);
+        sum = sum * exp_less(top, ref) + s2 * exp_less(t2, ref);
         top = hi;
     }
     if (r < rows && p0 == 0) {
-        const float l = (top + __builtin_amdgcn_logf(sum)) * LN2;
+        const float l = __builtin_amdgcn_logf(sum) * LN2;
         const int64_t t = target[r];
         const float wt = row_weight(cw, t, ignore, classes);
-        const float loss = t == ignore ? 0.f : (wt == wt ? wt * (l - target_score[r]) : wt);
-        lse[r] = l;
+        const float loss = t == ignore ? 0.f : (wt == wt ? wt * ((top - target_score[r]) + l) : wt);
+        lse[r] = make_float2(top, l);
         nll[r] = loss;
         a = loss;
         b = wt;
@@ -972,7 +975,7 @@ __global__ __launch_bounds__(256) void k_ce_scale(const float *tops, int blocks,
         scale[1] = usable ? 1.f / top : 1.f;
     }
 }
-// g' = c_r / scale (exp(l - lse_r) - [v = target]) FACTOR in the element type, stored (v, r): the product C[v, r] again.  16-bit products
+// g' = c_r / scale (exp(l - lse_r) - [v = target]), lse in its two parts, FACTOR in the element type, stored (v, r): the product C[v, r] again.  16-bit products
 // need 16-bit operands; c / scale <= 1 keeps the range, and FACTOR 4096 in f16 lifts probabilities of large vocabularies (1e-5) out of
 // its subnormals.  A rounding is off by 2^-8 (bf16), 2^-11 (f16) of the element at most, like the rounding of dz in the linear layer.
 // The scores are multiplied out again rather than kept: at 1024 inputs in bf16 that costs 2 ps per score, writing and reading them in 32 bits
@@ -984,7 +987,8 @@ template <class T> struct EpiSoftmaxGrad {
     T *g;
     int64_t ldg;
     const T *b;
-    const float *lse, *coef, *scale;
+    const float2 *lse;
+    const float *coef, *scale;
     const int64_t *target;
     int64_t v0;
     int rows;
@@ -992,7 +996,9 @@ template <class T> struct EpiSoftmaxGrad {
     {
         const float lift = scale[1] * Factor<T>::VALUE;
         const int real = rows - j < cnt ? rows - j : cnt;        // (columns behind the last row of x pad g with zeros)
-        const f32x4 l = load4(lse + j, real), w = load4(coef + j, real);
+        const float *rows_lse = (const float *)(lse + j);
+        const f32x4 la = load4(rows_lse, 2 * real < 4 ? 2 * real : 4), lb = load4(rows_lse + 4, 2 * real - 4), w = load4(coef + j, real);
+        const float top[4] = {la[0], la[2], lb[0], lb[2]}, rest[4] = {la[1], la[3], lb[1], lb[3]};
         int64_t t[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) t[e] = e < real ? target[j + e] - v0 - i : -1;
@@ -1003,7 +1009,7 @@ template <class T> struct EpiSoftmaxGrad {
                 f32x4 o;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    float p = __expf(c[q][e] + add - l[e]);
+                    float p = __expf((c[q][e] + add - top[e]) - rest[e]);
                     if (t[e] == q * step) p -= 1.f;
                     o[e] = w[e] == 0.f ? 0.f : p * (w[e] * lift);
                 }
@@ -1077,7 +1083,7 @@ template <class T> __device__ __forceinline__ void few_weights(const T *w, int64
 }
 template <class T, int V, int NC>
 __global__ __launch_bounds__(256) void k_ce_few(const T *x, int64_t ldx, const T *w, int64_t ldw, const T *b, const int64_t *target, const float *cw,
-                                                int64_t ignore, int rows, int classes, int k, int G, float *lse, float *nll, double *sums)
+                                                int64_t ignore, int rows, int classes, int k, int G, float2 *lse, float *nll, double *sums)
 {
     extern __shared__ float few[];           // classes x kp weights, V biases
     __shared__ double part[2][4];
@@ -1102,9 +1108,9 @@ __global__ __launch_bounds__(256) void k_ce_few(const T *x, int64_t ldx, const T
                 sum += v < classes ? __expf(l[v] - ref) : 0.f;
                 if (t == v) mine = l[v];
             }
-            const float z = top + logf(sum), wt = row_weight(cw, t, ignore, classes);
-            const float loss = t == ignore ? 0.f : (wt == wt ? wt * (z - mine) : wt);
-            lse[r] = z;
+            const float z = logf(sum), wt = row_weight(cw, t, ignore, classes);
+            const float loss = t == ignore ? 0.f : (wt == wt ? wt * ((top - mine) + z) : wt);
+            lse[r] = make_float2(top, z);
             nll[r] = loss;
             a += loss;
             n += wt;
@@ -1119,7 +1125,7 @@ __global__ __launch_bounds__(256) void k_ce_few(const T *x, int64_t ldx, const T
 // sums: per workgroup its share (class, k) of dw and behind it (class) of db, fp32; dx written whole
 template <class T, int V, int NC>
 __global__ __launch_bounds__(256) void k_ce_few_backward(const T *x, int64_t ldx, const T *w, int64_t ldw, const T *b, const int64_t *target,
-                                                         const float *cw, int64_t ignore, const float *lse, const float *dloss, int stride,
+                                                         const float *cw, int64_t ignore, const float2 *lse, const float *dloss, int stride,
                                                          const float *total, T *dx, float *sums, int rows, int classes, int k, int G)
 {
     constexpr int P = FewRow<T, V, NC>::P;
@@ -1134,18 +1140,19 @@ __global__ __launch_bounds__(256) void k_ce_few_backward(const T *x, int64_t ldx
 #pragma unroll
         for (int e = 0; e < NC * P; e++) aw[v][e] = 0.f;
     }
-    struct Ahead { FewRow<T, V, NC> q; float c, z; int64_t t; } next;          // the next row travels while this one is worked on
+    struct Ahead { FewRow<T, V, NC> q; float c; float2 z; int64_t t; } next;          // the next row travels while this one is worked on
     const auto fetch = [&](int64_t r) {
         next.q.load(x + r * ldx, k, g, G, r < rows);
         next.c = r < rows ? row_coefficient(dloss, stride, total, target, cw, ignore, classes, (int)r) : 0.f;
-        next.z = r < rows ? lse[r] : 0.f;
+        next.z = r < rows ? lse[r] : make_float2(0.f, 0.f);
         next.t = r < rows ? target[r] : -1;
     };
     fetch((int64_t)blockIdx.x * per + threadIdx.x / G);
     for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < rows; r0 += gridDim.x * per) {
         const int64_t r = r0 + threadIdx.x / G;
         FewRow<T, V, NC> q = next.q;
-        const float c = next.c, z = next.z;
+        const float c = next.c;
+        const float2 z = next.z;
         const int64_t t = next.t;
         float l[V], out[NC * P];
         fetch(r + (int64_t)gridDim.x * per);
@@ -1157,7 +1164,7 @@ __global__ __launch_bounds__(256) void k_ce_few_backward(const T *x, int64_t ldx
 #pragma unroll
         for (int v = 0; v < V; v++)
             if (v < classes) {
-                const float p = __expf(l[v] - z) - (t == v ? 1.f : 0.f), gr = c == 0.f ? 0.f : p * c;
+                const float p = __expf((l[v] - z.x) - z.y) - (t == v ? 1.f : 0.f), gr = c == 0.f ? 0.f : p * c;
                 ab[v] += gr;
 #pragma unroll
                 for (int m = 0; m < NC; m++)
@@ -1396,6 +1403,8 @@ template <class T, bool RC> bool direct(const Operand<T> &o, int64_t k)
     return RC ? row_bytes <= (1 << 24) : k % Elem<T>::PER_CHUNK == 0 && row_bytes <= (1 << 22);
 }
 
+template <class Epi> constexpr bool always_whole = false;                        // its operands are always whole aligned chunks, its reduction in one part
+template <class T> constexpr bool always_whole<EpiSoftmaxGrad<T>> = true;
 template <class T, bool RCA, bool RCB, class Epi>
 int gemm(const Operand<T> &a, const Operand<T> &b, int64_t m, int64_t n, int64_t k, const Plan &p, float *partial, const Epi &epi, hipStream_t st)
 {
@@ -1407,14 +1416,19 @@ int gemm(const Operand<T> &a, const Operand<T> &b, int64_t m, int64_t n, int64_t
 #define LAUNCH(TILE, EDGE, WM, WN)                                                                                                               \
     hipLaunchKernelGGL((k_gemm<T, EDGE, EDGE, TILE<T, EDGE, EDGE, WM, WN, RCA, RCB>, Epi>), grid, dim3(64 * WM * WN), 0, st, a, b, (int)m, (int)n, \
                        (int)k, p.part, partial, epi)
-    if (edge == 256) LAUNCH(DirectTile, 256, 2, 4);
-    else if (edge == 128) { if (fast) LAUNCH(DirectTile, 128, 2, 2); else LAUNCH(Tile, 128, 2, 2); }
-    else { if (fast) LAUNCH(DirectTile, 64, 2, 2); else LAUNCH(Tile, 64, 2, 2); }
-#undef LAUNCH
-    if (p.parts > 1) {
-        const int64_t blocks = ceil_div(m * ceil_div(n, 4), 256);
-        hipLaunchKernelGGL((k_join<Epi>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, partial, p.parts, (int)m, (int)n, epi);
+    if constexpr (always_whole<Epi>) {
+        if (!fast || p.parts > 1) return -1;
     }
+    if (edge == 256) LAUNCH(DirectTile, 256, 2, 4);
+    else if (fast) { if (edge == 128) LAUNCH(DirectTile, 128, 2, 2); else LAUNCH(DirectTile, 64, 2, 2); }
+    if constexpr (!always_whole<Epi>) {
+        if (!fast) { if (edge == 128) LAUNCH(Tile, 128, 2, 2); else LAUNCH(Tile, 64, 2, 2); }
+        if (p.parts > 1) {
+            const int64_t blocks = ceil_div(m * ceil_div(n, 4), 256);
+            hipLaunchKernelGGL((k_join<Epi>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, partial, p.parts, (int)m, (int)n, epi);
+        }
+    }
+#undef LAUNCH
     return status();
 }
 
@@ -1606,7 +1620,7 @@ CeForward ce_layout(int dtype, int64_t rows, int64_t classes, int64_t k)
 }
 template <class T>
 int ce_forward_t(int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw, const void *b, const int64_t *target, const float *cw, int64_t ignore,
-                 float *lse, float *nll, float *total, int64_t rows, int64_t classes, int64_t k, char *ws, hipStream_t st)
+                 float2 *lse, float *nll, float *total, int64_t rows, int64_t classes, int64_t k, char *ws, hipStream_t st)
 {
     const CeForward l = ce_layout(dtype, rows, classes, k);
     double *sums = (double *)ws;
@@ -1672,7 +1686,7 @@ CeBackward ce_backward_layout(int dtype, int64_t rows, int64_t classes, int64_t 
 }
 template <class T>
 int ce_backward_t(int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw, const void *b, const int64_t *target, const float *cw,
-                  int64_t ignore, const float *lse, const float *dloss, int stride, const float *total, void *dx, void *dw, void *db, int64_t rows,
+                  int64_t ignore, const float2 *lse, const float *dloss, int stride, const float *total, void *dx, void *dw, void *db, int64_t rows,
                   int64_t classes, int64_t k, char *ws, hipStream_t st)
 {
     const CeBackward l = ce_backward_layout(dtype, rows, classes, k);
@@ -1827,7 +1841,7 @@ extern "C" int nirrt_nn_cross_entropy(int dtype, const void *x, int64_t ldx, con
 {
     if (!good_type(dtype) || !good_dims(rows, classes, k) || classes < 1 || !total || ldx < k || ldw < k) return -1;
     if (rows > 0 && (!target || !lse || !nll || !workspace || (k > 0 && (!x || !w)))) return -1;
-#define CALL(T) ce_forward_t<T>(dtype, x, ldx, w, ldw, b, target, class_weight, ignore_index, lse, nll, total, rows, classes, k, (char *)workspace, (hipStream_t)stream)
+#define CALL(T) ce_forward_t<T>(dtype, x, ldx, w, ldw, b, target, class_weight, ignore_index, (float2 *)lse, nll, total, rows, classes, k, (char *)workspace, (hipStream_t)stream)
     return BY_TYPE(dtype, CALL);
 #undef CALL
 }
@@ -1847,7 +1861,7 @@ extern "C" int nirrt_nn_cross_entropy_backward(int dtype, const void *x, int64_t
     if (dloss_stride != 0 && dloss_stride != 1) return -1;
     if (rows > 0 && (!target || !lse || !dloss || (k > 0 && (!x || !w)))) return -1;
 #define CALL(T)                                                                                                                                  \
-    ce_backward_t<T>(dtype, x, ldx, w, ldw, b, target, class_weight, ignore_index, lse, dloss, dloss_stride, total, dx, dw, db, rows, classes, k, \
+    ce_backward_t<T>(dtype, x, ldx, w, ldw, b, target, class_weight, ignore_index, (const float2 *)lse, dloss, dloss_stride, total, dx, dw, db, rows, classes, k, \
                      (char *)workspace, (hipStream_t)stream)
     return BY_TYPE(dtype, CALL);
 #undef CALL

@@ -9,6 +9,10 @@
 float32, bfloat16 and float16; sums are held in 32 bits and rounded once.  Tensors must live on the GPU (a CPU tensor is an error,
 there is no other implementation); rows may have any stride, other layouts are copied.  Results are the same bits for the same input
 (no atomics).  Backward passes are differentiable once.
+
+Everything can be captured into a graph; a backward pass through torch.autograd.grad, or with .backward() while no eager graph of the same
+leaves is alive (torch's accumulators of a leaf remember the stream they were made on, and adding to them from a capture ends the
+process).
 """
 import contextlib
 import ctypes as C
@@ -212,7 +216,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         with _on(x.device):
             x2, ldx = _rows(x)
             w2, ldw = _rows(w)
-            lse = torch.empty(rows, dtype=torch.float32, device=x.device)
+            lse = torch.empty(rows, 2, dtype=torch.float32, device=x.device)
             nll = torch.empty(target.shape, dtype=torch.float32, device=x.device)
             total = torch.empty(3, dtype=torch.float32, device=x.device)
             L, dt = _lib(), _TYPES[x.dtype]

@@ -268,6 +268,8 @@ class get_model(nn.Module):
 def train_step(model, optimizer, points, labels, class_weight=None, max_norm=None, fps_starts=None):
     """one optimiser step on a batch of clouds: points (B, 6, N), labels (B, N) -> (loss, norm of the gradients before clipping), scalars on
     the device.  max_norm: the gradients are scaled down to this norm (None: they are left as they are)."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("train_step: not under a graph capture (sampling draws on the host, gradients accumulate on the stream of their first use)")
     optimizer.zero_grad(set_to_none=True)
     loss = model.loss(points, labels, class_weight, fps_starts)
     loss.backward()

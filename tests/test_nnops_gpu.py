@@ -340,6 +340,36 @@ def test_cross_entropy_ignored_rows_masked_classes_and_bad_targets():
     assert torch.isfinite(nnops.linear_cross_entropy(x * 1e4, w, t, bias=b))
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [5, 19])
+def test_cross_entropy_masks_of_the_lowest_value(v, dt):
+    """a masked target (a loss near the largest number, not infinite) and a row with nothing but masked classes (as good as equal scores)"""
+    from nirrt_star_amd import nnops
+    g = gen(v)
+    rows, k, low = 66, 40, torch.finfo(dt).min
+    x, w, b = randn((rows, k), g, dt), randn((v, k), g, dt, k ** -0.5), randn((v,), g, dt)
+    t = torch.randint(0, v - 1, (rows,), generator=g, device="cuda")
+    t[3] = v - 1
+    b[v - 1] = low
+    per = nnops.linear_cross_entropy(x, w, t, bias=b, reduction="none")
+    assert torch.isfinite(per).all() and abs(float(per[3]) + low) <= 4 * U * abs(low)
+    for bias in (b, torch.full_like(b, low)):
+        leaves = [q.clone().requires_grad_(True) for q in (x, w, bias)]
+        loss = nnops.linear_cross_entropy(leaves[0], leaves[1], t, bias=leaves[2], reduction="none")
+        got = torch.autograd.grad(loss, leaves, torch.ones_like(loss))
+        # (scores 3e38 apart leave nothing of the others; 64 bits hold them to 4e22, so equal ones are equal there too)
+        p = torch.softmax(x.double() @ w.double().t() + bias.double(), 1)
+        one = torch.zeros_like(p).scatter_(1, t[:, None], 1.0)
+        gm = p - one
+        # scores to (k + 3) 2^-24 sum |x w| absolutely, exponentials and sums a few 2^-24; gm is rounded to the element type
+        eg = ((k + 3) * U * 2 * (x.double().abs() @ w.double().abs().t()) + 64 * U) * (p + one) + half(dt) * gm.abs()
+        top = gm.abs() + eg
+        within(got[0], gm @ w.double(), eg @ w.double().abs() + (v + 4) * U * (top @ w.double().abs()), dt)
+        within(got[1], gm.t() @ x.double(), eg.t() @ x.double().abs() + (rows + 4) * U * (top.t() @ x.double().abs()), dt)
+        within(got[2], gm.sum(0), eg.sum(0) + (rows + 4) * U * top.sum(0), dt)
+    assert (loss.double() - math.log(v)).abs().max() <= 16 * U * (1 + math.log(v))
+
+
 def test_cross_entropy_shapes_and_refusals():
     from nirrt_star_amd import nnops
     g = gen(4)

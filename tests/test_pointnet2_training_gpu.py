@@ -102,3 +102,23 @@ def test_a_folded_model_in_eval_mode_is_refused():
         m.loss(x, labels)
     m.train()
     assert torch.isfinite(m.loss(x, labels, None, starts))
+
+
+def test_a_capture_is_refused_before_anything_is_recorded():
+    from nirrt_star_amd.pointnet2 import train_step
+    m = _model(7)
+    x, labels, starts = _batch(1, 1100, 4)
+    opt = torch.optim.SGD(m.parameters(), lr=1.0)
+    y, side = torch.zeros(4, device="cuda"), torch.zeros(4, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError):
+            train_step(m, opt, x, labels, fps_starts=starts)
+        y.copy_(side + 1)
+    assert all(p.grad is None for p in m.parameters())
+    for _ in range(3):
+        y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert (y == 1).all()
