@@ -4,15 +4,15 @@
 //   cross entropy   softmax cross entropy of the scores x w^T + b without keeping them, and its gradients
 //   norm / scale    2-norm of many tensors, and the clipping by it
 //
-// Products of more than 32 rows run on v_mfma_f32_32x32x*: a workgroup of 4 or 8 waves owns a tile C[i, j] = sum_k A[i, k] B[j, k].  An operand is
+// Products of more than 32 rows run on MFMA (16 x 16 x 32 or 32 x 32 x 16 for 16-bit, 32 x 32 x 2 for 32-bit operands): a workgroup of 4 or 8 waves owns a tile C[i, j] = sum_k A[i, k] B[j, k].  An operand is
 // stored either with k contiguous ("KC": x, w in the forward product) or with i contiguous ("RC": w in dx = dz w, dz and x in dw = dz^T x).
 // Two tile loops: DirectTile for operands of whole aligned 16-byte chunks (memory -> LDS, a ring of four stages), Tile for all others
 // (memory -> registers -> LDS).  A lane's 16 bytes are one operand of a 16-bit MFMA (8 k) or four of a 32-bit one (4 x 1 k); the order of k
 // inside a step is the same in A and B, so the sum is the same whatever it is.  Accumulators and partial sums are fp32.
 //
 // Times are those of an MI355X that copies at 5.1 TB/s; its library's products reach 1135 - 1290 TFLOP/s (bf16) and 131 (fp32).  For 16384 x 4096 x
-// 4096 in bf16: 560 us forward (z, r and y in the epilogue: 590), 514 dx, 482 dw (1140 TFLOP/s; the library 425 - 480); under these kernels the
-// clock falls to 1.5 GHz (power), where MFMA alone reach 1313.
+// 4096 in bf16: 585 us forward with z, r and y in the epilogue, 506 dx, 476 dw (1155 TFLOP/s; the library 425 - 480 for the product); under
+// these kernels the clock falls to 1.5 GHz (power).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -48,6 +48,22 @@ __device__ __forceinline__ f32x16 mma(float, u32x4 a, u32x4 b, f32x16 c)
 {
 #pragma unroll
     for (int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
+    return c;
+}
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4_t mma16(bf16_t, u32x4 a, u32x4 b, f32x4_t c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4_t mma16(f16_t, u32x4 a, u32x4 b, f32x4_t c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4_t mma16(float, u32x4 a, u32x4 b, f32x4_t c)
+{
+#pragma unroll
+    for (int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
     return c;
 }
 
@@ -156,14 +172,18 @@ template <class T, int R, int NT, bool RC> struct Stage {
     }
 };
 
-// the tile of C that a wave holds: MI x NI blocks of 32 x 32; block register e of a lane is row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32
+// The tile of C that a wave holds: MI x NI blocks of 32 x 32, 16 registers of a lane each.  SUB = 1, one 32 x 32 MFMA: register e is row 8 (e / 4) +
+// 4 (lane / 32) + e % 4, column lane % 32.  SUB = 2, four 16 x 16 ones: row 16 (e / 8) + 4 (lane / 16) + e % 4, column 16 (e / 4 % 2) + lane % 16.
+template <int SUB> __device__ __forceinline__ int block_row(int lane, int e) { return SUB == 2 ? 16 * (e >> 3) + 4 * (lane >> 4) + (e & 3) : 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3); }
+template <int SUB> __device__ __forceinline__ int block_col(int lane, int e) { return SUB == 2 ? 16 * ((e >> 2) & 1) + (lane & 15) : lane & 31; }
 template <class T, int BM, int BN, int WM, int WN, bool RCA, bool RCB> struct Tile {
     static constexpr int NT = 64 * WM * WN, WAVES_M = WM, WAVES_N = WN, MI = BM / WM / 32, NI = BN / WN / 32;
-    static constexpr int LDS_CHUNKS = (BM + BN) * CHUNKS;
+    static constexpr int LDS_CHUNKS = (BM + BN) * CHUNKS, SUB = 1;
     f32x16 acc[MI][NI];
+    __device__ __forceinline__ float get(int mi, int ni, int e) const { return acc[mi][ni][e]; }
 
-    static __device__ __forceinline__ int row(int wave, int lane, int mi, int e) { return (wave / WN) * (BM / WM) + mi * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3); }
-    static __device__ __forceinline__ int col(int wave, int lane, int ni) { return (wave % WN) * (BN / WN) + ni * 32 + (lane & 31); }
+    static __device__ __forceinline__ int first_row(int wave) { return (wave / WN) * (BM / WM); }
+    static __device__ __forceinline__ int first_col(int wave) { return (wave % WN) * (BN / WN); }
 
     // acc = sum over k in [k0, k1) of A[i0 + ., k] B[j0 + ., k]
     __device__ __forceinline__ void mainloop(const Operand<T> &a, const Operand<T> &b, int i0, int j0, int k0, int k1, u32x4 *lds)
@@ -238,9 +258,9 @@ template <class T, int R, int NT, bool RC> struct DirectOperand {
     unsigned at[N];            // a lane's offset in a step
     int first;                 // KC: the first k of its chunk (the same in all N: rows NT / 4 apart have the same swizzle)
 
-    // 16-byte blocks of an RC row are moved by whole bank groups: 64 bytes by k mod 4 (16-bit: a transposing read takes 4 k x 64 bytes at
-    // a time), 128 bytes by k / 4 (32-bit: the halves of a wave read k 4 apart)
-    static __device__ __forceinline__ int turn(int k) { return sizeof(T) == 2 ? (R >= 128 ? (k & 3) << 2 : (k & 1) << 2) : ((k >> 2) & 1) << 3; }
+    // 16-byte blocks of an RC row are moved by whole bank groups: 64 bytes by k mod 4 and 32 by k / 8 (16-bit: a transposing read takes 4 k x 32
+    // bytes per 16 lanes, their neighbours the k 8 on), 128 bytes by k / 4 (32-bit: the halves of a wave read k 4 apart)
+    static __device__ __forceinline__ int turn(int k) { return sizeof(T) == 2 ? ((R >= 128 ? k & 3 : k & 1) << 2) | ((k >> 3) & 1) << 1 : ((k >> 2) & 1) << 3; }
 
     __device__ __forceinline__ void start(const Operand<T> &o, int r0, int k0, int k1, int tid)
     {
@@ -284,24 +304,27 @@ template <class T, int R, int NT, bool RC> struct DirectOperand {
     }
 };
 
-// reads the operands of an MFMA group (32 bytes of k, two per stage) for M blocks of 32 rows: the lane's byte offsets in the operand's part
-// of a stage, so that everything else is a constant in the instruction
+// Reads MFMA operands from an operand's part of a stage: the lane's byte offsets are kept, so that everything else is a constant in the
+// instruction.  16-bit: a stage is one MFMA's k, M is counted in blocks of 16 rows (s = 0).  32-bit: two groups s of 32 bytes of k, M blocks of 32 rows.
 template <class T, int R, bool RC, int M> struct Reader {
-    static constexpr int GROUPS = RING_CHUNKS / 2;
-    int at[RC ? M : GROUPS];
+    static constexpr bool HALF = sizeof(T) == 2;
+    int at[RC ? M : HALF ? 1 : 2];
 
     __device__ __forceinline__ void start(int row0, int lane, int where)
     {
-        if constexpr (!RC) {
+        typedef DirectOperand<T, R, 64, true> Op;
+        const int i = lane & 15;
+        if constexpr (!RC && HALF) {
+            const int r = row0 + i;
+            at[0] = where + r * RING_BYTES + ((lane >> 4) ^ ring_sw(r)) * 16;
+        } else if constexpr (!RC) {
             const int r = row0 + (lane & 31), c = (lane >> 5) ^ ring_sw(r);
 #pragma unroll
-            for (int s = 0; s < GROUPS; s++) at[s] = where + r * RING_BYTES + (c ^ (2 * s)) * 16;
+            for (int s = 0; s < 2; s++) at[s] = where + r * RING_BYTES + (c ^ (2 * s)) * 16;
         } else {
-            typedef DirectOperand<T, R, 64, true> Op;
-            const int i = lane & 15, k = sizeof(T) == 2 ? 8 * (lane >> 5) + (i >> 2) : 4 * (lane >> 5);
-            const int row = sizeof(T) == 2 ? row0 + (lane & 16) + 4 * (i & 3) : row0 + (lane & 31);
+            const int k = HALF ? 8 * (lane >> 4) + (i >> 2) : 4 * (lane >> 5), row = row0 + (HALF ? 4 * (i & 3) : lane & 31);
 #pragma unroll
-            for (int m = 0; m < M; m++) at[m] = where + k * (R * (int)sizeof(T)) + (((row + 32 * m) * (int)sizeof(T)) ^ (Op::turn(k) * 16));
+            for (int m = 0; m < M; m++) at[m] = where + k * (R * (int)sizeof(T)) + (((row + (HALF ? 16 : 32) * m) * (int)sizeof(T)) ^ (Op::turn(k) * 16));
         }
     }
     __device__ __forceinline__ u32x4 read(const u32x4 *lds, int stage, int m, int s) const
@@ -309,13 +332,12 @@ template <class T, int R, bool RC, int M> struct Reader {
 #ifdef __HIP_DEVICE_COMPILE__
         const __attribute__((address_space(3))) char *p = (const __attribute__((address_space(3))) char *)lds + stage;
         if constexpr (!RC) {
-            return *(const __attribute__((address_space(3))) u32x4 *)(p + at[s] + m * 32 * RING_BYTES);
-        } else if constexpr (sizeof(T) == 2) {
+            return *(const __attribute__((address_space(3))) u32x4 *)(p + at[HALF ? 0 : s] + m * (HALF ? 16 : 32) * RING_BYTES);
+        } else if constexpr (HALF) {
             typedef short s16x4 __attribute__((ext_vector_type(4)));
             s16x4 q[2];
 #pragma unroll
-            for (int h = 0; h < 2; h++)
-                q[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p + at[m] + (16 * s + 4 * h) * (R * 2)));
+            for (int h = 0; h < 2; h++) q[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p + at[m] + 4 * h * (R * 2)));
             u32x4 v;
             __builtin_memcpy(&v, q, 16);
             return v;
@@ -342,10 +364,19 @@ template <int left> __device__ __forceinline__ void arrive()
 template <class T, int BM, int BN, int WM, int WN, bool RCA, bool RCB> struct DirectTile {
     static constexpr int NT = 64 * WM * WN, WAVES_M = WM, WAVES_N = WN, MI = BM / WM / 32, NI = BN / WN / 32;
     static constexpr int STAGE = (BM + BN) * RING_CHUNKS, LDS_CHUNKS = STAGES * STAGE, STEP = RING_BYTES / sizeof(T);
-    f32x16 acc[MI][NI];
+    // 16-bit: 16 x 16 x 32 MFMA, FA x FB blocks.  Half the accumulator traffic of 32 x 32 x 16, which is what the clock allows under power:
+    // 2090 against 1860 TFLOP/s for nothing but MFMA of normal numbers, 1484 -> 1455 us for a training step of 16384 x 4096 x 4096.
+    static constexpr int SUB = sizeof(T) == 2 ? 2 : 1, FA = MI * SUB, FB = NI * SUB;
+    f32x16 acc[SUB == 1 ? MI : 1][SUB == 1 ? NI : 1];
+    f32x4_t acc4[SUB == 2 ? FA : 1][SUB == 2 ? FB : 1];
+    __device__ __forceinline__ float get(int mi, int ni, int e) const
+    {
+        if constexpr (SUB == 2) return acc4[2 * mi + (e >> 3)][2 * ni + ((e >> 2) & 1)][e & 3];
+        else return acc[mi][ni][e];
+    }
 
-    static __device__ __forceinline__ int row(int wave, int lane, int mi, int e) { return (wave / WN) * (BM / WM) + mi * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3); }
-    static __device__ __forceinline__ int col(int wave, int lane, int ni) { return (wave % WN) * (BN / WN) + ni * 32 + (lane & 31); }
+    static __device__ __forceinline__ int first_row(int wave) { return (wave / WN) * (BM / WM); }
+    static __device__ __forceinline__ int first_col(int wave) { return (wave % WN) * (BN / WN); }
 
     typedef DirectOperand<T, BM, NT, RCA> OpA;
     typedef DirectOperand<T, BN, NT, RCB> OpB;
@@ -356,24 +387,74 @@ template <class T, int BM, int BN, int WM, int WN, bool RCA, bool RCB> struct Di
         else ob.load(stage + BM * RING_CHUNKS, i - OpA::N, left, wave);
     }
 
+    // a step of 16-bit products: a row of FB blocks at a time.  In between, the A operand two rows on, the B operands of the next stage and the
+    // loads of three stages on (the memory pipe takes a load of a wave in 16 cycles: all of a step's at once hold up the products behind them)
+    template <int P> __device__ __forceinline__ void step(const OpA &oa, const OpB &ob, const Reader<T, BM, RCA, FA> &xa, const Reader<T, BN, RCB, FB> &xb,
+                                                          u32x4 (&fa)[4], u32x4 (&fb)[2][FB], u32x4 *lds, int now, int next, int free, int left, int wave)
+    {
+        constexpr int AT = FA % 4 ? FA * P : 0;          // where the stage's A operands begin in the ring of four registers
+#pragma unroll
+        for (int i = 0; i < FA; i++) {
+            fa[(AT + i + 2) & 3] = xa.read(lds, (i + 2 < FA ? now : next) * 16, (i + 2) % FA, 0);
+#pragma unroll
+            for (int j = 0; j < FB; j++)
+                if (j * FA / FB == i) fb[1 - P][j] = xb.read(lds, next * 16, j, 0);
+#pragma unroll
+            for (int l = 0; l < LOADS; l++)
+                if (l * FA / LOADS == i) load(oa, ob, lds + free, l, left, wave);
+            __builtin_amdgcn_sched_barrier(0);           // (left alone, the compiler reads behind the products and waits)
+#pragma unroll
+            for (int j = 0; j < FB; j++) acc4[i][j] = mma16((T)0.f, fa[(AT + i) & 3], fb[P][j], acc4[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // a step of 32-bit products: two groups of 16 bytes of k per half wave
+    __device__ __forceinline__ void step(const OpA &oa, const OpB &ob, const Reader<T, BM, RCA, FA> &xa, const Reader<T, BN, RCB, FB> &xb, u32x4 (&fa)[2][MI],
+                                         u32x4 (&fb)[2][NI], u32x4 *lds, int now, int next, int free, int left, int wave)
+    {
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int mi = 0; mi < MI; mi++) {
+                fa[1 - s][mi] = xa.read(lds, (s ? next : now) * 16, mi, 1 - s);
+#pragma unroll
+                for (int ni = 0; ni < NI; ni++)
+                    if (ni * MI / NI == mi) fb[1 - s][ni] = xb.read(lds, (s ? next : now) * 16, ni, 1 - s);
+#pragma unroll
+                for (int i = 0; i < LOADS; i++)
+                    if (i * 2 * MI / LOADS == s * MI + mi) load(oa, ob, lds + free, i, left, wave);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int ni = 0; ni < NI; ni++) acc[mi][ni] = mma((T)0.f, fa[s][mi], fb[s][ni], acc[mi][ni]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+    }
+
     __device__ __forceinline__ void mainloop(const Operand<T> &a, const Operand<T> &b, int i0, int j0, int k0, int k1, u32x4 *lds)
     {
         const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        if constexpr (SUB == 2) {
 #pragma unroll
-        for (int mi = 0; mi < MI; mi++)
+            for (int i = 0; i < FA; i++)
 #pragma unroll
-            for (int ni = 0; ni < NI; ni++)
+                for (int j = 0; j < FB; j++) acc4[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        } else {
 #pragma unroll
-                for (int e = 0; e < 16; e++) acc[mi][ni][e] = 0.f;
+            for (int mi = 0; mi < MI; mi++)
+#pragma unroll
+                for (int ni = 0; ni < NI; ni++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) acc[mi][ni][e] = 0.f;
+        }
         if (k0 >= k1) return;
         OpA oa;
         OpB ob;
         oa.start(a, i0, k0, k1, tid);
         ob.start(b, j0, k0, k1, tid);
-        Reader<T, BM, RCA, MI> xa;
-        Reader<T, BN, RCB, NI> xb;
-        xa.start((wave / WN) * (BM / WM), lane, 0);
-        xb.start((wave % WN) * (BN / WN), lane, BM * RING_BYTES);
+        Reader<T, BM, RCA, FA> xa;
+        Reader<T, BN, RCB, FB> xb;
+        xa.start(first_row(wave), lane, 0);
+        xb.start(first_col(wave), lane, BM * RING_BYTES);
         __syncthreads();                     // (a tile before this one has been read)
         int left = k1 - k0;                  // k that have not been asked for; behind the end the loads give zeros, the count stays even
 #pragma unroll
@@ -385,37 +466,48 @@ template <class T, int BM, int BN, int WM, int WN, bool RCA, bool RCB> struct Di
             left -= STEP;
         }
         arrive<LOADS>();
-        u32x4 fa[2][MI], fb[2][NI];
-#pragma unroll
-        for (int mi = 0; mi < MI; mi++) fa[0][mi] = xa.read(lds, 0, mi, 0);
-#pragma unroll
-        for (int ni = 0; ni < NI; ni++) fb[0][ni] = xb.read(lds, 0, ni, 0);
-        int now = 0;                         // this stage's place in the ring, in chunks
-        for (int k = k0; k < k1; k += STEP) {
-            const int next = now + STAGE == LDS_CHUNKS ? 0 : now + STAGE, free = now == 0 ? LDS_CHUNKS - STAGE : now - STAGE;
-            // a row of products at a time, with the operands of the next group and the loads of three stages on in between (the memory
-            // pipe takes a load of a wave in 16 cycles: all of a step's at once hold up the products behind them)
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-#pragma unroll
-                for (int mi = 0; mi < MI; mi++) {
-                    fa[1 - s][mi] = xa.read(lds, (s ? next : now) * 16, mi, 1 - s);
-#pragma unroll
-                    for (int ni = 0; ni < NI; ni++)
-                        if (ni * MI / NI == mi) fb[1 - s][ni] = xb.read(lds, (s ? next : now) * 16, ni, 1 - s);
-#pragma unroll
-                    for (int i = 0; i < LOADS; i++)
-                        if (i * 2 * MI / LOADS == s * MI + mi) load(oa, ob, lds + free, i, left, wave);
-                    __builtin_amdgcn_sched_barrier(0);      // (left alone, the compiler reads behind the products and waits)
-#pragma unroll
-                    for (int ni = 0; ni < NI; ni++) acc[mi][ni] = mma((T)0.f, fa[s][mi], fb[s][ni], acc[mi][ni]);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
+        int now = 0, next, free;             // this stage's place in the ring, in chunks; the next one's; the one that has been read
+        const auto turn = [&] {
+            next = now + STAGE == LDS_CHUNKS ? 0 : now + STAGE;
+            free = now == 0 ? LDS_CHUNKS - STAGE : now - STAGE;
+        };
+        const auto done = [&] {
             oa.next();
             ob.next();
             left -= STEP;
             arrive<LOADS>();
             now = next;
+        };
+        if constexpr (SUB == 2) {
+            u32x4 fa[4], fb[2][FB];
+            fa[0] = xa.read(lds, 0, 0, 0);
+            fa[1] = xa.read(lds, 0, 1, 0);
+#pragma unroll
+            for (int j = 0; j < FB; j++) fb[0][j] = xb.read(lds, 0, j, 0);
+            int k = k0;
+            for (; k + STEP < k1; k += 2 * STEP) {
+                turn();
+                step<0>(oa, ob, xa, xb, fa, fb, lds, now, next, free, left, wave);
+                done();
+                turn();
+                step<1>(oa, ob, xa, xb, fa, fb, lds, now, next, free, left, wave);
+                done();
+            }
+            if (k < k1) {
+                turn();
+                step<0>(oa, ob, xa, xb, fa, fb, lds, now, next, free, left, wave);
+            }
+        } else {
+            u32x4 fa[2][MI], fb[2][NI];
+#pragma unroll
+            for (int mi = 0; mi < MI; mi++) fa[0][mi] = xa.read(lds, 0, mi, 0);
+#pragma unroll
+            for (int ni = 0; ni < NI; ni++) fb[0][ni] = xb.read(lds, 0, ni, 0);
+            for (int k = k0; k < k1; k += STEP) {
+                turn();
+                step(oa, ob, xa, xb, fa, fb, lds, now, next, free, left, wave);
+                done();
+            }
         }
         arrive<0>();                         // (the loads behind the end)
     }
@@ -581,7 +673,7 @@ __global__ __launch_bounds__(Tl::NT) void k_gemm(Operand<T> a, Operand<T> b, int
     const int k0 = blockIdx.y * part, k1 = k - k0 < part ? k : k0 + part;
     t.mainloop(a, b, ti * BM, tj * BN, k0, k1, lds);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int i0 = ti * BM + Tl::row(wave, 0, 0, 0), j0 = tj * BN + Tl::col(wave, 0, 0);
+    const int i0 = ti * BM + Tl::first_row(wave), j0 = tj * BN + Tl::first_col(wave);
     float *slab = (float *)(lds + wave * SLAB);
     constexpr int PER_ROW = COLS / 4, STEP = 64 / PER_ROW, Q = 32 / STEP;     // lanes per row, rows per pass, passes
     const int r = lane / PER_ROW, c = lane % PER_ROW * 4, j = j0 + c, cnt = n - j < 4 ? n - j : 4;
@@ -592,7 +684,7 @@ __global__ __launch_bounds__(Tl::NT) void k_gemm(Operand<T> a, Operand<T> b, int
 #pragma unroll
         for (int ni = 0; ni < Tl::NI; ni++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) slab[(8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * LD + ni * 32 + (lane & 31)] = t.acc[mi][ni][e];
+            for (int e = 0; e < 16; e++) slab[block_row<Tl::SUB>(lane, e) * LD + ni * 32 + block_col<Tl::SUB>(lane, e)] = t.get(mi, ni, e);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         f32x4 v[Q];
@@ -610,21 +702,6 @@ __global__ __launch_bounds__(Tl::NT) void k_gemm(Operand<T> a, Operand<T> b, int
 // A workgroup of eight waves owns 16 columns; each wave takes every eighth step of 64 bytes per row of w, eight steps in flight (8 KB per
 // wave: some 64 KB per CU cover the latency), multiplies them on 16 x 16 MFMA with the rows of x straight from memory, and the waves' sums
 // meet in the LDS.  One launch, nothing cut, no workspace.  7 x 4096 x 4096 in fp16: 9.8 us, 3.4 TB/s of w (a cut 64-wide tile and its join: 9 + 4 us).
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ f32x4_t mma16(bf16_t, u32x4 a, u32x4 b, f32x4_t c)
-{
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4_t mma16(f16_t, u32x4 a, u32x4 b, f32x4_t c)
-{
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4_t mma16(float, u32x4 a, u32x4 b, f32x4_t c)
-{
-#pragma unroll
-    for (int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
-    return c;
-}
 template <class T> __device__ __forceinline__ u32x4 chunk_of(const T *row, int at, int k)
 {
     constexpr int P = 16 / sizeof(T);
@@ -795,26 +872,26 @@ __device__ __forceinline__ float exp_less(float a, float b) { return __builtin_a
 
 // C[v, r] = w_v . x_r: a lane holds scores of NI rows r (its columns), so the running maximum and sum over the classes stay in the
 // lane; the two halves of a wave and the waves above one another meet once, at the end.  grid (row tiles, parts of the classes).  Bound by the
-// products: 8192 x 1024 x 32003 in bf16 561 us (957 TFLOP/s; the library's product alone, scores written: 499; 544 with scores in units of log2,
-// which a mask of the type's lowest value overflows).
+// products: 8192 x 1024 x 32003 in bf16 537 us (1000 TFLOP/s; the library's product alone, scores written: 499).
 template <class T, int BM, int BN, class Tl>
 __global__ __launch_bounds__(Tl::NT) void k_ce_stats(Operand<T> w, Operand<T> x, const T *b, const int64_t *target, int rows, int classes,
                                                            int k, int part, float2 *stats, float *target_score)
 {
-    constexpr int WM = Tl::WAVES_M, WN = Tl::WAVES_N;
+    constexpr int WM = Tl::WAVES_M, WN = Tl::WAVES_N, SUB = Tl::SUB, NC = Tl::NI * SUB, WIDE = 32 / SUB, GROUPS = 64 / WIDE;   // NC: a lane's columns
     __shared__ u32x4 lds[Tl::LDS_CHUNKS];
-    __shared__ float2 meet[2 * WM][BN];
+    __shared__ float2 meet[GROUPS * WM][BN];
     __shared__ __attribute__((aligned(16))) float add[BM];   // b of the tile's classes, -inf behind the last
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r0 = blockIdx.x * BN, top_row = Tl::row(wave, lane, 0, 0);
-    float m[Tl::NI], s[Tl::NI], mine[Tl::NI];
-    int tg[Tl::NI];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r0 = blockIdx.x * BN, top_row = Tl::first_row(wave) + block_row<SUB>(lane, 0);
+    const int col0 = Tl::first_col(wave) + (lane & (WIDE - 1));
+    float m[NC], s[NC], mine[NC];
+    int tg[NC];
 #pragma unroll
-    for (int ni = 0; ni < Tl::NI; ni++) {
-        m[ni] = -__builtin_inff();
-        s[ni] = mine[ni] = 0.f;
-        const int r = r0 + Tl::col(wave, lane, ni);
+    for (int c = 0; c < NC; c++) {
+        m[c] = -__builtin_inff();
+        s[c] = mine[c] = 0.f;
+        const int r = r0 + col0 + c * WIDE;
         const int64_t t = r < rows ? target[r] : -1;
-        tg[ni] = t >= 0 && t < classes ? (int)t : -1;
+        tg[c] = t >= 0 && t < classes ? (int)t : -1;
     }
     const int v_end = classes - (int)blockIdx.y * part < part ? classes : ((int)blockIdx.y + 1) * part;
     for (int v0 = blockIdx.y * part; v0 < v_end; v0 += BM) {
@@ -824,58 +901,53 @@ __global__ __launch_bounds__(Tl::NT) void k_ce_stats(Operand<T> w, Operand<T> x,
         t.mainloop(w, x, v0, r0, 0, k, lds);
         if (k == 0) __syncthreads();                         // (otherwise the products' barriers stand between)
 #pragma unroll
-        for (int mi = 0; mi < Tl::MI; mi++)
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const f32x4 bb = *(const f32x4 *)(add + top_row + mi * 32 + 8 * q);
-#pragma unroll
-                for (int ni = 0; ni < Tl::NI; ni++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) t.acc[mi][ni][4 * q + e] += bb[e];
-            }
-#pragma unroll
-        for (int ni = 0; ni < Tl::NI; ni++) {
-            float top = m[ni];
+        for (int c = 0; c < NC; c++) {
+            // the lane's scores of the column: four classes at a time
+            float l[Tl::MI * 16 / SUB];
 #pragma unroll
             for (int mi = 0; mi < Tl::MI; mi++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) top = fmaxf(top, t.acc[mi][ni][e]);
+                for (int q = 0; q < 4 / SUB; q++) {
+                    const int e0 = SUB == 2 ? 8 * q + 4 * (c & 1) : 4 * q;
+                    const f32x4 bb = *(const f32x4 *)(add + top_row + mi * 32 + block_row<SUB>(0, e0));
+#pragma unroll
+                    for (int e = 0; e < 4; e++) l[(mi * 4 / SUB + q) * 4 + e] = t.get(mi, c / SUB, e0 + e) + bb[e];
+                }
+            float top = m[c];
+#pragma unroll
+            for (int e = 0; e < Tl::MI * 16 / SUB; e++) top = fmaxf(top, l[e]);
             const float ref = top == -__builtin_inff() ? 0.f : top;   // (nothing but -inf so far: exp(-inf) adds zeros)
-            const int want = tg[ni] - v0 - top_row;
-            if (__ballot(tg[ni] >= v0 && tg[ni] < v0 + BM)) {         // a row of this wave has its target in the tile
+            const int want = tg[c] - v0 - top_row;
+            if (__ballot(tg[c] >= v0 && tg[c] < v0 + BM)) {           // a row of this wave has its target in the tile
 #pragma unroll
-                for (int mi = 0; mi < Tl::MI; mi++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) mine[ni] = want == mi * 32 + 8 * (e >> 2) + (e & 3) ? t.acc[mi][ni][e] : mine[ni];
+                for (int e = 0; e < Tl::MI * 16 / SUB; e++) mine[c] = want == 8 * SUB * (e >> 2) + (e & 3) ? l[e] : mine[c];
             }
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int mi = 0; mi < Tl::MI; mi++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) sum[e & 3] += exp_less(t.acc[mi][ni][e], ref);
-            s[ni] = s[ni] * exp_less(m[ni], ref) + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-            m[ni] = top;
+            for (int e = 0; e < Tl::MI * 16 / SUB; e++) sum[e & 3] += exp_less(l[e], ref);
+            s[c] = s[c] * exp_less(m[c], ref) + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+            m[c] = top;
         }
     }
-    // the lane that met a row's target leaves its score: its share of the classes holds 4-row groups 8 apart from its own row on
+    // the lane that met a row's target leaves its score: its share of the classes holds 4-row groups 8 SUB apart from its own row on
 #pragma unroll
-    for (int ni = 0; ni < Tl::NI; ni++) {
-        const int in = tg[ni] - (int)blockIdx.y * part;
-        if (tg[ni] >= 0 && in >= 0 && tg[ni] < v_end) {
+    for (int c = 0; c < NC; c++) {
+        const int in = tg[c] - (int)blockIdx.y * part;
+        if (tg[c] >= 0 && in >= 0 && tg[c] < v_end) {
             const int at = in % BM - top_row;
-            if (at >= 0 && at < Tl::MI * 32 && (at & 7) < 4) target_score[r0 + Tl::col(wave, lane, ni)] = mine[ni];
+            if (at >= 0 && at < Tl::MI * 32 && (at & (8 * SUB - 1)) < 4) target_score[r0 + col0 + c * WIDE] = mine[c];
         }
     }
 #pragma unroll
-    for (int ni = 0; ni < Tl::NI; ni++) meet[2 * (wave / WN) + (lane >> 5)][Tl::col(wave, lane, ni)] = make_float2(m[ni], s[ni]);
+    for (int c = 0; c < NC; c++) meet[GROUPS * (wave / WN) + lane / WIDE][col0 + c * WIDE] = make_float2(m[c], s[c]);
     __syncthreads();
     for (int c = threadIdx.x; c < BN; c += Tl::NT) {
         float top = -__builtin_inff(), sum = 0.f;
 #pragma unroll
-        for (int p = 0; p < 2 * WM; p++) top = fmaxf(top, meet[p][c].x);
+        for (int p = 0; p < GROUPS * WM; p++) top = fmaxf(top, meet[p][c].x);
         const float ref = top == -__builtin_inff() ? 0.f : top;
 #pragma unroll
-        for (int p = 0; p < 2 * WM; p++) sum += meet[p][c].y * exp_less(meet[p][c].x, ref);
+        for (int p = 0; p < GROUPS * WM; p++) sum += meet[p][c].y * exp_less(meet[p][c].x, ref);
         if (r0 + c < rows) stats[(int64_t)blockIdx.y * rows + r0 + c] = make_float2(top, sum);
     }
 }
