@@ -47,8 +47,8 @@ def listed():
         _ce("classes_odd", 513, 771, 5003, "fp16", True, False),
         # a large set of classes: the logits alone would be a gigabyte in 32 bits
         _ce("many_classes", 8192, 1024, 32003, "bf16", False, False),
-        # the gradients of the guidance network (1.9 M parameters in 138 tensors)
-        _clip("net_gradients", 138, 1880000, "fp32", "fp32"),
+        # the gradients of the guidance network (1.9 M parameters in 132 tensors)
+        _clip("net_gradients", 132, 1880000, "fp32", "fp32"),
         # half-precision gradients of a large model, clipped into 32-bit ones
         _clip("large_gradients", 300, 260000000, "bf16", "fp32"),
     ]
