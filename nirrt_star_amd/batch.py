@@ -565,6 +565,17 @@ class Guidance:
         return out
 
 
+def _refuse_two_threads(trees):
+    """The two schedules of a guided batch that keep a persistent launch on one thread while another refreshes clouds have ended
+    full-size runs with corrupted trees and with GPU memory faults, from a cause that is not known: refused for trees on a device (the
+    host logic alone can still be driven with stand-ins)."""
+    asked = [k for k, on in (("NIRRT_BATCH_OVERLAP", os.environ.get("NIRRT_BATCH_OVERLAP", "0") == "1"),
+                             ("NIRRT_BATCH_GROUPS", int(os.environ.get("NIRRT_BATCH_GROUPS", "1")) > 1)) if on]
+    if asked and any(isinstance(t, _hip.HipTree) for t in trees):
+        raise RuntimeError("run_batch: %s = %s is refused: a launch on one thread with cloud refreshes on another corrupts trees and faults the GPU"
+                           % (asked[0], os.environ[asked[0]]))
+
+
 def run_batch(trees, streams, iters, flags, dim, problems=None, guidance=None, frames=None, want_trace=True, stop_first=False,
               window=65536, init_clouds=True, overlap_min=None):
     """`iters` loop bodies for every tree of the batch (fewer for trees that stop: first solution with stop_first, full
@@ -575,6 +586,8 @@ def run_batch(trees, streams, iters, flags, dim, problems=None, guidance=None, f
     irrt = bool(flags & _hip.F_IRRT)
     png = guidance is not None
     need_py = dim == 2 and irrt
+    if png:
+        _refuse_two_threads(trees)
     hand_over(trees, streams)
     run_flags = flags | (_hip.F_STOP_FIRST if stop_first else 0) | (_hip.F_PNG if png else 0)
     remaining = np.full(B, int(iters), dtype=np.int64)
@@ -689,14 +702,10 @@ def run_batch(trees, streams, iters, flags, dim, problems=None, guidance=None, f
         prof["refresh"] += time.perf_counter() - t_r
         return [i for i in act if not finished[i] and remaining[i] > 0]
 
-    # Guided runs alternate between the loop and the cloud refresh.  Round 2 split a large batch into two halves so that one
-    # half's (host-side) refresh overlapped the other half's launch.  With candidates, down-sampling, network input and
-    # predictions all on the device there is little host work left to hide, and the halves cost more than they gave: a half
-    # batch runs at two waves per SIMD instead of four, and PointNet++'s set-abstraction kernel (151 KB of LDS per workgroup)
-    # cannot share a CU with resident trees, so its forward waited for the other half's launch anyway.  4096 trees, 2D, 50000
-    # iterations: two halves 10.4 M it/s; one group 11.1 M (window 4096), 16.6 M (2048), 19.6 M (1024), 18.2 M (768), 16.1 M (512).
-    # NIRRT_BATCH_GROUPS / NIRRT_BATCH_INFLIGHT bring the split back (groups launched from worker threads; the C call releases
-    # the GIL); trees are independent and draw from their own generators, so no grouping changes a result.
+    # Guided runs alternate between the loop and the cloud refresh: one group, one thread.  (Two halves whose refreshes overlap the other
+    # half's launch: 10.4 M it/s on 4096 trees, 2D, 50000 iterations; one group 11.1 M with 4096-iteration launches, 16.6 M with 2048, 19.6 M
+    # with 1024, 18.2 M with 768, 16.1 M with 512.)  NIRRT_BATCH_GROUPS / _INFLIGHT split the batch into groups that worker threads
+    # launch, NIRRT_BATCH_OVERLAP=1 refreshes due trees while the others run: both are refused for trees on a device (_refuse_two_threads).
     if overlap_min is None:
         overlap_min = int(os.environ.get("NIRRT_BATCH_OVERLAP_MIN", "1024"))   # trees per group when splitting; tests set 1
     # iterations per persistent launch: a tree whose cloud is due idles in its slot until the launch ends, so guided runs take
@@ -706,16 +715,8 @@ def run_batch(trees, streams, iters, flags, dim, problems=None, guidance=None, f
     window = int(os.environ.get("NIRRT_BATCH_WINDOW", window))
     n_groups = max(1, int(os.environ.get("NIRRT_BATCH_GROUPS", "1"))) if (png and B >= 2 * overlap_min) else 1
     in_flight = max(1, min(max(1, n_groups - 1), int(os.environ.get("NIRRT_BATCH_INFLIGHT", "1"))))   # launches on the device at once
-    # Overlapped refresh (round 6, one group, NIRRT_BATCH_OVERLAP=1; OFF by default): the trees whose cloud is due sit a launch out -
-    # the others are launched again at once, and the due trees' clouds (candidates, down-sampling, PointNet++ forward: device work
-    # on other streams + host bookkeeping) are made WHILE that launch runs; they join the launch after.  Nobody's results depend
-    # on launch boundaries.  Measured at pc_update_cost_ratio = 1.0 (demo_planning_3d.py:21; 2048 3D trees, profiles/README_r06.md):
-    # the refreshes are hidden (35 of 36 s), but the launches share the GPU with them and take 25.6 s instead of 14.6 s, and the
-    # smaller due sets mean more refreshes, each as long as its slowest cloud: 45.4 s per step against 43.5 s one after the other.
-    # AND IT IS NOT SAFE ON THIS STACK: like NIRRT_BATCH_GROUPS >= 2 (a persistent launch on one thread, refresh work on another) it
-    # ended full-size runs with trees whose best cost was below the straight start-goal distance, or with a GPU memory fault
-    # (gpurun_out of round 6: ov_full, c4r10_p25_g2) - small runs pass.  Both stay available for whoever hunts that down; nothing
-    # in the library turns them on.
+    # Overlapped refresh: the trees whose cloud is due sit a launch out and join the one after; nobody's results depend on launch
+    # boundaries.  (At pc_update_cost_ratio = 1.0, 2048 3D trees: 45.4 s per step against 43.5 s one after the other.)
     overlap = png and n_groups == 1 and B > 1 and os.environ.get("NIRRT_BATCH_OVERLAP", "0") == "1"
     if overlap:
         active = list(range(B))

@@ -441,3 +441,16 @@ def test_guided_windows_are_paced_by_each_trees_own_speed(dev, monkeypatch):
         assert second[4] == 1024 // 8                              # ... but never fewer than an eighth of the window
         assert len(log) > 3                                        # the slow trees catch up over more launches
         assert log[-1]["names"] == [4]
+
+
+@pytest.mark.parametrize("setting", [{"NIRRT_BATCH_OVERLAP": "1"}, {"NIRRT_BATCH_GROUPS": "2"}])
+def test_two_thread_schedules_are_refused_for_trees_on_a_device(dev, monkeypatch, setting):
+    for k, v in setting.items():
+        monkeypatch.setenv(k, v)
+    monkeypatch.setattr(_hip, "run_sampling", lambda *a, **k: pytest.fail("launched"))
+    tree = object.__new__(_hip.HipTree)
+    tree.device_id, tree.h = 0, None
+    g = FakeGuidance()
+    with pytest.raises(RuntimeError, match="refused"):
+        batch.run_batch([tree], [batch.ProblemStreams(0)], 3000, _hip.F_IRRT, 2, problems=[{}], guidance=g, frames=[None])
+    assert not g.calls and not dev.set_calls
