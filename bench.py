@@ -517,22 +517,21 @@ def secondary_runs(args):
     """Short driver-witnessed lines of the other BASELINE configurations (RRT* 2D / 3D, IRRT* 3D, the r in [16, 24] world, configs
     3 and 4): one step each, no warm-up, same iteration count; the fields a reader needs to judge them."""
     out = {}
+    ended = None                    # what ended badly: nothing more is started on the GPU behind it, and it is not tried again
     for label, extra in SECONDARY:
+        if ended:
+            out[label] = {"error": "not run: '%s' ended badly" % ended}
+            continue
         ttfs = "--ttfs" in extra
         cmd = [sys.executable, os.path.abspath(__file__), "--steps", "1", "--warmup", "0", "--iters", str(args.iters),
                "--no-cpu-baseline", "--no-secondary", "--no-single"] + ([] if ttfs else ["--no-ttfs"]) + list(extra)
         t0 = time.perf_counter()
         try:
-            first_error = None
-            for attempt in (0, 1):      # (one retry: a line that dies says so in `retried_after` and gets a second chance at a number)
-                p = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True, timeout=900)
-                line = [l for l in p.stdout.splitlines() if l.startswith("{")]
-                if p.returncode == 0 and line:
-                    break
-                err = "rc %d: %s" % (p.returncode, ([l for l in p.stderr.strip().splitlines() if "amdgpu.ids" not in l] or ["no output"])[-1][:160])
-                first_error = first_error or err
+            p = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True, timeout=900)
+            line = [l for l in p.stdout.splitlines() if l.startswith("{")]
             if p.returncode != 0 or not line:
-                out[label] = {"error": first_error}
+                out[label] = {"error": "rc %d: %s" % (p.returncode, ([l for l in p.stderr.strip().splitlines() if "amdgpu.ids" not in l] or ["no output"])[-1][:160])}
+                ended = label
                 continue
             d = json.loads(line[-1])
             cfg, rf = d["config"], d["roofline"]
@@ -545,10 +544,9 @@ def secondary_runs(args):
                           "kernel_share_of_step": rf.get("kernel_share_of_step"), "time_to_first_solution": d.get("time_to_first_solution"),
                           "workload": cfg.get("workload"),
                           "warning": d.get("warning"), "wall_s": time.perf_counter() - t0}
-            if first_error:
-                out[label]["retried_after"] = first_error
         except subprocess.TimeoutExpired:
             out[label] = {"error": "timed out after 900 s"}
+            ended = label
     return out
 
 
@@ -567,7 +565,7 @@ def compact(v):
     t = v.get("time_to_first_solution")
     if t and t["single"]["median_seconds"] is not None and t["batch"]["median_seconds"] is not None:
         c["ttfs_ms"] = [round(t["single"]["median_seconds"] * 1e3, 2), round(t["batch"]["median_seconds"] * 1e3, 2)]
-    for k in ("resumed_s", "problems", "retried_after"):
+    for k in ("resumed_s", "problems"):
         if k in v:
             c[k] = v[k]
     if v.get("trees_stopped_early"):

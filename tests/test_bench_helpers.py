@@ -147,3 +147,23 @@ def test_scale_script_dry_run_collects_and_checks_every_line(tmp_path):
     (bad / "weak_2.json").write_text(json.dumps(d))
     r2 = subprocess.run([sys.executable, os.path.join(ROOT, "scripts", "scale_check.py"), str(bad)], capture_output=True, text=True)
     assert r2.returncode == 1 and "3 ranks answered" in r2.stdout
+
+
+@pytest.mark.parametrize("how", ["status", "time"])
+def test_a_secondary_line_that_ends_badly_is_not_tried_again_and_ends_the_others(monkeypatch, how):
+    from types import SimpleNamespace as NS
+    m = _bench()
+    started = []
+
+    def run(cmd, **kw):
+        started.append(cmd)
+        if how == "time":
+            raise subprocess.TimeoutExpired(cmd, 900)
+        return NS(returncode=-6, stdout="", stderr="Memory access fault")
+
+    monkeypatch.setattr(m.subprocess, "run", run)
+    out = m.secondary_runs(NS(iters=100))
+    assert len(started) == 1 and len(out) == len(m.SECONDARY)
+    labels = [label for label, _ in m.SECONDARY]
+    assert ("rc -6" if how == "status" else "timed out") in out[labels[0]]["error"]
+    assert all("not run" in out[label]["error"] for label in labels[1:])
