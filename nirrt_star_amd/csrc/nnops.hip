@@ -1457,6 +1457,9 @@ int64_t plan_bytes(const Plan &p, int64_t m, int64_t n) { return p.parts > 1 ? r
 double copy_us(int dtype, int64_t rows, int64_t k) { return 4. + (double)rows * k * 2 * elem_size(dtype) / 3e6; }
 int64_t padded(int dtype, int64_t k) { const int64_t c = 16 / elem_size(dtype); return (k + c - 1) / c * c; }
 bool whole_rows(int dtype, const void *p, int64_t ld, int64_t k) { return (uintptr_t)p % 16 == 0 && ld * elem_size(dtype) % 16 == 0 && k == padded(dtype, k); }
+// ... and no further apart than direct() takes as rows of a KC operand (the last token of every sequence lies a sequence apart)
+constexpr int64_t KC_ROW_BYTES = 1 << 22;
+bool near_whole_rows(int dtype, const void *p, int64_t ld, int64_t k) { return whole_rows(dtype, p, ld, k) && ld * elem_size(dtype) <= KC_ROW_BYTES; }
 bool aligned_rows(int dtype, const void *p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld * elem_size(dtype) % 16 == 0; }
 template <class T>
 void copy_rows(const void *x, int64_t ldx, const float *coef, T *out, int64_t ld, int64_t rows, int64_t rows_out, int64_t k, hipStream_t st)
@@ -1472,7 +1475,7 @@ template <class T, bool RC> bool direct(const Operand<T> &o, int64_t k)
 {
     const int64_t row_bytes = o.ld * (int64_t)sizeof(T);
     if ((uintptr_t)o.p % 16 || row_bytes % 16) return false;
-    return RC ? row_bytes <= (1 << 24) : k % Elem<T>::PER_CHUNK == 0 && row_bytes <= (1 << 22);
+    return RC ? row_bytes <= (1 << 24) : k % Elem<T>::PER_CHUNK == 0 && row_bytes <= KC_ROW_BYTES;
 }
 
 template <class Epi> constexpr bool always_whole = false;                        // its operands are always whole aligned chunks, its reduction in one part
@@ -1668,7 +1671,7 @@ bool few_layout(int dtype, int64_t rows, int64_t classes, int64_t k, Few &f)
 #define FEW_ONE(KERNEL, V, NC, BLOCKS, LDS, ...) hipLaunchKernelGGL((KERNEL<T, V, NC>), dim3((unsigned)BLOCKS), dim3(256), LDS, st, __VA_ARGS__)
 
 // cross entropy: tile edge, and parts of the classes so that row tiles x parts fill the GPU; x and w whose rows are no whole aligned chunks
-// are copied into such (k_rows_copy): the products read them many times
+// or lie far apart are copied into such that are not (k_rows_copy): the products read them many times
 struct CeForward { int edge, parts, part; int64_t stats, score, sums, xs, ws, total; };
 CeForward ce_layout(int dtype, int64_t rows, int64_t classes, int64_t k)
 {
@@ -1708,11 +1711,10 @@ int ce_forward_t(int dtype, const void *x, int64_t ldx, const void *w, int64_t l
     } else if (rows > 0) {
         blocks = ceil_div(rows, CE_ROWS);
         const int64_t kp = padded(dtype, k), row_tiles = ceil_div(rows, l.edge);
-        if (!whole_rows(dtype, x, ldx, k)) { copy_rows(x, ldx, nullptr, xs, kp, rows, rows, k, st); x = xs; ldx = kp; }
-        if (!whole_rows(dtype, w, ldw, k)) { copy_rows(w, ldw, nullptr, wsp, kp, classes, classes, k, st); w = wsp; ldw = kp; }
+        if (!near_whole_rows(dtype, x, ldx, k)) { copy_rows(x, ldx, nullptr, xs, kp, rows, rows, k, st); x = xs; ldx = kp; }
+        if (!near_whole_rows(dtype, w, ldw, k)) { copy_rows(w, ldw, nullptr, wsp, kp, classes, classes, k, st); w = wsp; ldw = kp; }
         const dim3 grid((unsigned)row_tiles, (unsigned)l.parts);
         const Operand<T> ow = op((const T *)w, ldw, classes), ox = op((const T *)x, ldx, rows);
-        if (!direct<T, false>(ow, kp) || !direct<T, false>(ox, kp)) return -1;   // (rows of more than 4 MB)
 #define LAUNCH(EDGE, WM, WN)                                                                                                                \
     hipLaunchKernelGGL((k_ce_stats<T, EDGE, EDGE, DirectTile<T, EDGE, EDGE, WM, WN, false, false>>), grid, dim3(64 * WM * WN), 0, st, ow, ox, \
                        (const T *)b, target, (int)rows, (int)classes, (int)kp, l.part, stats, score)
@@ -1780,7 +1782,7 @@ int ce_backward_t(int dtype, const void *x, int64_t ldx, const void *w, int64_t 
         hipLaunchKernelGGL(k_ce_coefficients, dim3((unsigned)blocks), dim3(256), 0, st, dloss, stride, total, target, cw, ignore, (int)rows, (int)classes, coef, tops);
     hipLaunchKernelGGL(k_ce_scale, dim3(1), dim3(256), 0, st, tops, (int)blocks, scale);
     copy_rows(x, ldx, coef, xs, kp, rows, l.ldg, k, st);
-    if (!whole_rows(dtype, w, ldw, k)) { copy_rows(w, ldw, nullptr, wsp, kp, classes, classes, k, st); w = wsp; ldw = kp; }
+    if (!near_whole_rows(dtype, w, ldw, k)) { copy_rows(w, ldw, nullptr, wsp, kp, classes, classes, k, st); w = wsp; ldw = kp; }
     const float unlift = 1.f / Factor<T>::VALUE;
     for (int64_t v0 = 0; v0 < classes; v0 += l.piece) {
         const int64_t nv = classes - v0 < l.piece ? classes - v0 : l.piece;
@@ -1901,9 +1903,14 @@ extern "C" int nirrt_nn_linear_backward(int dtype, int act, const void *x, int64
 #undef CALL
 }
 
+static bool good_cross_entropy(int dtype, int64_t rows, int64_t classes, int64_t k)
+{
+    return good_type(dtype) && good_dims(rows, classes, k) && classes >= 1 && padded(dtype, k) * elem_size(dtype) <= KC_ROW_BYTES;
+}
+
 extern "C" int64_t nirrt_nn_cross_entropy_workspace(int dtype, int64_t rows, int64_t classes, int64_t k)
 {
-    if (!good_type(dtype) || !good_dims(rows, classes, k) || classes < 1) return -1;
+    if (!good_cross_entropy(dtype, rows, classes, k)) return -1;
     return ce_layout(dtype, rows, classes, k).total;
 }
 
@@ -1911,7 +1918,7 @@ extern "C" int nirrt_nn_cross_entropy(int dtype, const void *x, int64_t ldx, con
                                       const float *class_weight, int64_t ignore_index, float *lse, float *nll, float *total, int64_t rows,
                                       int64_t classes, int64_t k, void *workspace, void *stream)
 {
-    if (!good_type(dtype) || !good_dims(rows, classes, k) || classes < 1 || !total || ldx < k || ldw < k) return -1;
+    if (!good_cross_entropy(dtype, rows, classes, k) || !total || ldx < k || ldw < k) return -1;
     if (rows > 0 && (!target || !lse || !nll || !workspace || (k > 0 && (!x || !w)))) return -1;
 #define CALL(T) ce_forward_t<T>(dtype, x, ldx, w, ldw, b, target, class_weight, ignore_index, (float2 *)lse, nll, total, rows, classes, k, (char *)workspace, (hipStream_t)stream)
     return BY_TYPE(dtype, CALL);
@@ -1920,7 +1927,7 @@ extern "C" int nirrt_nn_cross_entropy(int dtype, const void *x, int64_t ldx, con
 
 extern "C" int64_t nirrt_nn_cross_entropy_backward_workspace(int dtype, int64_t rows, int64_t classes, int64_t k)
 {
-    if (!good_type(dtype) || !good_dims(rows, classes, k) || classes < 1) return -1;
+    if (!good_cross_entropy(dtype, rows, classes, k)) return -1;
     return ce_backward_layout(dtype, rows, classes, k).total;
 }
 
@@ -1929,7 +1936,7 @@ extern "C" int nirrt_nn_cross_entropy_backward(int dtype, const void *x, int64_t
                                                const float *dloss, int dloss_stride, const float *total, void *dx, void *dw, void *db,
                                                int64_t rows, int64_t classes, int64_t k, void *workspace, void *stream)
 {
-    if (!good_type(dtype) || !good_dims(rows, classes, k) || classes < 1 || ldx < k || ldw < k || !workspace) return -1;
+    if (!good_cross_entropy(dtype, rows, classes, k) || ldx < k || ldw < k || !workspace) return -1;
     if (dloss_stride != 0 && dloss_stride != 1) return -1;
     if (rows > 0 && (!target || !lse || !dloss || (k > 0 && (!x || !w)))) return -1;
 #define CALL(T)                                                                                                                                  \

@@ -270,6 +270,8 @@ def linear_cross_entropy(x, weight, target, bias=None, class_weight=None, ignore
                                      or class_weight.requires_grad):
         raise ValueError("%s: class_weight must be float32 (%d,) on %s, without a gradient" % (name, v, x.device))
     _sizes_ok(name, target.numel(), v, weight.shape[1])
+    if weight.shape[1] * weight.element_size() > 1 << 22:
+        raise ValueError("%s: %d inputs are more than 4 MB" % (name, weight.shape[1]))
     return _LinearCrossEntropy.apply(x, weight, bias.contiguous() if bias is not None else None, target.contiguous(),
                                      class_weight.contiguous() if class_weight is not None else None, int(ignore_index), reduction)
 

@@ -1,0 +1,17 @@
+"""CPU: calls of nirrt_star_amd.nnops that are refused, or that are decided before anything is launched."""
+import ctypes as C
+
+import pytest
+import torch
+
+
+def test_cross_entropy_refuses_rows_of_more_than_4_mb():
+    from nirrt_star_amd import nnops
+    L = nnops._lib()
+    p = C.c_void_p(4096)            # (never read: every call is refused)
+    for dt, most in ((0, 1 << 20), (1, 1 << 21), (2, 1 << 21)):
+        assert L.nirrt_nn_cross_entropy_workspace(dt, 9, 20, most) > 0 and L.nirrt_nn_cross_entropy_backward_workspace(dt, 9, 20, most) > 0
+        k = most + 1
+        assert L.nirrt_nn_cross_entropy_workspace(dt, 9, 20, k) == -1 and L.nirrt_nn_cross_entropy_backward_workspace(dt, 9, 20, k) == -1
+        assert L.nirrt_nn_cross_entropy(dt, p, k, p, k, None, p, None, -100, p, p, p, 9, 20, k, p, None) == -1
+        assert L.nirrt_nn_cross_entropy_backward(dt, p, k, p, k, None, p, None, -100, p, p, 0, None, p, p, None, 9, 20, k, p, None) == -1

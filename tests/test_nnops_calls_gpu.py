@@ -1,0 +1,70 @@
+"""GPU: calls of nirrt_star_amd.nnops that its documentation allows beyond sizes and types (test_nnops_gpu.py has those): operands far apart,
+losses and gradients used in place, autocast, the largest dimensions."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(shape, g, dt, scale=1.0):
+    return (torch.randn(shape, generator=g, device="cuda") * scale).to(dt)
+
+
+# ---- cross entropy: operands of any stride -----------------------------------------------------------------------------------------------
+def spread(t, row_bytes, shift=0):
+    """t's values in rows that lie row_bytes apart, from element `shift` on"""
+    ld = row_bytes // t.element_size()
+    flat = torch.zeros(t.shape[0] * ld + shift, dtype=t.dtype, device=t.device)
+    v = flat[shift:].as_strided(t.shape, (ld, 1), shift)
+    v.copy_(t)
+    return v
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("classes", [7, 33])
+@pytest.mark.parametrize("k", [64, 61])
+def test_cross_entropy_operands_of_any_stride(dt, classes, k):
+    """rows apart by less and more than the 4 MB that the products read directly, off 16 bytes, padded, transposed: what the kernels multiply is
+    the same in all of them, so the bits are those of contiguous operands"""
+    from nirrt_star_amd import nnops
+    g = gen(k + classes)
+    rows = 9
+    x, w, b = randn((rows, k), g, dt), randn((classes, k), g, dt), randn((classes,), g, dt)
+    t = torch.randint(0, classes, (rows,), generator=g, device="cuda")
+    t[4] = -100
+
+    def run(x, w):
+        leaves = [x.detach().requires_grad_(True), w.detach().requires_grad_(True)]
+        loss = nnops.linear_cross_entropy(leaves[0], leaves[1], t, bias=b)
+        return [loss.detach()] + list(torch.autograd.grad(loss, leaves))
+
+    want = run(x, w)
+    assert all(torch.isfinite(q).all() for q in want)
+    xs = [spread(x, 1 << 12), spread(x, 1 << 22), spread(x, (1 << 22) + 16), spread(x, 1 << 24, 3), spread(x, 1 << 10, 1), x.t().contiguous().t()]
+    ws = [spread(w, 1 << 22), spread(w, (1 << 22) + 16), spread(w, 1 << 23, 1), spread(w, 1 << 10, 1), w.t().contiguous().t()]
+    for q in xs:
+        assert all(torch.equal(a, e) for a, e in zip(run(q, w), want))
+    for q in ws:
+        assert all(torch.equal(a, e) for a, e in zip(run(x, q), want))
+    assert all(torch.equal(a, e) for a, e in zip(run(xs[3], ws[2]), want))
+
+
+def test_cross_entropy_of_the_last_token():
+    from nirrt_star_amd import nnops
+    g = gen(2)
+    h = torch.zeros(5, 1030, 2048, dtype=torch.bfloat16, device="cuda")
+    h[:, -1] = randn((5, 2048), g, torch.bfloat16)
+    w, t = randn((100, 2048), g, torch.bfloat16, 0.02), torch.arange(5, device="cuda") * 7
+    h.requires_grad_(True)
+    loss = nnops.linear_cross_entropy(h[:, -1], w, t, reduction="sum")
+    dh, = torch.autograd.grad(loss, h)
+    last = h[:, -1].detach().contiguous().requires_grad_(True)
+    want = nnops.linear_cross_entropy(last, w, t, reduction="sum")
+    d, = torch.autograd.grad(want, last)
+    assert torch.equal(loss, want) and torch.equal(dh[:, -1], d) and (dh[:, :-1] == 0).all()
