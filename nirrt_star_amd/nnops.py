@@ -8,7 +8,8 @@
 
 float32, bfloat16 and float16; sums are held in 32 bits and rounded once.  Tensors must live on the GPU (a CPU tensor is an error,
 there is no other implementation); rows may have any stride, other layouts are copied.  Results are the same bits for the same input
-(no atomics).  Backward passes are differentiable once.
+(no atomics).  Backward passes are differentiable once; there is no forward mode, and a call cannot be traced (torch.jit.trace, make_fx):
+both are refused.
 
 Everything can be captured into a graph; a backward pass through torch.autograd.grad, or with .backward() while no eager graph of the same
 leaves is alive (torch's accumulators of a leaf remember the stream they were made on, and adding to them from a capture ends the
@@ -19,6 +20,7 @@ import ctypes as C
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
@@ -73,8 +75,24 @@ def _on(device):
     return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
+_is_tracing = torch._C._is_tracing
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+
+
+def _not_recorded(name):
+    """torch.jit.trace and make_fx see the allocation of a result and not the kernel that fills it: what they record returns whatever
+    the memory holds"""
+    recorded = _is_tracing()
+    if not recorded and _dispatch_modes():
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+        recorded = get_proxy_mode() is not None
+    if recorded:
+        raise RuntimeError("nirrt_star_amd.nnops.%s cannot be traced: its kernels are launched through the C library" % name)
+
+
 def _need(name, first, **others):
     """one device (a GPU) and one element type for all of them"""
+    _not_recorded(name)
     if not first.is_cuda:
         raise RuntimeError("nirrt_star_amd.nnops.%s got a CPU tensor: the package only has the HIP kernels (move it to 'cuda')" % name)
     if first.dtype not in _TYPES:
@@ -201,7 +219,8 @@ def linear_act(x, weight, bias=None, residual=None, activation="none"):
     if bias is not None:
         bias = bias.contiguous()
     act = ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+    # (dual numbers go through autograd too, which refuses them: there is no forward mode)
+    if forward_ad._current_level >= 0 or torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
         return _Linear.apply(x, weight, bias, residual, act)
     with _on(x.device):
@@ -282,7 +301,10 @@ _TENSOR = np.dtype([("data", "<u8"), ("out", "<u8"), ("n", "<i8"), ("dtype", "<i
 
 def _tensor_list(name, tensors):
     """-> the tensors that are not None, their device, their element types if they differ (else the one they share)"""
+    _not_recorded(name)
     ts = [t for t in tensors if t is not None]
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise NotImplementedError("%s: no forward mode" % name)
     if not ts:
         raise ValueError("%s: no tensors" % name)
     # (one pass per property into a set: with hundreds of small tensors the host's time is what counts)

@@ -15,3 +15,16 @@ def test_cross_entropy_refuses_rows_of_more_than_4_mb():
         assert L.nirrt_nn_cross_entropy_workspace(dt, 9, 20, k) == -1 and L.nirrt_nn_cross_entropy_backward_workspace(dt, 9, 20, k) == -1
         assert L.nirrt_nn_cross_entropy(dt, p, k, p, k, None, p, None, -100, p, p, p, 9, 20, k, p, None) == -1
         assert L.nirrt_nn_cross_entropy_backward(dt, p, k, p, k, None, p, None, -100, p, p, 0, None, p, p, None, 9, 20, k, p, None) == -1
+
+
+def test_traces_are_refused():
+    """(whatever the device: a trace would hold the allocation of the result and not what fills it)"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from nirrt_star_amd import nnops
+    x, w, t = torch.zeros(3, 4), torch.zeros(5, 4), torch.zeros(3, dtype=torch.int64)
+    for call in (lambda x: nnops.linear_act(x, w), lambda x: nnops.linear_cross_entropy(x, w, t), lambda x: nnops.grad_norm([x]),
+                 lambda x: nnops.clip_grad_norm_([x], 1.0)):
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(call, (x,), check_trace=False)
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(call)(x)

@@ -68,3 +68,30 @@ def test_cross_entropy_of_the_last_token():
     want = nnops.linear_cross_entropy(last, w, t, reduction="sum")
     d, = torch.autograd.grad(want, last)
     assert torch.equal(loss, want) and torch.equal(dh[:, -1], d) and (dh[:, :-1] == 0).all()
+
+
+# ---- forward mode and traces ---------------------------------------------------------------------------------------------------------------
+def test_dual_numbers_are_refused_where_a_tangent_would_be_lost():
+    from torch.autograd import forward_ad
+    from nirrt_star_amd import nnops
+    x, w, t = torch.randn(5, 4, device="cuda"), torch.randn(3, 4, device="cuda"), torch.zeros(5, dtype=torch.int64, device="cuda")
+    plain = nnops.linear_act(x, w, activation="silu")
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: nnops.linear_act(d, w), lambda: nnops.linear_act(x, forward_ad.make_dual(w, torch.ones_like(w))),
+                     lambda: nnops.linear_act(x, w, residual=forward_ad.make_dual(plain, torch.ones_like(plain))),
+                     lambda: nnops.linear_cross_entropy(d, w, t), lambda: nnops.grad_norm([x, d]), lambda: nnops.clip_grad_norm_([d], 1.0)):
+            with pytest.raises(NotImplementedError):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                call()
+        assert torch.equal(nnops.linear_act(x, w, activation="silu"), plain)         # (no dual number: as everywhere)
+    assert (d == x).all()
+
+
+def test_traces_are_refused():
+    from nirrt_star_amd import nnops
+    x, w = torch.randn(5, 4, device="cuda"), torch.randn(3, 4, device="cuda", requires_grad=True)
+    for weight in (w, w.detach()):
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(lambda q: nnops.linear_act(q, weight), (x,), check_trace=False)
