@@ -244,7 +244,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
                                             nll.data_ptr(), total.data_ptr(), rows, v, k, _ptr(ws), _stream(x.device)), "cross_entropy")
         ctx.ignore, ctx.mode = ignore, mode
         ctx.save_for_backward(x, w, b, target, cw, lse, total)
-        return nll if mode == "none" else total[2 if mode == "mean" else 0]
+        # (.data: no view of `total` for autograd, with a version of its own, so that a caller may scale or add to the loss in place; of
+        # `total` the backward pass reads the sum of the weights only)
+        return nll if mode == "none" else total[2 if mode == "mean" else 0].data
 
     @staticmethod
     @torch.autograd.function.once_differentiable

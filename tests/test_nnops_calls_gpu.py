@@ -95,3 +95,33 @@ def test_traces_are_refused():
     for weight in (w, w.detach()):
         with pytest.raises(RuntimeError, match="traced"):
             torch.jit.trace(lambda q: nnops.linear_act(q, weight), (x,), check_trace=False)
+
+
+# ---- in place on results and on saved tensors ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("classes", [2, 40])
+def test_the_loss_can_be_changed_in_place(reduction, classes):
+    """loss /= steps; loss += another term: as on any loss"""
+    from nirrt_star_amd import nnops
+    g = gen(classes)
+    x, w = randn((30, 16), g, torch.float32), randn((classes, 16), g, torch.float32)
+    t = torch.randint(0, classes, (30,), generator=g, device="cuda")
+    cw = torch.rand(classes, generator=g, device="cuda") + 0.5
+
+    def leaves():
+        return [q.clone().requires_grad_(True) for q in (x, w)]
+
+    a, b = leaves(), leaves()
+    want = nnops.linear_cross_entropy(a[0], a[1], t, class_weight=cw, reduction=reduction)
+    value = want.detach().clone()
+    (want / 4 + (a[0] ** 2).sum()).sum().backward()
+    loss = nnops.linear_cross_entropy(b[0], b[1], t, class_weight=cw, reduction=reduction)
+    loss /= 4
+    loss += (b[0] ** 2).sum()
+    loss.sum().backward()
+    assert torch.equal(loss.detach(), value / 4 + (x ** 2).sum())
+    for p, q in zip(a, b):
+        assert torch.equal(p.grad, q.grad)
+    total = torch.zeros((), device="cuda")
+    total += nnops.linear_cross_entropy(x, w, t, class_weight=cw, reduction="sum")
+    assert float(total) > 0
