@@ -17,6 +17,7 @@ process).
 """
 import contextlib
 import ctypes as C
+import operator
 
 import numpy as np
 import torch
@@ -298,6 +299,7 @@ def linear_cross_entropy(x, weight, target, bias=None, class_weight=None, ignore
 
 
 # ---- norm and clipping of many tensors -------------------------------------------------------------------------------------------------
+_dtype_of, _layout_of = operator.attrgetter("dtype"), operator.attrgetter("layout")
 _TENSOR = np.dtype([("data", "<u8"), ("out", "<u8"), ("n", "<i8"), ("dtype", "<i4"), ("out_dtype", "<i4")])   # nirrt_nn_tensor
 
 
@@ -309,25 +311,25 @@ def _tensor_list(name, tensors):
         raise NotImplementedError("%s: no forward mode" % name)
     if not ts:
         raise ValueError("%s: no tensors" % name)
-    # (one pass per property into a set: with hundreds of small tensors the host's time is what counts)
-    where = {t.get_device() for t in ts}
+    # (one pass per property, without a step of the interpreter per tensor: with hundreds of small tensors the host's time is what counts)
+    where = set(map(torch.Tensor.get_device, ts))
     if where == {-1}:
         raise RuntimeError("nirrt_star_amd.nnops.%s got a CPU tensor: the package only has the HIP kernels (move it to 'cuda')" % name)
-    types = [t.dtype for t in ts]
+    types = list(map(_dtype_of, ts))
     kinds = set(types)
-    if len(where) != 1 or {t.layout for t in ts} != {torch.strided} or not kinds <= _TYPES.keys():
+    if len(where) != 1 or set(map(_layout_of, ts)) != {torch.strided} or not kinds <= _TYPES.keys():
         raise ValueError("%s: dense float32, bfloat16 or float16 tensors of one device" % name)
     return ts, ts[0].device, _TYPES[types[0]] if len(kinds) == 1 else [_TYPES[t] for t in types]
 
 
 def _dense(ts):
-    return ts if all([t.is_contiguous() for t in ts]) else [t if t.is_contiguous() else t.contiguous() for t in ts]
+    return ts if all(map(torch.Tensor.is_contiguous, ts)) else [t if t.is_contiguous() else t.contiguous() for t in ts]
 
 
 def _table(ts, types):
     tab = np.zeros(len(ts), dtype=_TENSOR)
-    tab["data"] = [t.data_ptr() for t in ts]
-    tab["n"] = [t.numel() for t in ts]
+    tab["data"] = list(map(torch.Tensor.data_ptr, ts))
+    tab["n"] = list(map(torch.Tensor.numel, ts))
     tab["dtype"] = types
     return tab
 
@@ -366,13 +368,14 @@ def clip_grad_norm_(grads, max_norm, out=None):
     ts, dev, types = _tensor_list(name, grads)
     src = _dense(ts)
     tab = _table(src, types)
+    dst = ts
     if out is None:
         tab["out"], tab["out_dtype"] = tab["data"], tab["dtype"]
     else:
         dst, dev_o, types = _tensor_list(name, out)
-        if dev_o != dev or [o.numel() for o in dst] != tab["n"].tolist() or not all([o.is_contiguous() for o in dst]):
+        if dev_o != dev or list(map(torch.Tensor.numel, dst)) != tab["n"].tolist() or not all(map(torch.Tensor.is_contiguous, dst)):
             raise ValueError("%s: outputs must be contiguous, of as many elements as the gradients and on their device" % name)
-        tab["out"], tab["out_dtype"] = [o.data_ptr() for o in dst], types
+        tab["out"], tab["out_dtype"] = list(map(torch.Tensor.data_ptr, dst)), types
     full = tab[tab["n"] > 0]
     places = set(full["out"].tolist())
     if len(places) != len(full):
@@ -384,8 +387,10 @@ def clip_grad_norm_(grads, max_norm, out=None):
     with _on(dev):
         norm = _norm(tab, dev)
         _check(_lib().nirrt_nn_scale_by_norm(tab.ctypes.data, len(tab), norm.data_ptr(), max_norm, _stream(dev)), "scale_by_norm")
-        if out is None:
+        if out is None and src is not ts:
             for t, s in zip(ts, src):
                 if s is not t:
                     t.copy_(s)
+    # the kernel writes where autograd does not see it: a graph that saved one of these tensors has to find out
+    torch.autograd.graph.increment_version(dst)
     return norm

@@ -125,3 +125,21 @@ def test_the_loss_can_be_changed_in_place(reduction, classes):
     total = torch.zeros((), device="cuda")
     total += nnops.linear_cross_entropy(x, w, t, class_weight=cw, reduction="sum")
     assert float(total) > 0
+
+
+def test_clipping_is_seen_by_graphs_that_saved_the_tensor():
+    from nirrt_star_amd import nnops
+    x = torch.ones(8, device="cuda", requires_grad=True)
+    wide = torch.ones(8, 3, device="cuda")
+    for g, out in ((torch.full((8,), 3.0, device="cuda"), None), (wide[:, 1], None), (torch.ones(8, device="cuda"), torch.zeros(8, device="cuda"))):
+        saved = g if out is None else out
+        y = (x * saved).sum()                       # keeps `saved` for x's gradient
+        before = saved._version
+        nnops.clip_grad_norm_([None, g], 0.5, out=None if out is None else [None, out])
+        assert saved._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():                    # (tensors without a version)
+        g = torch.full((8,), 3.0, device="cuda")
+        nnops.clip_grad_norm_([g], 1.0)
+        assert abs(float(g.norm()) - 1) < 1e-5
