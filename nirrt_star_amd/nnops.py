@@ -299,7 +299,7 @@ def linear_cross_entropy(x, weight, target, bias=None, class_weight=None, ignore
 
 
 # ---- norm and clipping of many tensors -------------------------------------------------------------------------------------------------
-_dtype_of, _layout_of = operator.attrgetter("dtype"), operator.attrgetter("layout")
+_dtype_of, _layout_of, _wants_grad = operator.attrgetter("dtype"), operator.attrgetter("layout"), operator.attrgetter("requires_grad")
 _TENSOR = np.dtype([("data", "<u8"), ("out", "<u8"), ("n", "<i8"), ("dtype", "<i4"), ("out_dtype", "<i4")])   # nirrt_nn_tensor
 
 
@@ -354,7 +354,8 @@ def grad_norm(tensors):
 def clip_grad_norm_(grads, max_norm, out=None):
     """scales the tensors by min(1, max_norm / (norm + 1e-6)), norm as grad_norm gives it, and returns the norm (float32 scalar on their
     device; nothing waits for it).  In place, or into `out`: as many contiguous tensors of as many elements each, of any of the three types
-    (half-precision gradients into float32 ones, say).  None entries are skipped (in `out` too).  A tensor may be named once only, and an
+    (half-precision gradients into float32 ones, say).  It takes the gradients themselves: a leaf that requires a gradient (a parameter) is
+    refused as a tensor to write into.  None entries are skipped (in `out` too).  A tensor may be named once only, and an
     `out` tensor may share memory with its own gradient (of the same type) but not with another one."""
     name = "clip_grad_norm_"
     max_norm = float(max_norm)
@@ -384,6 +385,8 @@ def clip_grad_norm_(grads, max_norm, out=None):
         own = full["out"] == full["data"]
         if not places.isdisjoint(full["data"][~own].tolist()) or ((full["dtype"] != full["out_dtype"]) & own).any():
             raise ValueError("%s: an output shares memory with another gradient, or with its own of another type" % name)
+    if any(map(_wants_grad, dst)) and any(t.requires_grad and t.is_leaf for t in dst):
+        raise ValueError("%s: a leaf that requires a gradient would be scaled: pass the gradients (p.grad), not the parameters" % name)
     with _on(dev):
         norm = _norm(tab, dev)
         _check(_lib().nirrt_nn_scale_by_norm(tab.ctypes.data, len(tab), norm.data_ptr(), max_norm, _stream(dev)), "scale_by_norm")

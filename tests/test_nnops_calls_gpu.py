@@ -143,3 +143,25 @@ def test_clipping_is_seen_by_graphs_that_saved_the_tensor():
         g = torch.full((8,), 3.0, device="cuda")
         nnops.clip_grad_norm_([g], 1.0)
         assert abs(float(g.norm()) - 1) < 1e-5
+
+
+def test_clipping_refuses_parameters():
+    from nirrt_star_amd import nnops
+    model = torch.nn.Linear(6, 4).cuda()
+    model(torch.randn(3, 6, device="cuda")).sum().backward()
+    before = [p.detach().clone() for p in model.parameters()]
+    grads = [p.grad for p in model.parameters()]
+    with pytest.raises(ValueError, match="not the parameters"):
+        nnops.clip_grad_norm_(model.parameters(), 1.0)
+    with pytest.raises(ValueError, match="not the parameters"):
+        nnops.clip_grad_norm_(grads, 1.0, out=list(model.parameters()))
+    assert all(torch.equal(p, q) for p, q in zip(model.parameters(), before))
+    assert float(nnops.grad_norm(model.parameters())) > 0                 # (reading them is fine)
+    nnops.clip_grad_norm_(grads, 1.0)
+    assert abs(float(nnops.grad_norm(grads)) - 1) < 1e-5
+    # gradients that carry a graph of their own are no leaves
+    x = torch.randn(5, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad((x ** 3).sum(), x, create_graph=True)
+    assert g.requires_grad
+    nnops.clip_grad_norm_([g], 1.0)
+    assert abs(float(nnops.grad_norm([g])) - 1) < 1e-5
