@@ -256,13 +256,17 @@ class get_model(nn.Module):
     def loss(self, points, labels, class_weight=None, fps_starts=None):
         """mean cross entropy of the points' labels (B, N) int64 (-100: the point counts for nothing), weighted by class (the training
         set's labelweights), as the reference trains with: F.nll_loss(log_softmax, target, weight).  With gradients for all parameters;
-        the head works on the points' rows as they come, its second layer and the loss are one operator."""
+        the head works on the points' rows as they come, its second layer and the loss are one operator.  Under autocast the layers
+        before the head run in 16 bits as in forward(), the head and the loss in the parameters' type."""
         if self._head is not None and not self.training:
             raise RuntimeError("loss: a folded model in eval mode has no gradients for its layers: call train() first (and fold() again afterwards)")
         f0, _ = self._point_features(points, fps_starts, None)
-        x = nnops.linear_act(f0.reshape(-1, f0.shape[2]), self.conv1.weight.squeeze(2), self.conv1.bias)
-        x = self.drop1(F.relu(self.bn1(x)))
-        return nnops.linear_cross_entropy(x, self.conv2.weight.squeeze(2), labels.reshape(-1), bias=self.conv2.bias, class_weight=class_weight)
+        # (under autocast the layers before leave 16-bit features: the head and the loss take the parameters' type)
+        with torch.autocast(f0.device.type, enabled=False):
+            x = f0.reshape(-1, f0.shape[2]).to(self.conv1.weight.dtype)
+            x = nnops.linear_act(x, self.conv1.weight.squeeze(2), self.conv1.bias)
+            x = self.drop1(F.relu(self.bn1(x)))
+            return nnops.linear_cross_entropy(x, self.conv2.weight.squeeze(2), labels.reshape(-1), bias=self.conv2.bias, class_weight=class_weight)
 
 
 def train_step(model, optimizer, points, labels, class_weight=None, max_norm=None, fps_starts=None):

@@ -122,3 +122,28 @@ def test_a_capture_is_refused_before_anything_is_recorded():
         graph.replay()
         torch.cuda.synchronize()
         assert (y == 1).all()
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_loss_under_autocast(dt):
+    """the layers before the head in 16 bits, the head and the loss as without autocast; gradients in the parameters' type"""
+    m = _model(8)
+    x, labels, starts = _batch(2, 1300, 5)
+    cw = torch.tensor([1.0, 1.7], device="cuda")
+    seen = {}
+    hook = m.bn1.register_forward_hook(lambda mod, i, o: seen.__setitem__("h", o.detach()))
+    with torch.autocast("cuda", dtype=dt):
+        loss = m.loss(x, labels, cw, starts)
+        hook.remove()
+        assert m(x, fps_starts=starts)[0].shape == (2, 1300, 2)            # (what the loss replaces works there too)
+    loss.backward()
+    h = seen["h"].relu().double()
+    w, b = m.conv2.weight.squeeze(2).detach().double(), m.conv2.bias.detach().double()
+    t = labels.reshape(-1)
+    keep = t >= 0
+    logp = torch.log_softmax(h @ w.t() + b, 1)
+    wt = cw.double()[t[keep]]
+    want = -(logp[keep, t[keep]] * wt).sum() / wt.sum()
+    assert loss.dtype == torch.float32 and seen["h"].dtype == torch.float32
+    assert abs(float(loss.detach()) - float(want)) <= 130 * 2.0 ** -24 * (1 + float((h.abs() @ w.abs().t()).max()))
+    assert all(p.grad is not None and p.grad.dtype == torch.float32 and torch.isfinite(p.grad).all() for p in m.parameters())
