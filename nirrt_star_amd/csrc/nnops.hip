@@ -559,7 +559,7 @@ __device__ __forceinline__ float act_slope(int act, float z)
 {
     float e;
     switch (act) {
-    case NIRRT_NN_ACT_RELU: return z > 0.f ? 1.f : 0.f;
+    case NIRRT_NN_ACT_RELU: return z > 0.f ? 1.f : (z == z ? 0.f : z);        // (NaN stays)
     case NIRRT_NN_ACT_GELU: { const float c = normal_cdf(z, e); return __builtin_fmaf(z * 0.39894228040143268f, e, c); }
     case NIRRT_NN_ACT_SILU: { const float s = logistic(z); return s * (1.f + z * (1.f - s)); }
     default: return 1.f;

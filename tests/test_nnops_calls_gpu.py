@@ -165,3 +165,21 @@ def test_clipping_refuses_parameters():
     assert g.requires_grad
     nnops.clip_grad_norm_([g], 1.0)
     assert abs(float(nnops.grad_norm([g])) - 1) < 1e-5
+
+
+# ---- special values --------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu"])
+@pytest.mark.parametrize("with_res", [False, True])
+def test_a_nan_before_the_activation_reaches_the_gradients(act, dt, with_res):
+    """row 2 of x is NaN: its pre-activations, values and slopes are; the other rows' dx do not see it, dw and db (sums over the rows) do"""
+    from nirrt_star_amd import nnops
+    g = gen(5)
+    x, w, b, r = randn((40, 16), g, dt), randn((24, 16), g, dt), randn((24,), g, dt), randn((40, 24), g, dt)
+    x[2, 3] = float("nan")
+    leaves = [q.clone().requires_grad_(True) for q in (x, w, b)]
+    y = nnops.linear_act(*leaves, residual=r if with_res else None, activation=act)
+    dx, dw, db = torch.autograd.grad(y, leaves, torch.ones_like(y))
+    rest = torch.arange(40, device="cuda") != 2
+    assert torch.isnan(y[2]).all() and torch.isfinite(y[rest]).all()
+    assert torch.isnan(dx[2]).all() and torch.isfinite(dx[rest]).all() and torch.isnan(dw).all() and torch.isnan(db).all()
