@@ -6,7 +6,7 @@
  * Workspaces are the caller's: at least the bytes that the _workspace function of the same sizes returns, 256-byte aligned, in use until
  * the launches have run (two captured graphs that may replay at the same time need one each).
  * Element types: NIRRT_NN_F32 / _BF16 / _F16; sums are held in 32 bits.  Matrices are row-major with a row stride in elements (ld >= row
- * length); dimensions are < 2^31, their products may be larger. */
+ * length); dimensions are at most 2^31 - 4096, their products may be larger. */
 #ifndef NIRRT_NNOPS_H
 #define NIRRT_NNOPS_H
 #include <stdint.h>

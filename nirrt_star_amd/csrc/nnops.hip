@@ -1411,6 +1411,7 @@ __global__ __launch_bounds__(256) void k_scale(TensorTable t, const float *norm,
 
 // ---- host side ---------------------------------------------------------------------------------------------------------------------
 constexpr int64_t DIM_MAX = 0x7fffffffll;
+constexpr int64_t MOST = DIM_MAX - 4095;  // of a dimension: kernels look up to 2048 elements past an index in 32 bits (k_few_rows; k_dz 1024)
 int64_t round256(int64_t b) { return (b + 255) & ~255ll; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int status() { return hipGetLastError() == hipSuccess ? 0 : -2; }
@@ -1507,7 +1508,7 @@ int gemm(const Operand<T> &a, const Operand<T> &b, int64_t m, int64_t n, int64_t
     return status();
 }
 
-bool good_dims(int64_t a, int64_t b, int64_t c) { return a >= 0 && b >= 0 && c >= 0 && a <= DIM_MAX - 256 && b <= DIM_MAX - 256 && c <= DIM_MAX - 256; }
+bool good_dims(int64_t a, int64_t b, int64_t c) { return a >= 0 && b >= 0 && c >= 0 && a <= MOST && b <= MOST && c <= MOST; }
 
 // k_dz: lanes per row, rows per workgroup and chunks so that some 2000 workgroups share a large matrix and a chunk is no shorter than 4 passes
 struct Columns { int lanes, blocks, chunk, parts; };

@@ -25,7 +25,7 @@ from torch.autograd import forward_ad
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
-_DIM_MAX = 0x7fffffff - 256
+_DIM_MAX = (1 << 31) - 4096
 
 
 _library = None

@@ -28,3 +28,20 @@ def test_traces_are_refused():
             torch.jit.trace(call, (x,), check_trace=False)
         with pytest.raises(RuntimeError, match="traced"):
             make_fx(call)(x)
+
+
+def test_dimensions_are_bounded():
+    """kernels look a little past an index in 32 bits"""
+    from nirrt_star_amd import nnops
+    L = nnops._lib()
+    p = C.c_void_p(4096)            # (never read)
+    most = (1 << 31) - 4096
+    assert nnops._DIM_MAX == most
+    for dims in ((most, 1, 1), (1, most, 1), (1, 1, most)):
+        m, n, k = dims
+        assert L.nirrt_nn_linear_workspace(1, p, k, p, k, m, n, k) >= 0 and L.nirrt_nn_linear_backward_workspace(1, 1, p, k, p, k, p, n, m, n, k) >= 0
+        m, n, k = (d + (d == most) for d in dims)
+        assert L.nirrt_nn_linear_workspace(1, p, k, p, k, m, n, k) == -1 and L.nirrt_nn_linear_backward_workspace(1, 1, p, k, p, k, p, n, m, n, k) == -1
+        assert L.nirrt_nn_linear(1, 0, p, k, p, k, None, None, n, p, n, None, m, n, k, p, None) == -1
+        assert L.nirrt_nn_linear_backward(1, 0, p, k, p, k, None, p, n, p, p, p, m, n, k, p, None) == -1
+    assert L.nirrt_nn_cross_entropy_workspace(1, most + 1, 2, 8) == -1 and L.nirrt_nn_cross_entropy_workspace(1, 8, most + 1, 8) == -1

@@ -183,3 +183,32 @@ def test_a_nan_before_the_activation_reaches_the_gradients(act, dt, with_res):
     rest = torch.arange(40, device="cuda") != 2
     assert torch.isnan(y[2]).all() and torch.isfinite(y[rest]).all()
     assert torch.isnan(dx[2]).all() and torch.isfinite(dx[rest]).all() and torch.isnan(dw).all() and torch.isnan(db).all()
+
+
+# ---- the largest dimensions --------------------------------------------------------------------------------------------------------------------
+MOST = (1 << 31) - 4096
+
+
+def test_the_longest_reduction():
+    """few rows: whole numbers, so the sum is exact whatever its order"""
+    from nirrt_star_amd import nnops
+    x, w = (torch.zeros(1, MOST, dtype=torch.float16, device="cuda") for _ in range(2))
+    at = torch.tensor([0, 1, 2047, 2048, 1 << 30, MOST - 2049, MOST - 2048, MOST - 257, MOST - 256, MOST - 1], device="cuda")
+    x[0, at] = torch.arange(1, 11, device="cuda").half()
+    w[0, at] = 2.0
+    assert float(nnops.linear_act(x, w)) == 110.0
+    with pytest.raises(ValueError, match="beyond"):
+        nnops.linear_act(torch.empty(0, MOST + 1, device="cuda"), torch.empty(0, MOST + 1, device="cuda"))
+
+
+def test_column_sums_of_the_most_rows():
+    from nirrt_star_amd import nnops
+    L = nnops._lib()
+    dy = torch.zeros(MOST, 8, dtype=torch.float16, device="cuda")
+    at = torch.tensor([0, 255, 256, 1023, 1024, 1 << 30, MOST - 1025, MOST - 1024, MOST - 256, MOST - 1], device="cuda")
+    dy[at] = (torch.arange(80, device="cuda") % 13).view(10, 8).half()
+    db = torch.empty(8, dtype=torch.float16, device="cuda")
+    ws = torch.empty(L.nirrt_nn_linear_backward_workspace(2, 0, None, 8, None, 8, dy.data_ptr(), 8, MOST, 8, 0), dtype=torch.uint8, device="cuda")
+    assert L.nirrt_nn_linear_backward(2, 0, None, 8, None, 8, None, dy.data_ptr(), 8, None, None, db.data_ptr(), MOST, 8, 0, ws.data_ptr(),
+                                      torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(db, (torch.arange(80, device="cuda") % 13).view(10, 8).sum(0).half())
