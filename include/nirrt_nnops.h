@@ -37,7 +37,7 @@ int nirrt_nn_linear_backward(int dtype, int act, const void *x, int64_t ldx, con
  * target int64 (rows,), class_weight f32 (classes,) or NULL.  A row whose target is ignore_index counts for nothing; any other target
  * outside [0, classes) gives NaN.  lse (rows, 2) = the largest l and log sum exp(l - it), nll (rows,) = weight * (log sum exp l - l[target]) (0 where ignored),
  * total (3,) = {sum of nll, sum of the weights, their quotient}, all f32.  Rows may lie any distance apart; k elements are
- * 4 MB at most. */
+ * 4 MB at most, and more than 8 classes take less than 2^29 rows. */
 int64_t nirrt_nn_cross_entropy_workspace(int dtype, int64_t rows, int64_t classes, int64_t k);
 int nirrt_nn_cross_entropy(int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw, const void *b, const int64_t *target,
                            const float *class_weight, int64_t ignore_index, float *lse, float *nll, float *total, int64_t rows,

@@ -1479,15 +1479,18 @@ template <class T, bool RC> bool direct(const Operand<T> &o, int64_t k)
     return RC ? row_bytes <= (1 << 24) : k % Elem<T>::PER_CHUNK == 0 && row_bytes <= KC_ROW_BYTES;
 }
 
+constexpr int64_t MOST_WORKGROUPS = (1ll << 32) / 512 - 1;      // of 512 threads: a launch has less than 2^32 of them
+
 template <class Epi> constexpr bool always_whole = false;                        // its operands are always whole aligned chunks, its reduction in one part
 template <class T> constexpr bool always_whole<EpiSoftmaxGrad<T>> = true;
 template <class T, bool RCA, bool RCB, class Epi>
 int gemm(const Operand<T> &a, const Operand<T> &b, int64_t m, int64_t n, int64_t k, const Plan &p, float *partial, const Epi &epi, hipStream_t st)
 {
     const bool fast = direct<T, RCA>(a, k) && direct<T, RCB>(b, k);
-    const int edge = fast || p.edge < 256 ? p.edge : 128;   // (a plan for whole chunks, and operands beyond direct()'s row length)
+    int edge = fast || p.edge < 256 ? p.edge : 128;         // (a plan for whole chunks, and operands beyond direct()'s row length)
+    if (edge == 64 && ceil_div(m, 64) * ceil_div(n, 64) > MOST_WORKGROUPS) edge = 128;     // (a quarter of them)
     const int64_t tiles = ceil_div(m, edge) * ceil_div(n, edge);
-    if (tiles > DIM_MAX) return -1;
+    if (tiles > 2 * MOST_WORKGROUPS) return -1;
     const dim3 grid((unsigned)tiles, (unsigned)p.parts);
 #define LAUNCH(TILE, EDGE, WM, WN)                                                                                                               \
     hipLaunchKernelGGL((k_gemm<T, EDGE, EDGE, TILE<T, EDGE, EDGE, WM, WN, RCA, RCB>, Epi>), grid, dim3(64 * WM * WN), 0, st, a, b, (int)m, (int)n, \
@@ -1534,7 +1537,7 @@ struct Linear { bool few, copy_x, copy_w; Plan p; int64_t kp, xs, ws, part, tota
 Linear linear_layout(int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t m, int64_t n, int64_t k)
 {
     Linear l = {};
-    l.few = m <= 32;
+    l.few = m <= 32 && ceil_div(n, 16) <= MOST_WORKGROUPS;
     l.kp = k;
     if (l.few) return l;
     l.copy_x = !whole_rows(dtype, x, ldx, k);
@@ -1906,7 +1909,8 @@ extern "C" int nirrt_nn_linear_backward(int dtype, int act, const void *x, int64
 
 static bool good_cross_entropy(int dtype, int64_t rows, int64_t classes, int64_t k)
 {
-    return good_type(dtype) && good_dims(rows, classes, k) && classes >= 1 && padded(dtype, k) * elem_size(dtype) <= KC_ROW_BYTES;
+    return good_type(dtype) && good_dims(rows, classes, k) && classes >= 1 && padded(dtype, k) * elem_size(dtype) <= KC_ROW_BYTES &&
+           (classes <= 8 || rows < 1 << 29);          // (k_ce_rows: eight lanes per row, 2^32 in a launch)
 }
 
 extern "C" int64_t nirrt_nn_cross_entropy_workspace(int dtype, int64_t rows, int64_t classes, int64_t k)

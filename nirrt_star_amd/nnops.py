@@ -294,6 +294,8 @@ def linear_cross_entropy(x, weight, target, bias=None, class_weight=None, ignore
     _sizes_ok(name, target.numel(), v, weight.shape[1])
     if weight.shape[1] * weight.element_size() > 1 << 22:
         raise ValueError("%s: %d inputs are more than 4 MB" % (name, weight.shape[1]))
+    if v > 8 and target.numel() >= 1 << 29:
+        raise ValueError("%s: %d rows of more than 8 classes" % (name, target.numel()))
     return _LinearCrossEntropy.apply(x, weight, bias.contiguous() if bias is not None else None, target.contiguous(),
                                      class_weight.contiguous() if class_weight is not None else None, int(ignore_index), reduction)
 

@@ -44,4 +44,5 @@ def test_dimensions_are_bounded():
         assert L.nirrt_nn_linear_workspace(1, p, k, p, k, m, n, k) == -1 and L.nirrt_nn_linear_backward_workspace(1, 1, p, k, p, k, p, n, m, n, k) == -1
         assert L.nirrt_nn_linear(1, 0, p, k, p, k, None, None, n, p, n, None, m, n, k, p, None) == -1
         assert L.nirrt_nn_linear_backward(1, 0, p, k, p, k, None, p, n, p, p, p, m, n, k, p, None) == -1
+    assert L.nirrt_nn_cross_entropy_workspace(1, 1 << 29, 8, 8) > 0 and L.nirrt_nn_cross_entropy_workspace(1, 1 << 29, 9, 8) == -1
     assert L.nirrt_nn_cross_entropy_workspace(1, most + 1, 2, 8) == -1 and L.nirrt_nn_cross_entropy_workspace(1, 8, most + 1, 8) == -1

@@ -212,3 +212,20 @@ def test_column_sums_of_the_most_rows():
     assert L.nirrt_nn_linear_backward(2, 0, None, 8, None, 8, None, dy.data_ptr(), 8, None, None, db.data_ptr(), MOST, 8, 0, ws.data_ptr(),
                                       torch.cuda.current_stream().cuda_stream) == 0
     assert torch.equal(db, (torch.arange(80, device="cuda") % 13).view(10, 8).sum(0).half())
+
+
+def test_more_rows_and_columns_than_a_launch_has_small_tiles_for():
+    """2^30 + 5 rows of a narrow layer, 2^27 + 5 columns for two rows: whole numbers, looked at in a few places"""
+    from nirrt_star_amd import nnops
+    g = gen(6)
+    for m, n, k in (((1 << 30) + 5, 3, 8), (2, (1 << 27) + 5, 8)):
+        x, w = torch.zeros(m, k, dtype=torch.float16, device="cuda"), torch.zeros(n, k, dtype=torch.float16, device="cuda")
+        at, long = torch.tensor([0, 1, 63, 64, 1 << 26, max(m, n) - 6, max(m, n) - 5, max(m, n) - 1], device="cuda"), x if m > n else w
+        short = w if m > n else x
+        long[at] = torch.randint(-3, 4, (8, k), generator=g, device="cuda").half()
+        short.copy_(torch.randint(-3, 4, tuple(short.shape), generator=g, device="cuda"))
+        y = nnops.linear_act(x, w)
+        got = y[at] if m > n else y[:, at].t()
+        assert torch.equal(got.double(), long[at].double() @ short.double().t())
+        assert int((y != 0).sum()) == int((got != 0).sum())
+        del x, w, long, short, y
