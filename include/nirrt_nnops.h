@@ -37,7 +37,10 @@ int nirrt_nn_linear_backward(int dtype, int act, const void *x, int64_t ldx, con
  * target int64 (rows,), class_weight f32 (classes,) or NULL.  A row whose target is ignore_index counts for nothing; any other target
  * outside [0, classes) gives NaN.  lse (rows, 2) = the largest l and log sum exp(l - it), nll (rows,) = weight * (log sum exp l - l[target]) (0 where ignored),
  * total (3,) = {sum of nll, sum of the weights, their quotient}, all f32.  Rows may lie any distance apart; k elements are
- * 4 MB at most, and more than 8 classes take less than 2^29 rows. */
+ * 4 MB at most, and more than 8 classes take less than 2^29 rows.
+ * More than 8 classes: the workspace ends in room for a copy of x, X = rows * k' elements, and one of w, W = classes * k' (k' = k rounded
+ * up to 16 bytes; X and W each rounded up to 256 bytes).  A copy is made where base, row stride and k are not all multiples of 16 bytes,
+ * or the stride is above 4 MB; a caller whose x or w needs none may leave its bytes out. */
 int64_t nirrt_nn_cross_entropy_workspace(int dtype, int64_t rows, int64_t classes, int64_t k);
 int nirrt_nn_cross_entropy(int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw, const void *b, const int64_t *target,
                            const float *class_weight, int64_t ignore_index, float *lse, float *nll, float *total, int64_t rows,
@@ -46,7 +49,8 @@ int nirrt_nn_cross_entropy(int dtype, const void *x, int64_t ldx, const void *w,
 /* Its gradients: c_i = dloss_i * weight(target_i) (0 where ignored), g_iv = c_i (exp(l_iv - lse_i) - [v = target_i]), dx = g w, dw = g^T x,
  * db = column sums of g.  dloss f32: `dloss_stride` 1 = one value per row, 0 = one value for all rows; where `total` is given, it is
  * divided by total[1] (the mean over the weights).  lse as the forward pass left it.  dx (rows, k), dw (classes, k) contiguous,
- * db (classes,); each may be NULL. */
+ * db (classes,); each may be NULL.  More than 8 classes: the workspace ends in room for a copy of w, W bytes as above, which may be left
+ * out where w needs none. */
 int64_t nirrt_nn_cross_entropy_backward_workspace(int dtype, int64_t rows, int64_t classes, int64_t k);
 int nirrt_nn_cross_entropy_backward(int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw, const void *b, const int64_t *target,
                                     const float *class_weight, int64_t ignore_index, const float *lse, const float *dloss,

@@ -1676,10 +1676,15 @@ bool few_layout(int dtype, int64_t rows, int64_t classes, int64_t k, Few &f)
 
 // cross entropy: tile edge, and parts of the classes so that row tiles x parts fill the GPU; x and w whose rows are no whole aligned chunks
 // or lie far apart are copied into such that are not (k_rows_copy): the products read them many times
+// (the copies lie behind everything else, so that a caller whose operands need none may leave their bytes out)
 struct CeForward { int edge, parts, part; int64_t stats, score, sums, xs, ws, total; };
 CeForward ce_layout(int dtype, int64_t rows, int64_t classes, int64_t k)
 {
-    CeForward f;
+    CeForward f = {};
+    Few few;
+    f.sums = round256(16 * (ceil_div(rows, CE_ROWS) + FEW_BLOCKS));
+    f.total = f.sums;
+    if (few_layout(dtype, rows, classes, k, few)) return f;
     const int64_t big = ceil_div(rows, 128) * ceil_div(classes, 128);
     f.edge = big >= 1024 ? 256 : big >= 256 ? 128 : 64;
     const int64_t row_tiles = ceil_div(rows, f.edge), class_tiles = ceil_div(classes, f.edge);
@@ -1691,7 +1696,6 @@ CeForward ce_layout(int dtype, int64_t rows, int64_t classes, int64_t k)
     f.parts = (int)(class_tiles > 0 ? ceil_div(class_tiles, per) : 1);
     f.stats = round256(8 * rows * f.parts);
     f.score = round256(4 * rows);
-    f.sums = round256(16 * (ceil_div(rows, CE_ROWS) + FEW_BLOCKS));
     f.xs = round256(rows * padded(dtype, k) * elem_size(dtype));
     f.ws = round256(classes * padded(dtype, k) * elem_size(dtype));
     f.total = f.stats + f.score + f.sums + f.xs + f.ws;
@@ -1705,7 +1709,8 @@ int ce_forward_t(int dtype, const void *x, int64_t ldx, const void *w, int64_t l
     double *sums = (double *)ws;
     float *score = (float *)(ws + l.sums);
     float2 *stats = (float2 *)(ws + l.sums + l.score);
-    T *xs = (T *)(ws + l.sums + l.score + l.stats), *wsp = (T *)((char *)xs + l.xs);
+    const bool copy_x = !near_whole_rows(dtype, x, ldx, k), copy_w = !near_whole_rows(dtype, w, ldw, k);
+    T *xs = (T *)(ws + l.sums + l.score + l.stats), *wsp = (T *)((char *)xs + (copy_x ? l.xs : 0));
     int64_t blocks = 0;
     Few f;
     if (rows > 0 && few_layout(dtype, rows, classes, k, f)) {
@@ -1715,8 +1720,8 @@ int ce_forward_t(int dtype, const void *x, int64_t ldx, const void *w, int64_t l
     } else if (rows > 0) {
         blocks = ceil_div(rows, CE_ROWS);
         const int64_t kp = padded(dtype, k), row_tiles = ceil_div(rows, l.edge);
-        if (!near_whole_rows(dtype, x, ldx, k)) { copy_rows(x, ldx, nullptr, xs, kp, rows, rows, k, st); x = xs; ldx = kp; }
-        if (!near_whole_rows(dtype, w, ldw, k)) { copy_rows(w, ldw, nullptr, wsp, kp, classes, classes, k, st); w = wsp; ldw = kp; }
+        if (copy_x) { copy_rows(x, ldx, nullptr, xs, kp, rows, rows, k, st); x = xs; ldx = kp; }
+        if (copy_w) { copy_rows(w, ldw, nullptr, wsp, kp, classes, classes, k, st); w = wsp; ldw = kp; }
         const dim3 grid((unsigned)row_tiles, (unsigned)l.parts);
         const Operand<T> ow = op((const T *)w, ldw, classes), ox = op((const T *)x, ldx, rows);
 #define LAUNCH(EDGE, WM, WN)                                                                                                                \
@@ -1779,8 +1784,9 @@ int ce_backward_t(int dtype, const void *x, int64_t ldx, const void *w, int64_t 
         return status();
     }
     float *scale = (float *)ws, *coef = scale + 64, *tops = (float *)(ws + l.coef);
-    T *xs = (T *)(ws + l.coef + l.tops), *wsp = (T *)((char *)xs + l.xs), *g = (T *)((char *)wsp + l.ws);
+    T *xs = (T *)(ws + l.coef + l.tops), *g = (T *)((char *)xs + l.xs);
     float *acc = (float *)((char *)g + l.g), *part = (float *)((char *)acc + l.acc);
+    T *wsp = (T *)((char *)part + l.part);            // (last: see ce_layout)
     const int64_t kp = padded(dtype, k), blocks = ceil_div(rows, 256);
     if (blocks > 0)
         hipLaunchKernelGGL(k_ce_coefficients, dim3((unsigned)blocks), dim3(256), 0, st, dloss, stride, total, target, cw, ignore, (int)rows, (int)classes, coef, tops);

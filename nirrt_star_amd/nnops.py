@@ -229,6 +229,16 @@ def linear_act(x, weight, bias=None, residual=None, activation="none"):
 
 
 # ---- head with softmax cross entropy ---------------------------------------------------------------------------------------------------
+def _copy_not_made(t, ld):
+    """the bytes of a copy of the rows of t (n, k) that cross entropy of many classes leaves out of its workspaces where they lie in whole aligned
+    16-byte chunks, at most 4 MB apart (include/nirrt_nnops.h)"""
+    n, k = t.shape
+    e = t.element_size()
+    if n * k == 0 or t.data_ptr() % 16 or k * e % 16 or ld * e % 16 or ld * e > 1 << 22:
+        return 0
+    return (n * k * e + 255) & ~255
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, target, cw, ignore, mode):
@@ -240,7 +250,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
             nll = torch.empty(target.shape, dtype=torch.float32, device=x.device)
             total = torch.empty(3, dtype=torch.float32, device=x.device)
             L, dt = _lib(), _TYPES[x.dtype]
-            ws = _workspace(L.nirrt_nn_cross_entropy_workspace(dt, rows, v, k), x.device)
+            most = L.nirrt_nn_cross_entropy_workspace(dt, rows, v, k)
+            ws = _workspace(most - (_copy_not_made(x2, ldx) + _copy_not_made(w2, ldw) if v > 8 else 0), x.device)
             _check(L.nirrt_nn_cross_entropy(dt, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b), target.data_ptr(), _ptr(cw), ignore, lse.data_ptr(),
                                             nll.data_ptr(), total.data_ptr(), rows, v, k, _ptr(ws), _stream(x.device)), "cross_entropy")
         ctx.ignore, ctx.mode = ignore, mode
@@ -263,7 +274,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
             w2, ldw = _rows(w)
             dloss = dloss.float().contiguous()
             L, dt = _lib(), _TYPES[x.dtype]
-            ws = _workspace(L.nirrt_nn_cross_entropy_backward_workspace(dt, rows, v, k), x.device)
+            most = L.nirrt_nn_cross_entropy_backward_workspace(dt, rows, v, k)
+            ws = _workspace(most - (_copy_not_made(w2, ldw) if v > 8 else 0), x.device)
             _check(L.nirrt_nn_cross_entropy_backward(dt, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b), target.data_ptr(), _ptr(cw), ctx.ignore,
                                                      lse.data_ptr(), dloss.data_ptr(), 1 if ctx.mode == "none" else 0,
                                                      total.data_ptr() if ctx.mode == "mean" else None, _ptr(dx), _ptr(dw), _ptr(db), rows, v, k,

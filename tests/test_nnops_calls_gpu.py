@@ -229,3 +229,74 @@ def test_more_rows_and_columns_than_a_launch_has_small_tiles_for():
         assert torch.equal(got.double(), long[at].double() @ short.double().t())
         assert int((y != 0).sum()) == int((got != 0).sum())
         del x, w, long, short, y
+
+
+# ---- workspaces ----------------------------------------------------------------------------------------------------------------------------------
+def test_cross_entropy_holds_no_copies_that_are_not_made():
+    from nirrt_star_amd import nnops
+    g = gen(3)
+    rows, k, classes = 64, 512, 50000
+    x, w = randn((rows, k), g, torch.bfloat16).requires_grad_(True), randn((classes, k), g, torch.bfloat16, 0.05)
+    t = torch.randint(0, classes, (rows,), generator=g, device="cuda")
+
+    def more(call):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        held = torch.cuda.memory_allocated()
+        out = call()
+        torch.cuda.synchronize()
+        return torch.cuda.max_memory_allocated() - held, out
+
+    for weight in (w, w.detach()[:, :500]):                         # (51 MB each; rows of 1000 bytes are copied)
+        xx = x[:, :weight.shape[1]]
+        extra, loss = more(lambda: nnops.linear_cross_entropy(xx, weight, t))
+        assert extra < (4 << 20) + (0 if weight is w else 51 << 20)
+        extra, _ = more(lambda: torch.autograd.grad(loss, x))       # g' is rows x classes
+        assert extra < (4 << 20) + rows * classes * 2 + 32 * rows * k * 4 + (0 if weight is w else 51 << 20)
+    x2 = randn((1 << 20, 128), g, torch.float32)                    # two classes: sums of the workgroups only
+    extra, _ = more(lambda: nnops.linear_cross_entropy(x2, randn((2, 128), g, torch.float32), torch.zeros(1 << 20, dtype=torch.int64, device="cuda")))
+    assert extra < (8 << 20) + (1 << 20) * (8 + 4 + 8)
+
+
+@pytest.mark.parametrize("dt", [0, 1])
+@pytest.mark.parametrize("far_x", [False, True])
+@pytest.mark.parametrize("far_w", [False, True])
+def test_cross_entropy_workspaces_without_the_copies(dt, far_x, far_w):
+    """the C entry points with exactly the bytes they need, and marked bytes behind them that have to stay"""
+    from nirrt_star_amd import nnops
+    L = nnops._lib()
+    g = gen(dt)
+    T = TYPES[dt]
+    rows, k, classes = 300, 64, 700
+    x, w = randn((rows, k), g, T), randn((classes, k), g, T)
+    if far_x:
+        x = spread(x, 1 << 10, 1)
+    if far_w:
+        w = spread(w, 1 << 10, 1)
+    t = torch.randint(0, classes, (rows,), generator=g, device="cuda")
+    X, W = (r * k * T.itemsize + 255 & ~255 for r in (rows, classes))
+    st = torch.cuda.current_stream().cuda_stream
+
+    def space(nbytes):
+        return torch.full((nbytes + 4096,), 0x5a, dtype=torch.uint8, device="cuda")
+
+    def outs():
+        return (torch.empty(rows, 2, device="cuda"), torch.empty(rows, device="cuda"), torch.empty(3, device="cuda"), torch.empty(rows, k, dtype=T, device="cuda"),
+                torch.empty(classes, k, dtype=T, device="cuda"), torch.empty(classes, dtype=T, device="cuda"))
+
+    one = torch.ones((), device="cuda")
+    res = []
+    for short in (False, True):
+        lse, nll, total, dx, dw, db = o = outs()
+        n = L.nirrt_nn_cross_entropy_workspace(dt, rows, classes, k) - ((0 if far_x else X) + (0 if far_w else W) if short else 0)
+        ws = space(n)
+        assert L.nirrt_nn_cross_entropy(dt, x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), None, t.data_ptr(), None, -100, lse.data_ptr(), nll.data_ptr(),
+                                        total.data_ptr(), rows, classes, k, ws.data_ptr(), st) == 0
+        assert (ws[n:] == 0x5a).all()
+        n = L.nirrt_nn_cross_entropy_backward_workspace(dt, rows, classes, k) - ((0 if far_w else W) if short else 0)
+        ws = space(n)
+        assert L.nirrt_nn_cross_entropy_backward(dt, x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), None, t.data_ptr(), None, -100, lse.data_ptr(),
+                                                 one.data_ptr(), 0, total.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(), rows, classes, k, ws.data_ptr(), st) == 0
+        assert (ws[n:] == 0x5a).all()
+        res.append(o)
+    assert all(torch.equal(p, q) and torch.isfinite(p).all() for p, q in zip(*res))
