@@ -139,7 +139,7 @@ int nirrt_connect_round(const nirrt_connect_job *jobs, int n_jobs, double radius
 int nirrt_connect_masks(const nirrt_connect_job *jobs, int n_jobs, double radius, const int32_t *seed_idx, int device_id);
 
 /* atan2 / sin / cos (what math.atan2 / math.cos / math.sin of the reference's new_state, rrt_star_2d.py:67-78, and np.sin / np.cos of
- * irrt_star_3d.py:146-158 call) as the steer and the samplers get them: evaluated ON THE DEVICE to ~70 bits, the values whose rounding is
+ * irrt_star_3d.py:146-158 call) as the steer and the samplers get them: evaluated ON THE DEVICE to 66 bits and more, the values whose rounding is
  * not certain by a call of this host's libm.  fn 0 = atan2(a[i], b[i]), 1 = sin(a[i]), 2 = cos(a[i]); a, b, out HOST f64 (n,).  A caller
  * compares `out` with its own libm bit for bit before trusting the device-side steer / samplers on this host
  * (nirrt_star_amd/_hip.libm_check does, once per process): a difference means a libm that is more than 1/2 + 1/32 ulp off.  sin and

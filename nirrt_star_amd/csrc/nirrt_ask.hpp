@@ -1,6 +1,6 @@
 // nirrt_ask.hpp - a kernel's question to the host's libm.
 //
-// The reference steers with math.atan2 / math.cos / math.sin of its host.  The device evaluates these functions itself to ~70 bits
+// The reference steers with math.atan2 / math.cos / math.sin of its host.  The device evaluates these functions itself to 66 bits and more
 // (glibc235_libm.inc) and knows the libm's result unless the true value lies next to a rounding border; then the wave asks: it draws a
 // ticket, writes (function, arguments) into the ticket's slot in pinned host memory and waits for the reply, which the host thread that
 // waits for the launch writes after CALLING its libm (ask_wait below instead of hipStreamSynchronize).  About 2.6 % of the 2D steers

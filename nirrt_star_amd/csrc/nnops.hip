@@ -242,7 +242,8 @@ constexpr unsigned NOWHERE = 0x7ffffff0u;   // an offset beyond every buffer (di
 
 // 16 bytes per lane from buffer + offset to lds + 16 lane.  Written out, because the compiler does not know which part of the LDS a load of its
 // own writes, and would wait for all of them before every read.  It has no result register; the waits are arrive() below, which every use of
-// the LDS stands behind.
+// the LDS stands behind.  m0 is a reserved register: the compiler keeps no value in it and writes it right before a use of its own, of which
+// these kernels have none (naming it as clobbered is answered with a warning and changes nothing).
 __device__ __forceinline__ void load_to_lds(u32x4 buffer, const u32x4 *lds, unsigned offset)
 {
 #ifdef __HIP_DEVICE_COMPILE__
@@ -526,7 +527,7 @@ __device__ __forceinline__ void tile_of(int id, int count, int tiles_i, int tile
 
 // ---- activations ---------------------------------------------------------------------------------------------------------------
 // Phi(z) and e = exp(-z^2 / 2) (its density is 0.3989 e): Phi(-|z|) = 1/2 erfcx(|z| / sqrt 2) e, erfcx as a polynomial of degree 9 in
-// t = 1 / (1 + 0.3 x) (weighted least squares on x in [0, 14]: relative error 4e-8; behind it e is 0).  A sixth of erfcf's instructions.
+// t = 1 / (1 + 0.3 x) (weighted least squares on x in [0, 14]: relative error 6.5e-8; behind it e is 0).  A sixth of erfcf's instructions.
 __device__ __forceinline__ float normal_cdf(float z, float &e)
 {
     const float a = __builtin_fabsf(z);
@@ -583,7 +584,8 @@ template <class T> __device__ __forceinline__ void store4(T *p, f32x4 v, int n)
     for (int e = 0; e < 4; e++) q.e[e] = (T)v[e];
     store_some(p, q, n);
 }
-// y = act(C + b[j]) + r, and z
+// y = act(C + b[j]) + r, and z in the element type, as y is: half the bytes for 16-bit types, and gradients that move by 6e-4 of themselves in
+// bf16 (2-norms, 4097 x 321 x 515 and 4096 x 4096 x 4096), where the rounding of a result is 1.7e-3
 template <class T> struct EpiLinear {
     const T *b, *r;
     T *y, *z;
@@ -771,7 +773,9 @@ template <class Epi> __global__ __launch_bounds__(256) void k_join(const float *
 
 // ---- dz = dy act'(z) and its column sums -------------------------------------------------------------------------------------------
 // grid (column blocks, row chunks).  A row's 16-byte packs lie on `lanes` (a power of two) neighbouring lanes, 256 / lanes rows at a time;
-// a lane keeps the sums of its columns over the chunk, the rows' lanes meet in the LDS: sums (chunk, column), joined by k_column_join.  Bound by
+// a lane keeps the sums of its columns over the chunk, the rows' lanes meet in the LDS: sums (chunk, column), joined by k_column_join.  The sums take
+// dz in 32 bits; what is stored is rounded to the element type, which is what 16-bit MFMA multiplies: dx and dw are 2.4e-3 off in bf16 (2-norm,
+// sizes as above; 1.7e-3 is the rounding of the result alone), and in f16 a dy above 65504 / 1.13 may become infinite.  Bound by
 // memory: 16384 x 4096 in bf16 93 us (4.3 TB/s; 106 with one row's loads at a time).
 template <class T>
 __global__ __launch_bounds__(256) void k_dz(const T *z, const T *dy, int64_t lddy, T *dz, int64_t lddz, float *sums, int m, int n, int chunk, int lanes, int act)
@@ -1049,10 +1053,10 @@ __global__ __launch_bounds__(256) void k_ce_scale(const float *tops, int blocks,
 }
 // g' = c_r / scale (exp(l - lse_r) - [v = target]), lse in its two parts, FACTOR in the element type, stored (v, r): the product C[v, r] again.  16-bit products
 // need 16-bit operands; c / scale <= 1 keeps the range, and FACTOR 4096 in f16 lifts probabilities of large vocabularies (1e-5) out of
-// its subnormals.  A rounding is off by 2^-8 (bf16), 2^-11 (f16) of the element at most, like the rounding of dz in the linear layer.
-// The scores are multiplied out again rather than kept: at 1024 inputs in bf16 that costs 2 ps per score, writing and reading them in 32 bits
-// 1.6; in fp32 it costs 15 fs per input and score, so a head of many inputs pays for the memory it saves (991 x 1703 x 1320: 290 us
-// against 232 of the elementary form).
+// its subnormals.  A rounding is off by 2^-8 (bf16), 2^-11 (f16) of the element at most, like the rounding of dz in the linear layer; db is the
+// sum of the rounded g'.  The scores are multiplied out again rather than kept between the passes, where rows x classes in 32 bits would
+// lie; g' itself is whole up to G_ELEMS elements at a time.  That is no saving of time: at 1024 inputs in bf16 it costs 2 ps per score, writing
+// and reading them 1.6, and in fp32 15 fs per input and score (991 x 1703 x 1320: 290 us against 232 of the elementary form, for 5 MB).
 template <class T> struct Factor { static constexpr float VALUE = 1.f; };
 template <> struct Factor<f16_t> { static constexpr float VALUE = 4096.f; };
 template <class T> struct EpiSoftmaxGrad {
@@ -1674,7 +1678,10 @@ bool few_layout(int dtype, int64_t rows, int64_t classes, int64_t k, Few &f)
     } while (0)
 #define FEW_ONE(KERNEL, V, NC, BLOCKS, LDS, ...) hipLaunchKernelGGL((KERNEL<T, V, NC>), dim3((unsigned)BLOCKS), dim3(256), LDS, st, __VA_ARGS__)
 
-// cross entropy: tile edge, and parts of the classes so that row tiles x parts fill the GPU; x and w whose rows are no whole aligned chunks
+// cross entropy: tile edge by the number of 128 x 128 tiles, and parts of the classes so that row tiles x parts fill the GPU.  us of the forward
+// pass at edge 64 / 128 / 256, 1024 inputs, bf16: 128 tiles 20.8 / 24.2 / 32.9, 256 tiles 32.0 / 26.3 / 34.7, 512 tiles 49.4 / 32.0 / 35.1, 1024
+// tiles 88.8 / 51.7 / 40.0, 4096 tiles 331 / 176 / 129; fp32: 53.8 / 77.5 / 247, 98.2 / 80.6 / 245, 170 / 138 / 246, 331 / 264 / 251, 1296 / 1028 / 975.
+// x and w whose rows are no whole aligned chunks
 // or lie far apart are copied into such that are not (k_rows_copy): the products read them many times
 // (the copies lie behind everything else, so that a caller whose operands need none may leave their bytes out)
 struct CeForward { int edge, parts, part; int64_t stats, score, sums, xs, ws, total; };

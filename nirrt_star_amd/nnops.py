@@ -6,7 +6,10 @@
     grad_norm             2-norm over many tensors
     clip_grad_norm_       the same, and the clipping by it (in place, or into other tensors)
 
-float32, bfloat16 and float16; sums are held in 32 bits and rounded once.  Tensors must live on the GPU (a CPU tensor is an error,
+float32, bfloat16 and float16; sums are held in 32 bits and rounded once.  In 16 bits the backward passes have roundings of their own: the
+pre-activation is kept in the tensors' type, and the gradient in front of a product (dz, or probability minus target) is rounded to it, as
+matrix instructions multiply 16-bit operands - dx and dW are 2.4e-3 off in bfloat16 (2-norm) where the rounding of the result alone is
+1.7e-3, and a float16 gradient above 5.8e4 may overflow in dz.  Tensors must live on the GPU (a CPU tensor is an error,
 there is no other implementation); rows may have any stride, other layouts are copied.  Results are the same bits for the same input
 (no atomics).  Backward passes are differentiable once; there is no forward mode, and a call cannot be traced (torch.jit.trace, make_fx):
 both are refused.
@@ -93,7 +96,8 @@ def _not_recorded(name):
 
 def _need(name, first, **others):
     """one device (a GPU) and one element type for all of them"""
-    _not_recorded(name)
+    if _is_tracing() or _dispatch_modes():
+        _not_recorded(name)
     if not first.is_cuda:
         raise RuntimeError("nirrt_star_amd.nnops.%s got a CPU tensor: the package only has the HIP kernels (move it to 'cuda')" % name)
     if first.dtype not in _TYPES:

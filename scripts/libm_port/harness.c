@@ -9,15 +9,9 @@
 static int g_unsupported = 0;
 static inline double D(uint64_t u) { double d; memcpy(&d, &u, 8); return d; }
 static inline uint64_t B(double d) { uint64_t u; memcpy(&u, &d, 8); return u; }
-#define DB(u) D(u)
-#define LIBM_CONST(name, val) static const uint64_t name = val;
 #define LIBM_TABLE(name, n) static const uint64_t name[n]
 #define LIBM_FN static
 #define UNSUPPORTED(msg) do { g_unsupported++; return NAN; } while (0)
-#define S64(off) stk[(off) / 8]
-#define W64(off, v) (stk[(off) / 8] = (v))
-#define S32(off) ((uint32_t)(stk[(off) / 8] >> (((off) & 4) * 8)))
-#define W32(off, v) (stk[(off) / 8] = (stk[(off) / 8] & ~(0xffffffffull << (((off) & 4) * 8))) | ((uint64_t)(uint32_t)(v) << (((off) & 4) * 8)))
 static inline uint64_t LD64(int64_t a);
 // (a question to the libm counts)
 static long g_asked = 0;
@@ -27,7 +21,6 @@ static double ask_c(double x) { g_asked++; return cos(x); }
 #define LIBM_ASK_ATAN2(y, x) ask2(y, x)
 #define LIBM_ASK_SIN(x) ask_s(x)
 #define LIBM_ASK_COS(x) ask_c(x)
-#define LD32(a) ((uint32_t)LD64(a))
 #include "../../nirrt_star_amd/csrc/glibc235_libm.inc"
 
 static inline uint64_t LD64(int64_t a)
