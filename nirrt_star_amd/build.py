@@ -74,34 +74,44 @@ def optional_flags(hipcc):
     return _optional
 
 
-def _compile(so, extra, verbose):
-    """the sources side by side, then one link"""
+def _compile(libs, verbose):
+    """libs: (library, its own flags) each; all sources of all of them side by side, then a link each"""
     import tempfile
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     tree = TREE + optional_flags(hipcc)
     with tempfile.TemporaryDirectory() as d:
-        objs, jobs = [], []
-        for src in SOURCES:
-            name = os.path.basename(src)
-            objs.append(os.path.join(d, name + ".o"))
-            cmd = [hipcc] + COMMON + ([] if name in PLAIN else tree) + extra + ["-c", "-o", objs[-1], src]
-            if verbose:
-                print(" ".join(cmd))
-            jobs.append((cmd, subprocess.Popen(cmd)))
-        for cmd, job in jobs:
-            if job.wait() != 0:
-                for _, other in jobs:
-                    other.wait()
-                raise subprocess.CalledProcessError(job.returncode, cmd)
-        subprocess.check_call([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", so] + objs)
+        jobs = {}
+        objs = []
+        for extra in (flags for _, flags in libs):
+            objs.append([])
+            for src in SOURCES:
+                name = os.path.basename(src)
+                # (the plain sources know none of the tests' small limits: one object serves both libraries)
+                flags = tuple(COMMON + (extra if extra != SMALL_FLAGS else []) if name in PLAIN else COMMON + tree + extra) + (src,)
+                if flags not in jobs:
+                    out = os.path.join(d, "%d.o" % len(jobs))
+                    cmd = [hipcc] + list(flags[:-1]) + ["-c", "-o", out, src]
+                    if verbose:
+                        print(" ".join(cmd))
+                    jobs[flags] = (out, cmd, subprocess.Popen(cmd))
+                objs[-1].append(jobs[flags][0])
+        codes = [(job.wait(), cmd) for _, cmd, job in jobs.values()]
+        for code, cmd in codes:
+            if code != 0:
+                raise subprocess.CalledProcessError(code, cmd)
+        for (so, _), o in zip(libs, objs):
+            subprocess.check_call([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", so] + o)
 
 
 def build(force=False, verbose=False, small=True):
-    """Compile libnirrt_hip.so (and the small-limits test build) when a source is newer than the library."""
+    """Compile libnirrt_hip.so (and the small-limits test build) when a source is newer than the library, or always (force)."""
+    libs = []
     if force or needs_build(SO):
-        _compile(SO, os.environ.get("NIRRT_EXTRA_FLAGS", "").split(), verbose)
+        libs.append((SO, os.environ.get("NIRRT_EXTRA_FLAGS", "").split()))
     if small and (force or needs_build(SO_SMALL)):
-        _compile(SO_SMALL, SMALL_FLAGS, verbose)
+        libs.append((SO_SMALL, SMALL_FLAGS))
+    if libs:
+        _compile(libs, verbose)
     return SO
 
 
