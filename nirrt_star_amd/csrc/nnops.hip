@@ -1617,7 +1617,7 @@ int linear_backward_t(int dtype, int act, const void *x, int64_t ldx, const void
     const LinearBackward l = linear_backward_layout(dtype, act, x, ldx, w, ldw, dy, lddy, m, n, k, dx != nullptr, dw != nullptr);
     T *dz = (T *)ws, *xs = (T *)(ws + l.dz), *wsp = (T *)((char *)xs + l.xs);
     float *sums = (float *)((char *)wsp + l.ws), *part = (float *)((char *)sums + l.sums);
-    if (l.own_dz || db) {
+    if (n > 0 && (l.own_dz || db)) {                  // (no columns: no dz and no db, and dx is zero)
         const Columns c = columns(dtype, m, n);
         if (m > 0)
             hipLaunchKernelGGL((k_dz<T>), dim3((unsigned)c.blocks, (unsigned)c.parts), dim3(256), 0, st, (const T *)z, (const T *)dy, lddy,

@@ -292,7 +292,7 @@ def linear_cross_entropy(x, weight, target, bias=None, class_weight=None, ignore
     target int64 (...), bias (classes,), class_weight float32 (classes,).  Rows whose target is ignore_index count for nothing (their
     gradients are zero, whatever they hold); any other target outside [0, classes) gives NaN.  reduction: "mean" = sum of weight x loss
     over the sum of weights (NaN if no row counts), "sum", or "none" (the shape of target); the loss is float32.  Gradients for x, weight
-    and bias."""
+    and bias; in float16 they are held relative to the largest dloss x weight of the call, so that rows with 1e-9 of it and less lose digits."""
     name = "linear_cross_entropy"
     if reduction not in ("mean", "sum", "none"):
         raise ValueError("%s: reduction %r is not mean, sum or none" % (name, reduction))

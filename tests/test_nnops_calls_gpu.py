@@ -300,3 +300,31 @@ def test_cross_entropy_workspaces_without_the_copies(dt, far_x, far_w):
         assert (ws[n:] == 0x5a).all()
         res.append(o)
     assert all(torch.equal(p, q) and torch.isfinite(p).all() for p, q in zip(*res))
+
+
+def test_c_backward_of_a_layer_without_outputs():
+    """n = 0 through the C entry: dx is zero, dw and db are empty"""
+    from nirrt_star_amd import nnops
+    L = nnops._lib()
+    x, dx = torch.randn(40, 16, device="cuda"), torch.full((40, 16), 7.0, device="cuda")
+    for act in range(4):
+        need = L.nirrt_nn_linear_backward_workspace(0, act, x.data_ptr(), 16, None, 16, None, 0, 40, 0, 16)
+        ws = torch.empty(max(need, 256), dtype=torch.uint8, device="cuda")
+        for db in (None, ws.data_ptr()):
+            dx.fill_(7.0)
+            assert L.nirrt_nn_linear_backward(0, act, x.data_ptr(), 16, None, 16, None, None, 0, dx.data_ptr(), ws.data_ptr(), db, 40, 0, 16, ws.data_ptr(),
+                                              torch.cuda.current_stream().cuda_stream) == 0
+            assert (dx == 0).all()
+
+
+@pytest.mark.parametrize("classes", [5, 30])
+def test_cross_entropy_without_inputs_has_a_bias_gradient(classes):
+    from nirrt_star_amd import nnops
+    g = gen(classes)
+    b = randn((classes,), g, torch.float32).requires_grad_(True)
+    x, w = torch.zeros(20, 0, device="cuda", requires_grad=True), torch.zeros(classes, 0, device="cuda", requires_grad=True)
+    t = torch.randint(0, classes, (20,), generator=g, device="cuda")
+    dx, dw, db = torch.autograd.grad(nnops.linear_cross_entropy(x, w, t, bias=b, reduction="sum"), (x, w, b))
+    want = 20 * torch.softmax(b.detach().double(), 0) - torch.bincount(t, minlength=classes)
+    # 20 terms below 1, each off by a few 2^-24 (exp, lse), and their sum
+    assert dx.shape == x.shape and dw.shape == w.shape and (db.double() - want).abs().max() <= 20 * 64 * 2.0 ** -24
