@@ -145,7 +145,7 @@ def _workspace(nbytes, device):
 
 
 def _sizes_ok(name, *dims):
-    if any(d > _DIM_MAX for d in dims):
+    if max(dims) > _DIM_MAX:
         raise ValueError("%s: a dimension of %d is beyond %d" % (name, max(dims), _DIM_MAX))
 
 
@@ -233,31 +233,30 @@ def linear_act(x, weight, bias=None, residual=None, activation="none"):
 
 
 # ---- head with softmax cross entropy ---------------------------------------------------------------------------------------------------
-def _copy_not_made(t, ld):
-    """the bytes of a copy of the rows of t (n, k) that cross entropy of many classes leaves out of its workspaces where they lie in whole aligned
+def _copy_not_made(address, n, row, apart):
+    """the bytes of a copy of n rows of `row` bytes that cross entropy of many classes leaves out of its workspaces where they lie in whole aligned
     16-byte chunks, at most 4 MB apart (include/nirrt_nnops.h)"""
-    n, k = t.shape
-    e = t.element_size()
-    if n * k == 0 or t.data_ptr() % 16 or k * e % 16 or ld * e % 16 or ld * e > 1 << 22:
-        return 0
-    return (n * k * e + 255) & ~255
+    return 0 if (address | row | apart) & 15 or apart > 1 << 22 else (n * row + 255) & ~255
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, target, cw, ignore, mode):
-        rows, v, k = target.numel(), w.shape[0], w.shape[1]
-        with _on(x.device):
+        rows, (v, k), dev, dtype = target.numel(), w.shape, x.device, x.dtype
+        with _on(dev):
             x2, ldx = _rows(x)
             w2, ldw = _rows(w)
-            lse = torch.empty(rows, 2, dtype=torch.float32, device=x.device)
-            nll = torch.empty(target.shape, dtype=torch.float32, device=x.device)
-            total = torch.empty(3, dtype=torch.float32, device=x.device)
-            L, dt = _lib(), _TYPES[x.dtype]
+            lse = torch.empty(rows, 2, dtype=torch.float32, device=dev)
+            nll = torch.empty(target.shape, dtype=torch.float32, device=dev)
+            total = torch.empty(3, dtype=torch.float32, device=dev)
+            L, dt, px, pw = _lib(), _TYPES[dtype], x2.data_ptr(), w2.data_ptr()
             most = L.nirrt_nn_cross_entropy_workspace(dt, rows, v, k)
-            ws = _workspace(most - (_copy_not_made(x2, ldx) + _copy_not_made(w2, ldw) if v > 8 else 0), x.device)
-            _check(L.nirrt_nn_cross_entropy(dt, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b), target.data_ptr(), _ptr(cw), ignore, lse.data_ptr(),
-                                            nll.data_ptr(), total.data_ptr(), rows, v, k, _ptr(ws), _stream(x.device)), "cross_entropy")
+            if v > 8:
+                e = 2 if dt else 4
+                most -= _copy_not_made(px, rows, k * e, ldx * e) + _copy_not_made(pw, v, k * e, ldw * e)
+            ws = _workspace(most, dev)
+            _check(L.nirrt_nn_cross_entropy(dt, px, ldx, pw, ldw, _ptr(b), target.data_ptr(), _ptr(cw), ignore, lse.data_ptr(),
+                                            nll.data_ptr(), total.data_ptr(), rows, v, k, _ptr(ws), _stream(dev)), "cross_entropy")
         ctx.ignore, ctx.mode = ignore, mode
         ctx.save_for_backward(x, w, b, target, cw, lse, total)
         # (.data: no view of `total` for autograd, with a version of its own, so that a caller may scale or add to the loss in place; of
@@ -268,22 +267,25 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
         x, w, b, target, cw, lse, total = ctx.saved_tensors
-        rows, v, k = target.numel(), w.shape[0], w.shape[1]
+        rows, (v, k), dev, dtype = target.numel(), w.shape, x.device, x.dtype
         need = ctx.needs_input_grad
-        with _on(x.device):
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
-            dw = torch.empty(v, k, dtype=x.dtype, device=x.device) if need[1] else None
-            db = torch.empty(v, dtype=x.dtype, device=x.device) if need[2] else None
+        with _on(dev):
+            dx = torch.empty(x.shape, dtype=dtype, device=dev) if need[0] else None
+            dw = torch.empty(v, k, dtype=dtype, device=dev) if need[1] else None
+            db = torch.empty(v, dtype=dtype, device=dev) if need[2] else None
             x2, ldx = _rows(x)
             w2, ldw = _rows(w)
             dloss = dloss.float().contiguous()
-            L, dt = _lib(), _TYPES[x.dtype]
+            L, dt, pw = _lib(), _TYPES[dtype], w2.data_ptr()
             most = L.nirrt_nn_cross_entropy_backward_workspace(dt, rows, v, k)
-            ws = _workspace(most - (_copy_not_made(w2, ldw) if v > 8 else 0), x.device)
-            _check(L.nirrt_nn_cross_entropy_backward(dt, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b), target.data_ptr(), _ptr(cw), ctx.ignore,
+            if v > 8:
+                e = 2 if dt else 4
+                most -= _copy_not_made(pw, v, k * e, ldw * e)
+            ws = _workspace(most, dev)
+            _check(L.nirrt_nn_cross_entropy_backward(dt, x2.data_ptr(), ldx, pw, ldw, _ptr(b), target.data_ptr(), _ptr(cw), ctx.ignore,
                                                      lse.data_ptr(), dloss.data_ptr(), 1 if ctx.mode == "none" else 0,
                                                      total.data_ptr() if ctx.mode == "mean" else None, _ptr(dx), _ptr(dw), _ptr(db), rows, v, k,
-                                                     _ptr(ws), _stream(x.device)), "cross_entropy_backward")
+                                                     _ptr(ws), _stream(dev)), "cross_entropy_backward")
         return dx, dw, db, None, None, None, None
 
 
@@ -292,7 +294,7 @@ def linear_cross_entropy(x, weight, target, bias=None, class_weight=None, ignore
     target int64 (...), bias (classes,), class_weight float32 (classes,).  Rows whose target is ignore_index count for nothing (their
     gradients are zero, whatever they hold); any other target outside [0, classes) gives NaN.  reduction: "mean" = sum of weight x loss
     over the sum of weights (NaN if no row counts), "sum", or "none" (the shape of target); the loss is float32.  Gradients for x, weight
-    and bias; in float16 they are held relative to the largest dloss x weight of the call, so that rows with 1e-9 of it and less lose digits."""
+    and bias; in float16 they are held relative to the largest dloss x weight of the call, so that rows with 1e-8 of it and less lose digits."""
     name = "linear_cross_entropy"
     if reduction not in ("mean", "sum", "none"):
         raise ValueError("%s: reduction %r is not mean, sum or none" % (name, reduction))
@@ -307,11 +309,12 @@ def linear_cross_entropy(x, weight, target, bias=None, class_weight=None, ignore
     if class_weight is not None and (class_weight.dtype != torch.float32 or class_weight.device != x.device or tuple(class_weight.shape) != (v,)
                                      or class_weight.requires_grad):
         raise ValueError("%s: class_weight must be float32 (%d,) on %s, without a gradient" % (name, v, x.device))
-    _sizes_ok(name, target.numel(), v, weight.shape[1])
-    if weight.shape[1] * weight.element_size() > 1 << 22:
-        raise ValueError("%s: %d inputs are more than 4 MB" % (name, weight.shape[1]))
-    if v > 8 and target.numel() >= 1 << 29:
-        raise ValueError("%s: %d rows of more than 8 classes" % (name, target.numel()))
+    rows, k = target.numel(), weight.shape[1]
+    _sizes_ok(name, rows, v, k)
+    if k > (1 << 20 if x.dtype is torch.float32 else 1 << 21):
+        raise ValueError("%s: %d inputs are more than 4 MB" % (name, k))
+    if v > 8 and rows >= 1 << 29:
+        raise ValueError("%s: %d rows of more than 8 classes" % (name, rows))
     return _LinearCrossEntropy.apply(x, weight, bias.contiguous() if bias is not None else None, target.contiguous(),
                                      class_weight.contiguous() if class_weight is not None else None, int(ignore_index), reduction)
 
